@@ -341,6 +341,131 @@ int actcomp_nf4_dequant(const uint8_t *packed, int64_t n, int64_t blocksize, con
                         const float *absmax, const uint8_t *absmax_q, const float *absmax2,
                         const float *code2, int64_t blocksize2, const float *offset, uint16_t *out, void *stream);
 
+/* ========================================================= residual branch
+ * Dropout without a stored mask, layer norm with its backward pass, and both
+ * across a residual branch.  No reference counterpart: they are what a training
+ * step runs between the linear layers of low_rank_system_profile_backward.py.
+ * dtype of the activations: 0 = float32, 1 = bf16, 2 = fp16; wdtype of weight,
+ * bias and their gradients: the activations' or 0 = float32.  Activations are
+ * rows x cols with unit column stride and row strides ld* in elements (any
+ * alignment of the type; 16-byte aligned rows of cols % 8 == 0 take the wide
+ * path).  rows may be 0.
+ *
+ * The mask: value (r, c) is kept iff half >= T, T = round(p * 65536) (p in
+ * [0, 1], held to 16 bits), half = the (c & 7)-th 16-bit half of Philox4x32-10
+ * at counter (c >> 3, 0, low 32 bits of R, high 32 bits of R), R = row_offset +
+ * r, keyed by the seed; kept values are scaled by 65536 / (65536 - T), others
+ * are 0 whatever they held (p = 1: all).  The backward pass draws the same mask
+ * from the same seed, rows and columns; a shard of the rows draws its part of
+ * the whole's mask when row_offset counts its first row.  seed_ptr, if not
+ * NULL, is 8 bytes of device memory read by the kernel in place of seed (a
+ * captured graph draws a new mask when the word is changed between replays). */
+typedef struct actcomp_drop_args {
+    int64_t rows, cols;
+    const void *x;
+    int64_t ldx;
+    void *y;
+    int64_t ldy;
+    int32_t dtype, reserved;
+    double p;
+    uint64_t seed;
+    const uint64_t *seed_ptr;
+    uint64_t row_offset;
+} actcomp_drop_args;
+/* y = dropout(x); also the backward pass, on the gradient.  y may be x. */
+int actcomp_dropout(const actcomp_drop_args *a, void *stream);
+
+/* Layer norm of each row: y = (h - mean) * rstd * weight + bias, mean and rstd =
+ * 1 / sqrt(var + eps) in float32 (rows each).  res == NULL: h = x.  Otherwise
+ * h = res + dropout(x), written to h, and y normalises the unrounded float32 sum.
+ * weight / bias may be NULL (1 / 0). */
+typedef struct actcomp_ln_args {
+    int64_t rows, cols;
+    const void *x;
+    int64_t ldx;
+    const void *res;
+    int64_t ldr;
+    const void *weight, *bias;
+    void *y;
+    int64_t ldy;
+    void *h;
+    int64_t ldh;
+    float *mean, *rstd;
+    int32_t dtype, wdtype;
+    float eps;
+    int32_t reserved;
+    double p;
+    uint64_t seed;
+    const uint64_t *seed_ptr;
+    uint64_t row_offset;
+} actcomp_ln_args;
+int actcomp_layer_norm(const actcomp_ln_args *a, void *stream);
+
+/* Backward of actcomp_layer_norm from dy, the normalised input x (h in the fused
+ * form), mean and rstd.  dr == NULL: dx is the input's gradient.  Otherwise dr =
+ * layer norm's gradient (+ dh, the gradient that h receives from elsewhere, if not
+ * NULL) is the residual's and dx = dropout(dr) the dropped input's.  dweight and
+ * dbias may be NULL; their sums over rows run in a fixed order (repeat calls give
+ * the same bits).  workspace: actcomp_layer_norm_bwd_workspace() bytes, 16-byte
+ * aligned, uninitialised. */
+typedef struct actcomp_ln_bwd_args {
+    int64_t rows, cols;
+    const void *dy;
+    int64_t lddy;
+    const void *x;
+    int64_t ldx;
+    const void *dh;
+    int64_t lddh;
+    const void *weight;
+    const float *mean, *rstd;
+    void *dx;
+    int64_t lddx;
+    void *dr;
+    int64_t lddr;
+    void *dweight, *dbias;
+    int32_t dtype, wdtype;
+    double p;
+    uint64_t seed;
+    const uint64_t *seed_ptr;
+    uint64_t row_offset;
+} actcomp_ln_bwd_args;
+size_t actcomp_layer_norm_bwd_workspace(int64_t rows, int64_t cols);
+int actcomp_layer_norm_bwd(const actcomp_ln_bwd_args *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ========================================================= microscaled 4-bit
+ * A rows x cols matrix in 4-bit floating point with one power-of-two scale per
+ * 32 consecutive values of a row (OCP Microscaling, MXFP4).  No reference
+ * counterpart: the framework's integer codes (cg) feed no 4-bit tensor cores.
+ *   codes   rows x ceil(cols / 32) * 16 bytes: e2m1 values (sign, 2 exponent
+ *           bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), column 2j in the
+ *           low nibble; columns past cols are 0
+ *   scales  ceil(rows / 128) * ceil(cols / 128) * 512 bytes: byte of (row r,
+ *           block b of 32 columns) at ((r / 128) * ceil(cols / 128) + b / 4) *
+ *           512 + (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4 (the layout the
+ *           tensor cores read); value 2^(byte - 127), 255 = NaN; places past
+ *           rows or cols hold 0
+ * A value is its code times its block's scale.  Quantisation: scale exponent
+ * max(floor(log2 amax) - 2, -127) over the block's values, code = value / scale
+ * to the nearest, ties to even, magnitudes past 6 to 6; a block that holds a NaN
+ * or an infinity gets scale 255 (all its values read as NaN).  Both buffers are
+ * 16-byte aligned.  rows and cols are at least 1. */
+typedef struct actcomp_mx4 {
+    int64_t rows, cols;
+    uint8_t *codes;
+    uint8_t *scales;
+} actcomp_mx4;
+size_t actcomp_mx4_code_bytes(int64_t rows, int64_t cols);
+size_t actcomp_mx4_scale_bytes(int64_t rows, int64_t cols);
+/* Quantise x (rows x cols, dtype 0 = float32, 1 = bf16, 2 = fp16, row stride ldx):
+ * q = x by rows (q->rows == rows), qt = x^T (qt->rows == cols), each may be NULL. */
+int actcomp_mx4_quantize(const void *x, int64_t rows, int64_t cols, int64_t ldx, int32_t dtype, const actcomp_mx4 *q,
+                         const actcomp_mx4 *qt, void *stream);
+/* The values of q as rows x cols of `dtype` (row stride ldo). */
+int actcomp_mx4_dequantize(const actcomp_mx4 *q, void *out, int64_t ldo, int32_t dtype, void *stream);
+/* c = a . b^T (a->rows x b->rows, row stride ldc), a->cols == b->cols, float32
+ * accumulation on the tensor cores; c_dtype 0 = float32, 1 = bf16, 2 = fp16. */
+int actcomp_mx4_gemm(const actcomp_mx4 *a, const actcomp_mx4 *b, void *c, int64_t ldc, int32_t c_dtype, void *stream);
+
 /* Error statistics of a reconstruction against its original (n bf16 values):
  * out[0] += sum (a-b)^2, out[1] += sum b^2, out[2] = max(out[2], max|a-b|),
  * out[3] += count(a != b); out: 4 doubles of device memory (accumulated into,

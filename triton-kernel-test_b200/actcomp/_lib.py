@@ -82,6 +82,37 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+class DropArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("cols", c_i64), ("x", c_vp), ("ldx", c_i64), ("y", c_vp), ("ldy", c_i64),
+        ("dtype", c_i32), ("reserved", c_i32), ("p", ctypes.c_double), ("seed", ctypes.c_uint64),
+        ("seed_ptr", c_vp), ("row_offset", ctypes.c_uint64),
+    ]
+
+
+class LnArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("cols", c_i64), ("x", c_vp), ("ldx", c_i64), ("res", c_vp), ("ldr", c_i64),
+        ("weight", c_vp), ("bias", c_vp), ("y", c_vp), ("ldy", c_i64), ("h", c_vp), ("ldh", c_i64),
+        ("mean", c_vp), ("rstd", c_vp), ("dtype", c_i32), ("wdtype", c_i32), ("eps", ctypes.c_float),
+        ("reserved", c_i32), ("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("seed_ptr", c_vp),
+        ("row_offset", ctypes.c_uint64),
+    ]
+
+
+class LnBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("cols", c_i64), ("dy", c_vp), ("lddy", c_i64), ("x", c_vp), ("ldx", c_i64),
+        ("dh", c_vp), ("lddh", c_i64), ("weight", c_vp), ("mean", c_vp), ("rstd", c_vp), ("dx", c_vp), ("lddx", c_i64),
+        ("dr", c_vp), ("lddr", c_i64), ("dweight", c_vp), ("dbias", c_vp), ("dtype", c_i32), ("wdtype", c_i32),
+        ("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("seed_ptr", c_vp), ("row_offset", ctypes.c_uint64),
+    ]
+
+
+class Mx4Desc(ctypes.Structure):
+    _fields_ = [("rows", c_i64), ("cols", c_i64), ("codes", c_vp), ("scales", c_vp)]
+
+
 #: entry point -> (restype, argtypes); mirrors include/actcomp.h
 SIGNATURES = {
     "actcomp_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -116,6 +147,16 @@ SIGNATURES = {
     "actcomp_error_stats": (ctypes.c_int, [c_vp, c_vp, c_i64, c_vp, c_vp]),
     "actcomp_nf4_dequant": (ctypes.c_int, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
                                            c_vp, c_vp, c_vp]),
+    "actcomp_dropout": (ctypes.c_int, [ctypes.POINTER(DropArgs), c_vp]),
+    "actcomp_layer_norm": (ctypes.c_int, [ctypes.POINTER(LnArgs), c_vp]),
+    "actcomp_layer_norm_bwd_workspace": (ctypes.c_size_t, [c_i64, c_i64]),
+    "actcomp_layer_norm_bwd": (ctypes.c_int, [ctypes.POINTER(LnBwdArgs), c_vp, ctypes.c_size_t, c_vp]),
+    "actcomp_mx4_code_bytes": (ctypes.c_size_t, [c_i64, c_i64]),
+    "actcomp_mx4_scale_bytes": (ctypes.c_size_t, [c_i64, c_i64]),
+    "actcomp_mx4_quantize": (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_i32, ctypes.POINTER(Mx4Desc),
+                                            ctypes.POINTER(Mx4Desc), c_vp]),
+    "actcomp_mx4_dequantize": (ctypes.c_int, [ctypes.POINTER(Mx4Desc), c_vp, c_i64, c_i32, c_vp]),
+    "actcomp_mx4_gemm": (ctypes.c_int, [ctypes.POINTER(Mx4Desc), ctypes.POINTER(Mx4Desc), c_vp, c_i64, c_i32, c_vp]),
 }
 
 _lock = threading.Lock()

@@ -261,6 +261,22 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// The same for packed e2m1 operands with one ue8m0 scale per 32 values of a row,
+// read from TMEM (K = 64: two scales a row, selected in the descriptor).
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(
+            d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+        : "memory");
+}
+// 32 rows of 16 bytes from shared memory to four TMEM columns, the same for
+// each of the four lane quadrants: the 128 rows' scale words of one K atom.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t sdesc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
 // Arrive once on `bar` when all previously issued tcgen05.mma of this thread complete.
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -333,6 +349,16 @@ __host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {
            | (1u << 7)          // A: signed 8-bit
            | (1u << 10)         // B: signed 8-bit
            | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// Instruction descriptor of kind::mxf4 (A, B e2m1, K-major; ue8m0 scales; D
+// fp32); sf: which half (0 or 2) of each row's four scale bytes the MMA takes.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N, uint32_t sf) {
+    return (sf << 4)            // B scale id
+           | (1u << 7)          // A format: E2M1
+           | (1u << 10)         // B format: E2M1
+           | ((uint32_t)(N >> 3) << 17) | (1u << 23)  // scale format: UE8M0
+           | ((uint32_t)(M >> 7) << 27) | (sf << 29);  // A scale id; bit 31 = 0: K = 64
 }
 
 }  // namespace tc
