@@ -27,9 +27,12 @@
 // the weight-gradient sums stay in registers from row to row); longer rows go
 // through kernels that re-read the row.
 #include <cuda_fp16.h>
+#include <string.h>
 
-#include "common.cuh"
+#include <type_traits>
+
 #include "philox.cuh"
+#include "tc_ptx.cuh"
 
 namespace act {
 namespace norm {
@@ -61,71 +64,148 @@ template <typename T>
 struct alignas(16) Raw8 {
     T v[8];
 };
+// Their float32 values in pairs (packed f32x2 arithmetic takes two at a time).
+struct F8 {
+    float2 p[4];
+};
 
-// A lane's eight values of the segment starting at `seg0` of a row of n values.
-// VEC: values seg0 + 8 lane + j; else seg0 + 32 j + lane.
-template <bool VEC>
-__device__ __forceinline__ int64_t col_of(int64_t seg0, int lane, int j) {
-    return VEC ? seg0 + 8 * lane + j : seg0 + 32 * j + lane;
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ Raw8<T> load8(const T *row, int64_t seg0, int64_t n, int lane) {
-    Raw8<T> r;
-    if constexpr (VEC) {  // n is a multiple of 8
-        const int64_t c = seg0 + 8 * lane;
-        uint4 *d = reinterpret_cast<uint4 *>(&r);
-        if (c < n) {
-            const uint4 *s = reinterpret_cast<const uint4 *>(row + c);
+template <typename T>
+__device__ __forceinline__ F8 unpack(const Raw8<T> &r) {
+    F8 f;
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(r) / 16; ++i) d[i] = s[i];
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) {
+            f.p[j] = make_float2(to_f<T>(r.v[2 * j]), to_f<T>(r.v[2 * j + 1]));
         } else {
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(r) / 16; ++i) d[i] = make_uint4(0, 0, 0, 0);
+            uint32_t w;
+            memcpy(&w, &r.v[2 * j], 4);
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                f.p[j] = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+            } else {
+                __half2 h;
+                memcpy(&h, &w, 4);
+                f.p[j] = __half22float2(h);
+            }
         }
-    } else {
+    }
+    return f;
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> pack(const F8 &f) {
+    Raw8<T> r;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t c = seg0 + 32 * j + lane;
-            r.v[j] = c < n ? row[c] : from_f<T>(0.f);
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) {
+            r.v[2 * j] = f.p[j].x, r.v[2 * j + 1] = f.p[j].y;
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat162 h = __float22bfloat162_rn(f.p[j]);
+            memcpy(&r.v[2 * j], &h, 4);
+        } else {
+            const __half2 h = __float22half2_rn(f.p[j]);
+            memcpy(&r.v[2 * j], &h, 4);
         }
     }
     return r;
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T *row, int64_t seg0, int64_t n, int lane, const float (&f)[8]) {
-    if constexpr (VEC) {
-        const int64_t c = seg0 + 8 * lane;
-        if (c >= n) return;
-        Raw8<T> r;
+// Keeps loop-invariant 16-bit values packed: without it their unpacked form is
+// carried through the loop in twice the registers.
+template <typename T>
+__device__ __forceinline__ void stay_packed(Raw8<T> &r) {
+    if constexpr (sizeof(T) == 2) {
+        uint32_t q[4];
+        memcpy(q, &r, 16);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r.v[j] = from_f<T>(f[j]);
-        const uint4 *s = reinterpret_cast<const uint4 *>(&r);
-        uint4 *d = reinterpret_cast<uint4 *>(row + c);
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(r) / 16; ++i) d[i] = s[i];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t c = seg0 + 32 * j + lane;
-            if (c < n) row[c] = from_f<T>(f[j]);
-        }
+        for (int i = 0; i < 4; ++i) asm volatile("" : "+r"(q[i]));
+        memcpy(&r, q, 16);
     }
 }
 
-// Keep bits of the lane's eight values (bit j: its value j).  All lanes of the warp call it.
+// Number of the lane's eight values of the segment at `seg0` that lie in a row
+// of n values (VEC: 8 or 0, the row length is a multiple of 8).
+// A lane's values: VEC seg0 + 8 lane + j; else seg0 + 32 j + lane.
 template <bool VEC>
-__device__ __forceinline__ uint32_t keep_bits(uint64_t row, int64_t seg0, int lane, uint64_t key, uint32_t threshold) {
-    const uint32_t mine = drop_keep8(row, (uint32_t)(seg0 >> 3) + lane, key, threshold);
-    if constexpr (VEC) return mine;
-    uint32_t bits = 0;
+__device__ __forceinline__ int count_of(int64_t seg0, int64_t n, int lane) {
+    const int64_t left = n - seg0 - (VEC ? 8 * lane : lane);
+    if (VEC) return left > 0 ? 8 : 0;
+    return left <= 0 ? 0 : (left > 224 ? 8 : (int)((left + 31) >> 5));
+}
+
+// Values outside the row read as `fill`.
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw8<T> load8(const T *row, int64_t seg0, int count, int lane, float fill = 0.f) {
+    Raw8<T> r;
+    if constexpr (VEC) {
+        if (count) {
+            const uint4 *s = reinterpret_cast<const uint4 *>(row + seg0 + 8 * lane);
+            uint4 q[sizeof(r) / 16];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {  // value 32 j + lane belongs to block 4 j + lane / 8
-        const uint32_t k = __shfl_sync(0xffffffffu, mine, 4 * j + (lane >> 3));
-        bits |= ((k >> (lane & 7)) & 1u) << j;
+            for (int i = 0; i < (int)sizeof(r) / 16; ++i) q[i] = s[i];
+            memcpy(&r, q, sizeof(r));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r.v[j] = from_f<T>(fill);
+        }
+    } else {
+        const T *s = row + seg0 + lane;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r.v[j] = j < count ? s[32 * j] : from_f<T>(fill);
     }
-    return bits;
+    return r;
+}
+// The same of a weight vector that may be absent.
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw8<T> load8_or(const T *row, float absent, int64_t seg0, int count, int lane) {
+    return load8<T, VEC>(row, seg0, row ? count : 0, lane, absent);
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T *row, int64_t seg0, int count, int lane, const F8 &f) {
+    const Raw8<T> r = pack<T>(f);
+    if constexpr (VEC) {
+        if (!count) return;
+        uint4 q[sizeof(r) / 16];
+        memcpy(q, &r, sizeof(r));
+        uint4 *d = reinterpret_cast<uint4 *>(row + seg0 + 8 * lane);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(r) / 16; ++i) d[i] = q[i];
+    } else {
+        T *d = row + seg0 + lane;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < count) d[32 * j] = r.v[j];
+    }
+}
+
+// x * scale where kept, else 0 (whatever x holds).  All lanes of the warp call it.
+template <bool VEC>
+__device__ __forceinline__ F8 drop8(const F8 &x, uint64_t row, int64_t seg0, int lane, uint64_t key,
+                                    const DropParams &d) {
+    F8 y;
+    const float2 sc = make_float2(d.scale, d.scale);
+    const uint32_t block = (uint32_t)(seg0 >> 3) + lane;
+    if constexpr (VEC) {
+        const uint4 r = philox4x32_10(block, (uint32_t)row, (uint32_t)(row >> 32), key);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 t = mul2(x.p[j], sc);
+            y.p[j] = make_float2((w[j] & 0xffffu) >= d.threshold ? t.x : 0.f, (w[j] >> 16) >= d.threshold ? t.y : 0.f);
+        }
+    } else {
+        const uint32_t mine = drop_keep8(row, block, key, d.threshold);
+        // value 32 j + lane belongs to block 4 j + lane / 8
+        const uint32_t bit = 1u << (lane & 7);
+        uint32_t k[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) k[j] = __shfl_sync(0xffffffffu, mine, 4 * j + (lane >> 3)) & bit;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 t = mul2(x.p[j], sc);
+            y.p[j] = make_float2(k[2 * j] ? t.x : 0.f, k[2 * j + 1] ? t.y : 0.f);
+        }
+    }
+    return y;
 }
 
 // ---------------------------------------------------------------- dropout
@@ -137,21 +217,31 @@ struct DropArgs {
     DropParams d;
 };
 
-// One warp per segment of 256 values, grid-stride over rows x segments.
+// One warp per segment of 256 values, two segments in flight; a warp's next
+// segment lies grid-many further on, which is `dr` rows and `ds` segments.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) dropout_kernel(DropArgs<T> a) {
+__global__ void __launch_bounds__(256) dropout_kernel(DropArgs<T> a, int64_t segs, int64_t dr, int64_t ds) {
     const int lane = threadIdx.x & 31;
-    const int64_t segs = (a.cols + SEG - 1) / SEG, total = a.rows * segs;
     const uint64_t key = drop_seed(a.d);
-    const int64_t step = (int64_t)gridDim.x * (blockDim.x >> 5);
-    for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += step) {
-        const int64_t r = i / segs, seg0 = (i - r * segs) * SEG;
-        const Raw8<T> x = load8<T, VEC>(a.x + r * a.ldx, seg0, a.cols, lane);
-        const uint32_t keep = keep_bits<VEC>(a.d.row_offset + (uint64_t)r, seg0, lane, key, a.d.threshold);
-        float f[8];
+    const int64_t first = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    int64_t r = first / segs, sg = first - r * segs;
+    while (r < a.rows) {
+        int64_t rr[2], s0[2];
+        int n[2];
+        Raw8<T> x[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = (keep >> j) & 1u ? to_f<T>(x.v[j]) * a.d.scale : 0.f;
-        store8<T, VEC>(a.y + r * a.ldy, seg0, a.cols, lane, f);
+        for (int u = 0; u < 2; ++u) {
+            rr[u] = r, s0[u] = sg * SEG;
+            n[u] = r < a.rows ? count_of<VEC>(s0[u], a.cols, lane) : 0;
+            x[u] = load8<T, VEC>(a.x + r * a.ldx, s0[u], n[u], lane);
+            r += dr, sg += ds;
+            if (sg >= segs) sg -= segs, ++r;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const F8 y = drop8<VEC>(unpack<T>(x[u]), a.d.row_offset + (uint64_t)rr[u], s0[u], lane, key, a.d);
+            store8<T, VEC>(a.y + rr[u] * a.ldy, s0[u], n[u], lane, y);
+        }
     }
 }
 
@@ -178,70 +268,141 @@ __device__ __forceinline__ float row_sum(float v, float *red, int wpr, int warp,
     return s;
 }
 
-template <typename T, typename W, int NCH, bool VEC, bool DROP>
-__global__ void __launch_bounds__(NCH == 4 ? 512 : 256) ln_fwd_kernel(FwdArgs<T, W> a, int wpr) {
+// Resident CTAs of 256 threads that the register use allows.
+__host__ __device__ constexpr int fwd_ctas(int nch) { return nch <= 2 ? 3 : 2; }
+constexpr int BWD_CTAS = 2;
+constexpr int MAX_DEPTH = 4;
+constexpr int RING_HEAD = 8 * MAX_DEPTH * 8 + 16;  // barriers of up to eight warps' rings, the abort word
+
+// The rows a CTA (or, with one warp per row, a warp) works through, brought to
+// shared memory ahead of their use: DEPTH slots, one bulk copy per input and
+// row, issued by one thread.  A slot is filled again once every reader has
+// passed the barrier that follows its last read.
+template <typename T, int INPUTS>
+struct RowRing {
+    uint8_t *slots;
+    uint64_t *bars;
+    uint32_t bytes;  // of one input's row
+    int depth, slot;
+    uint32_t phase;
+
+    // dyn: barriers of up to eight rings, the abort word, then the slots.
+    __device__ __forceinline__ void init(uint8_t *dyn, int which, uint32_t row_bytes, int d, bool leader) {
+        bytes = row_bytes, depth = d, slot = 0, phase = 0;
+        bars = reinterpret_cast<uint64_t *>(dyn) + which * MAX_DEPTH;
+        slots = dyn + RING_HEAD + (size_t)which * d * INPUTS * row_bytes;
+        if (threadIdx.x == 0) *abort_word(dyn) = 0;
+        if (leader) {
+            for (int i = 0; i < d; ++i) tc::mbar_init(&bars[i], 1);
+            tc::fence_mbar_init();
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ static volatile int *abort_word(uint8_t *dyn) {
+        return reinterpret_cast<volatile int *>(dyn + RING_HEAD - 16);
+    }
+    __device__ __forceinline__ void fill(int s, int k, const T *row) {
+        if (k == 0) tc::mbar_arrive_expect_tx(&bars[s], bytes * INPUTS);
+        tc::bulk_load(slots + (s * INPUTS + k) * bytes, row, bytes, &bars[s]);
+    }
+    __device__ __forceinline__ void wait(uint8_t *dyn) { tc::mbar_wait(&bars[slot], phase, abort_word(dyn)); }
+    __device__ __forceinline__ const T *row(int k) const {
+        return reinterpret_cast<const T *>(slots + (slot * INPUTS + k) * bytes);
+    }
+    __device__ __forceinline__ void next() {
+        if (++slot == depth) slot = 0, phase ^= 1;
+    }
+};
+
+// MAXT: the launch's thread count rounded up to 256 or 512.
+template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP>
+__global__ void __launch_bounds__(MAXT, MAXT == 256 ? fwd_ctas(NCH) : 1) ln_fwd_kernel(FwdArgs<T, W> a, int wpr, int depth) {
+    extern __shared__ __align__(128) uint8_t dyn[];
     __shared__ float red[2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
     const int rpc = wpr == 1 ? nwarps : 1;  // rows a CTA has in hand at once
-    const int w0 = wpr == 1 ? 0 : warp;
+    const int w0 = wpr == 1 ? 0 : warp, mine = wpr == 1 ? warp : 0;
     const float inv_n = 1.f / (float)a.cols;
     const uint64_t key = DROP ? drop_seed(a.d) : 0;
+    constexpr int IN = DROP ? 2 : 1;
+    RowRing<T, IN> ring;
+    const bool leader = wpr == 1 ? lane == 0 : threadIdx.x == 0;
+    const int64_t r0 = (int64_t)blockIdx.x * rpc + mine, step = (int64_t)gridDim.x * rpc;
+    auto fill = [&](int s, int64_t row) {
+        if (row >= a.rows) return;
+        ring.fill(s, 0, a.x + row * a.ldx);
+        if constexpr (DROP) ring.fill(s, 1, a.res + row * a.ldr);
+    };
+    if constexpr (VEC) {
+        ring.init(dyn, mine, (uint32_t)(a.cols * sizeof(T)), depth, leader);
+        if (leader)
+            for (int i = 0; i < depth; ++i) fill(i, r0 + i * step);
+    }
     Raw8<W> wv[NCH], bv[NCH];
+    int n[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        const int64_t seg0 = (int64_t)(w0 + i * wpr) * SEG;
-        if (a.w) wv[i] = load8<W, VEC>(a.w, seg0, a.cols, lane);
-        if (a.b) bv[i] = load8<W, VEC>(a.b, seg0, a.cols, lane);
+        const int seg0 = (w0 + i * wpr) * SEG;
+        n[i] = count_of<VEC>(seg0, a.cols, lane);
+        wv[i] = load8_or<W, VEC>(a.w, 1.f, seg0, n[i], lane);
+        bv[i] = load8_or<W, VEC>(a.b, 0.f, seg0, n[i], lane);
     }
-    for (int64_t r = (int64_t)blockIdx.x * rpc + (wpr == 1 ? warp : 0); r < a.rows; r += (int64_t)gridDim.x * rpc) {
-        float v[NCH][8];
-        float s = 0.f;
+    for (int64_t r = r0; r < a.rows; r += step) {
+        F8 v[NCH];
+        float2 s = make_float2(0.f, 0.f);
+        if constexpr (VEC) ring.wait(dyn);
+        const T *xr = VEC ? ring.row(0) : a.x + r * a.ldx;
+        const T *rr = DROP ? (VEC ? ring.row(IN - 1) : a.res + r * a.ldr) : nullptr;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int64_t seg0 = (int64_t)(w0 + i * wpr) * SEG;
-            const Raw8<T> x = load8<T, VEC>(a.x + r * a.ldx, seg0, a.cols, lane);
+            const int seg0 = (w0 + i * wpr) * SEG;
+            v[i] = unpack<T>(load8<T, VEC>(xr, seg0, n[i], lane));
             if constexpr (DROP) {
-                const Raw8<T> res = load8<T, VEC>(a.res + r * a.ldr, seg0, a.cols, lane);
-                const uint32_t keep =
-                    keep_bits<VEC>(a.d.row_offset + (uint64_t)r, seg0, lane, key, a.d.threshold);
+                const F8 res = unpack<T>(load8<T, VEC>(rr, seg0, n[i], lane));
+                const F8 d = drop8<VEC>(v[i], a.d.row_offset + (uint64_t)r, seg0, lane, key, a.d);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    v[i][j] = (keep >> j) & 1u ? __fmaf_rn(to_f<T>(x.v[j]), a.d.scale, to_f<T>(res.v[j]))
-                                               : to_f<T>(res.v[j]);
-                store8<T, VEC>(a.h + r * a.ldh, seg0, a.cols, lane, v[i]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = to_f<T>(x.v[j]);
+                for (int j = 0; j < 4; ++j) v[i].p[j] = add2(d.p[j], res.p[j]);
+                store8<T, VEC>(a.h + r * a.ldh, seg0, n[i], lane, v[i]);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += v[i][j];
+            for (int j = 0; j < 4; ++j) s = add2(s, v[i].p[j]);
         }
-        const float mean = row_sum(s, red[0], wpr, warp, lane) * inv_n;
-        float q = 0.f;
+        const float mean = row_sum(s.x + s.y, red[0], wpr, warp, lane) * inv_n;
+        if constexpr (VEC) {  // every reader of the slot is past its reads
+            if (wpr == 1) __syncwarp();
+            if (leader) fill(ring.slot, r + depth * step);
+            ring.next();
+        }
+        const float2 mean2 = make_float2(mean, mean);
+        float2 q = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int64_t seg0 = (int64_t)(w0 + i * wpr) * SEG;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[i][j] -= mean;
-                if (col_of<VEC>(seg0, lane, j) < a.cols) q = __fmaf_rn(v[i][j], v[i][j], q);
+            for (int j = 0; j < 4; ++j) {
+                v[i].p[j] = sub2(v[i].p[j], mean2);
+                if constexpr (!VEC) {
+                    if (2 * j >= n[i]) v[i].p[j].x = 0.f;
+                    if (2 * j + 1 >= n[i]) v[i].p[j].y = 0.f;
+                }
+                if (!VEC || n[i]) q = fma2(v[i].p[j], v[i].p[j], q);
             }
         }
-        const float var = row_sum(q, red[1], wpr, warp, lane) * inv_n;
+        const float var = row_sum(q.x + q.y, red[1], wpr, warp, lane) * inv_n;
         const float rstd = 1.f / sqrtf(var + a.eps);
         if (lane == 0 && w0 == 0) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
         }
+        const float2 rstd2 = make_float2(rstd, rstd);
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int64_t seg0 = (int64_t)(w0 + i * wpr) * SEG;
+            const int seg0 = (w0 + i * wpr) * SEG;
+            stay_packed(wv[i]);
+            stay_packed(bv[i]);
+            const F8 w = unpack<W>(wv[i]), b = unpack<W>(bv[i]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float xh = v[i][j] * rstd;
-                v[i][j] = __fmaf_rn(xh, a.w ? to_f<W>(wv[i].v[j]) : 1.f, a.b ? to_f<W>(bv[i].v[j]) : 0.f);
-            }
-            store8<T, VEC>(a.y + r * a.ldy, seg0, a.cols, lane, v[i]);
+            for (int j = 0; j < 4; ++j) v[i].p[j] = fma2(mul2(v[i].p[j], rstd2), w.p[j], b.p[j]);
+            store8<T, VEC>(a.y + r * a.ldy, seg0, n[i], lane, v[i]);
         }
     }
 }
@@ -256,38 +417,37 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_fwd_long_kernel(FwdArgs<T, W>
     const uint64_t key = DROP ? drop_seed(a.d) : 0;
     const int64_t segs = (a.cols + SEG - 1) / SEG;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        auto fetch = [&](int64_t seg0, float (&v)[8]) {
-            const Raw8<T> x = load8<T, VEC>(a.x + r * a.ldx, seg0, a.cols, lane);
+        auto fetch = [&](int64_t seg0, int n) {
+            F8 v = unpack<T>(load8<T, VEC>(a.x + r * a.ldx, seg0, n, lane));
             if constexpr (DROP) {
-                const Raw8<T> res = load8<T, VEC>(a.res + r * a.ldr, seg0, a.cols, lane);
-                const uint32_t keep =
-                    keep_bits<VEC>(a.d.row_offset + (uint64_t)r, seg0, lane, key, a.d.threshold);
+                const F8 res = unpack<T>(load8<T, VEC>(a.res + r * a.ldr, seg0, n, lane));
+                const F8 d = drop8<VEC>(v, a.d.row_offset + (uint64_t)r, seg0, lane, key, a.d);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    v[j] = (keep >> j) & 1u ? __fmaf_rn(to_f<T>(x.v[j]), a.d.scale, to_f<T>(res.v[j]))
-                                            : to_f<T>(res.v[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = to_f<T>(x.v[j]);
+                for (int j = 0; j < 4; ++j) v.p[j] = add2(d.p[j], res.p[j]);
             }
+            return v;
         };
         float s = 0.f;
         for (int64_t g = warp; g < segs; g += nw) {
-            float v[8], t = 0.f;
-            fetch(g * SEG, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) t += v[j];
-            s += t;
+            const F8 v = fetch(g * SEG, count_of<VEC>(g * SEG, a.cols, lane));
+            const float2 t = add2(add2(v.p[0], v.p[1]), add2(v.p[2], v.p[3]));
+            s += t.x + t.y;
         }
         const float mean = row_sum(s, red[0], nw, warp, lane) * inv_n;
+        const float2 mean2 = make_float2(mean, mean);
         float q = 0.f;
         for (int64_t g = warp; g < segs; g += nw) {
-            float v[8], t = 0.f;
-            fetch(g * SEG, v);
+            const int n = count_of<VEC>(g * SEG, a.cols, lane);
+            const F8 v = fetch(g * SEG, n);
+            float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (col_of<VEC>(g * SEG, lane, j) < a.cols) t = __fmaf_rn(v[j] - mean, v[j] - mean, t);
-            q += t;
+            for (int j = 0; j < 4; ++j) {
+                float2 c = sub2(v.p[j], mean2);
+                if (2 * j >= n) c.x = 0.f;
+                if (2 * j + 1 >= n) c.y = 0.f;
+                t = fma2(c, c, t);
+            }
+            q += t.x + t.y;
         }
         const float var = row_sum(q, red[1], nw, warp, lane) * inv_n;
         const float rstd = 1.f / sqrtf(var + a.eps);
@@ -295,17 +455,16 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_fwd_long_kernel(FwdArgs<T, W>
             a.mean[r] = mean;
             a.rstd[r] = rstd;
         }
+        const float2 rstd2 = make_float2(rstd, rstd);
         for (int64_t g = warp; g < segs; g += nw) {
-            float v[8];
-            fetch(g * SEG, v);
-            if constexpr (DROP) store8<T, VEC>(a.h + r * a.ldh, g * SEG, a.cols, lane, v);
-            Raw8<W> wv, bv;
-            if (a.w) wv = load8<W, VEC>(a.w, g * SEG, a.cols, lane);
-            if (a.b) bv = load8<W, VEC>(a.b, g * SEG, a.cols, lane);
+            const int n = count_of<VEC>(g * SEG, a.cols, lane);
+            F8 v = fetch(g * SEG, n);
+            if constexpr (DROP) store8<T, VEC>(a.h + r * a.ldh, g * SEG, n, lane, v);
+            const F8 w = unpack<W>(load8_or<W, VEC>(a.w, 1.f, g * SEG, n, lane));
+            const F8 b = unpack<W>(load8_or<W, VEC>(a.b, 0.f, g * SEG, n, lane));
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                v[j] = __fmaf_rn((v[j] - mean) * rstd, a.w ? to_f<W>(wv.v[j]) : 1.f, a.b ? to_f<W>(bv.v[j]) : 0.f);
-            store8<T, VEC>(a.y + r * a.ldy, g * SEG, a.cols, lane, v);
+            for (int j = 0; j < 4; ++j) v.p[j] = fma2(mul2(sub2(v.p[j], mean2), rstd2), w.p[j], b.p[j]);
+            store8<T, VEC>(a.y + r * a.ldy, g * SEG, n, lane, v);
         }
     }
 }
@@ -336,97 +495,139 @@ __device__ __forceinline__ float2 row_sum2(float u, float v, float2 *red, int wp
     return s;
 }
 
-template <typename T, typename W, int NCH, bool VEC, bool DROP>
-__global__ void __launch_bounds__(NCH == 4 ? 512 : 256) ln_bwd_kernel(BwdArgs<T, W> a, int wpr) {
+template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP>
+__global__ void __launch_bounds__(MAXT, MAXT == 256 ? BWD_CTAS : 1) ln_bwd_kernel(BwdArgs<T, W> a, int wpr, int depth) {
     __shared__ float2 red[2][32];
-    extern __shared__ float acc_s[];  // wpr == 1: nwarps x 2 x cols, the warps' sums
+    extern __shared__ __align__(128) uint8_t dyn[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
     const int rpc = wpr == 1 ? nwarps : 1;
-    const int w0 = wpr == 1 ? 0 : warp;
+    const int w0 = wpr == 1 ? 0 : warp, mine = wpr == 1 ? warp : 0;
     const float inv_n = 1.f / (float)a.cols;
     const uint64_t key = DROP ? drop_seed(a.d) : 0;
+    constexpr int IN = DROP ? 3 : 2;
+    RowRing<T, IN> ring;
+    const bool leader = wpr == 1 ? lane == 0 : threadIdx.x == 0;
+    const int64_t r0 = (int64_t)blockIdx.x * rpc + mine, step = (int64_t)gridDim.x * rpc;
+    auto fill = [&](int s, int64_t row) {
+        if (row >= a.rows) return;
+        ring.fill(s, 0, a.dy + row * a.lddy);
+        ring.fill(s, 1, a.x + row * a.ldx);
+        // without dh its slot holds dy again and is not read
+        if constexpr (DROP) ring.fill(s, 2, a.dh ? a.dh + row * a.lddh : a.dy + row * a.lddy);
+    };
+    if constexpr (VEC) {
+        ring.init(dyn, mine, (uint32_t)(a.cols * sizeof(T)), depth, leader);
+        if (leader)
+            for (int i = 0; i < depth; ++i) fill(i, r0 + i * step);
+    }
+    // Up to two segments a thread the row's g and x-hat are held from the sums to
+    // the output, past that they are computed again from the slot (registers).
+    constexpr bool HOLD = NCH <= 2;
     Raw8<W> wv[NCH];
-    float dw[NCH][8], db[NCH][8];
+    F8 dw[NCH], db[NCH];
+    int n[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        if (a.w) wv[i] = load8<W, VEC>(a.w, (int64_t)(w0 + i * wpr) * SEG, a.cols, lane);
+        n[i] = count_of<VEC>((w0 + i * wpr) * SEG, a.cols, lane);
+        wv[i] = load8_or<W, VEC>(a.w, 1.f, (w0 + i * wpr) * SEG, n[i], lane);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.f;
+        for (int j = 0; j < 4; ++j) dw[i].p[j] = db[i].p[j] = make_float2(0.f, 0.f);
     }
     int turn = 0;
-    for (int64_t r = (int64_t)blockIdx.x * rpc + (wpr == 1 ? warp : 0); r < a.rows; r += (int64_t)gridDim.x * rpc) {
-        const float mean = a.mean[r], rstd = a.rstd[r];
-        float g[NCH][8], xh[NCH][8];
-        float s1 = 0.f, s2 = 0.f;
+    float mean = r0 < a.rows ? a.mean[r0] : 0.f, rstd = r0 < a.rows ? a.rstd[r0] : 0.f;
+    for (int64_t r = r0; r < a.rows; r += step, ++turn) {
+        const float2 mean2 = make_float2(mean, mean), rstd2 = make_float2(rstd, rstd);
+        const float rs = rstd;
+        if (r + step < a.rows) mean = a.mean[r + step], rstd = a.rstd[r + step];
+        const T *yr = VEC ? ring.row(0) : a.dy + r * a.lddy;
+        const T *xr = VEC ? ring.row(1) : a.x + r * a.ldx;
+        float2 s1 = make_float2(0.f, 0.f), s2 = s1;
+        F8 gh[HOLD ? NCH : 1], xh[HOLD ? NCH : 1];
+        if constexpr (VEC) ring.wait(dyn);
+        auto values = [&](int i, F8 &dy, F8 &x) {  // dy and x-hat
+            const int seg0 = (w0 + i * wpr) * SEG;
+            dy = unpack<T>(load8<T, VEC>(yr, seg0, n[i], lane));
+            x = unpack<T>(load8<T, VEC>(xr, seg0, n[i], lane));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.p[j] = mul2(sub2(x.p[j], mean2), rstd2);
+        };
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int64_t seg0 = (int64_t)(w0 + i * wpr) * SEG;
-            const Raw8<T> y = load8<T, VEC>(a.dy + r * a.lddy, seg0, a.cols, lane);
-            const Raw8<T> x = load8<T, VEC>(a.x + r * a.ldx, seg0, a.cols, lane);
+            F8 dy, x;
+            values(i, dy, x);
+            stay_packed(wv[i]);
+            const F8 w = unpack<W>(wv[i]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float dy = to_f<T>(y.v[j]);
-                const bool in = col_of<VEC>(seg0, lane, j) < a.cols;
-                xh[i][j] = in ? (to_f<T>(x.v[j]) - mean) * rstd : 0.f;
-                dw[i][j] = __fmaf_rn(dy, xh[i][j], dw[i][j]);
-                db[i][j] += dy;
-                g[i][j] = a.w ? dy * to_f<W>(wv[i].v[j]) : dy;
-                s1 += g[i][j];
-                s2 = __fmaf_rn(g[i][j], xh[i][j], s2);
+            for (int j = 0; j < 4; ++j) {  // dy is 0 past the row's end
+                const float2 g = mul2(dy.p[j], w.p[j]);
+                dw[i].p[j] = fma2(dy.p[j], x.p[j], dw[i].p[j]);
+                db[i].p[j] = add2(db[i].p[j], dy.p[j]);
+                s1 = add2(s1, g);
+                s2 = fma2(g, x.p[j], s2);
+                if constexpr (HOLD) gh[i].p[j] = g, xh[i].p[j] = x.p[j];
             }
         }
-        const float2 s = row_sum2(s1, s2, red[turn], wpr, warp, lane);
-        turn ^= 1;
-        const float m1 = s.x * inv_n, m2 = s.y * inv_n;
+        const float2 s = row_sum2(s1.x + s1.y, s2.x + s2.y, red[turn & 1], wpr, warp, lane);
+        if constexpr (VEC) {  // the row before this one has been read by all
+            if (wpr == 1) __syncwarp();
+            if (leader && turn > 0) fill(ring.slot == 0 ? depth - 1 : ring.slot - 1, r + (depth - 1) * step);
+        }
+        // dx = rstd g - rstd mean(g) - x-hat rstd mean(g x-hat)
+        const float c1 = -rs * (s.x * inv_n), c2 = -rs * (s.y * inv_n);
+        const float2 c1_2 = make_float2(c1, c1), c2_2 = make_float2(c2, c2);
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int64_t seg0 = (int64_t)(w0 + i * wpr) * SEG;
+            const int seg0 = (w0 + i * wpr) * SEG;
+            F8 g, x;
+            if constexpr (HOLD) {
+                g = gh[i], x = xh[i];
+            } else {
+                values(i, g, x);
+                stay_packed(wv[i]);
+                const F8 w = unpack<W>(wv[i]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[i][j] = rstd * (g[i][j] - __fmaf_rn(xh[i][j], m2, m1));
+                for (int j = 0; j < 4; ++j) g.p[j] = mul2(g.p[j], w.p[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g.p[j] = fma2(x.p[j], c2_2, fma2(g.p[j], rstd2, c1_2));
             if constexpr (DROP) {
                 if (a.dh) {
-                    const Raw8<T> dh = load8<T, VEC>(a.dh + r * a.lddh, seg0, a.cols, lane);
+                    const F8 dh = unpack<T>(
+                        load8<T, VEC>(VEC ? ring.row(IN - 1) : a.dh + r * a.lddh, seg0, n[i], lane));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) g[i][j] += to_f<T>(dh.v[j]);
+                    for (int j = 0; j < 4; ++j) g.p[j] = add2(g.p[j], dh.p[j]);
                 }
-                store8<T, VEC>(a.dr + r * a.lddr, seg0, a.cols, lane, g[i]);
-                const uint32_t keep =
-                    keep_bits<VEC>(a.d.row_offset + (uint64_t)r, seg0, lane, key, a.d.threshold);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) g[i][j] = (keep >> j) & 1u ? g[i][j] * a.d.scale : 0.f;
+                store8<T, VEC>(a.dr + r * a.lddr, seg0, n[i], lane, g);
+                g = drop8<VEC>(g, a.d.row_offset + (uint64_t)r, seg0, lane, key, a.d);
             }
-            store8<T, VEC>(a.dx + r * a.lddx, seg0, a.cols, lane, g[i]);
+            store8<T, VEC>(a.dx + r * a.lddx, seg0, n[i], lane, g);
         }
+        if constexpr (VEC) ring.next();
     }
     if (!a.part) return;
     float *part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
-    if (wpr != 1) {
+    if (wpr == 1) {
+        // the warps' sums, over the ring's space once every warp is done with it
+        __syncthreads();
+        float *acc = reinterpret_cast<float *>(dyn + RING_HEAD), *own = acc + (int64_t)warp * 2 * a.cols;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int64_t seg0 = (int64_t)(w0 + i * wpr) * SEG;
-            store8<float, VEC>(part, seg0, a.cols, lane, dw[i]);
-            store8<float, VEC>(part + a.cols, seg0, a.cols, lane, db[i]);
+            store8<float, VEC>(own, i * SEG, n[i], lane, dw[i]);
+            store8<float, VEC>(own + a.cols, i * SEG, n[i], lane, db[i]);
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) {
+            float s = 0.f;
+            for (int i = 0; i < nwarps; ++i) s += acc[(int64_t)i * 2 * a.cols + c];
+            part[c] = s;
         }
         return;
     }
-    float *mine = acc_s + (int64_t)warp * 2 * a.cols;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        const int64_t seg0 = (int64_t)i * SEG;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t c = col_of<VEC>(seg0, lane, j);
-            if (c < a.cols) {
-                mine[c] = dw[i][j];
-                mine[a.cols + c] = db[i][j];
-            }
-        }
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) {
-        float s = 0.f;
-        for (int i = 0; i < nwarps; ++i) s += acc_s[(int64_t)i * 2 * a.cols + c];
-        part[c] = s;
+        const int seg0 = (w0 + i * wpr) * SEG;
+        store8<float, VEC>(part, seg0, n[i], lane, dw[i]);
+        store8<float, VEC>(part + a.cols, seg0, n[i], lane, db[i]);
     }
 }
 
@@ -441,22 +642,21 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_bwd_sums_kernel(BwdArgs<T, W>
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const float mean = a.mean[r], rstd = a.rstd[r];
         float s1 = 0.f, s2 = 0.f;
+        const float2 mean2 = make_float2(mean, mean), rstd2 = make_float2(rstd, rstd);
         for (int64_t sg = warp; sg < segs; sg += nw) {
-            const Raw8<T> y = load8<T, VEC>(a.dy + r * a.lddy, sg * SEG, a.cols, lane);
-            const Raw8<T> x = load8<T, VEC>(a.x + r * a.ldx, sg * SEG, a.cols, lane);
-            Raw8<W> wv;
-            if (a.w) wv = load8<W, VEC>(a.w, sg * SEG, a.cols, lane);
-            float t1 = 0.f, t2 = 0.f;
+            const int n = count_of<VEC>(sg * SEG, a.cols, lane);
+            const F8 y = unpack<T>(load8<T, VEC>(a.dy + r * a.lddy, sg * SEG, n, lane));
+            const F8 x = unpack<T>(load8<T, VEC>(a.x + r * a.ldx, sg * SEG, n, lane));
+            const F8 w = unpack<W>(load8_or<W, VEC>(a.w, 1.f, sg * SEG, n, lane));
+            float2 t1 = make_float2(0.f, 0.f), t2 = t1;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float g = to_f<T>(y.v[j]) * (a.w ? to_f<W>(wv.v[j]) : 1.f);
-                if (col_of<VEC>(sg * SEG, lane, j) < a.cols) {
-                    t1 += g;
-                    t2 = __fmaf_rn(g, (to_f<T>(x.v[j]) - mean) * rstd, t2);
-                }
+            for (int j = 0; j < 4; ++j) {  // dy is 0 past the row's end
+                const float2 g = mul2(y.p[j], w.p[j]);
+                t1 = add2(t1, g);
+                t2 = fma2(g, mul2(sub2(x.p[j], mean2), rstd2), t2);
             }
-            s1 += t1;
-            s2 += t2;
+            s1 += t1.x + t1.y;
+            s2 += t2.x + t2.y;
         }
         const float2 s = row_sum2(s1, s2, red[turn], nw, warp, lane);
         turn ^= 1;
@@ -472,39 +672,40 @@ __global__ void __launch_bounds__(128) ln_bwd_cols_kernel(BwdArgs<T, W> a, const
     const int64_t seg0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) * SEG;
     if (seg0 >= a.cols) return;
     const uint64_t key = DROP ? drop_seed(a.d) : 0;
-    Raw8<W> wv;
-    if (a.w) wv = load8<W, VEC>(a.w, seg0, a.cols, lane);
-    float dw[8] = {}, db[8] = {};
-    for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const float mean = a.mean[r], rstd = a.rstd[r];
-        const float2 m = sums[r];
-        const Raw8<T> y = load8<T, VEC>(a.dy + r * a.lddy, seg0, a.cols, lane);
-        const Raw8<T> x = load8<T, VEC>(a.x + r * a.ldx, seg0, a.cols, lane);
-        float g[8];
+    const int n = count_of<VEC>(seg0, a.cols, lane);
+    const F8 w = unpack<W>(load8_or<W, VEC>(a.w, 1.f, seg0, n, lane));
+    F8 dw, db;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float dy = to_f<T>(y.v[j]), xh = (to_f<T>(x.v[j]) - mean) * rstd;
-            if (col_of<VEC>(seg0, lane, j) < a.cols) dw[j] = __fmaf_rn(dy, xh, dw[j]);
-            db[j] += dy;
-            g[j] = rstd * ((a.w ? dy * to_f<W>(wv.v[j]) : dy) - __fmaf_rn(xh, m.y, m.x));
+    for (int j = 0; j < 4; ++j) dw.p[j] = db.p[j] = make_float2(0.f, 0.f);
+    for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
+        const float rstd = a.rstd[r];
+        const float2 mean2 = make_float2(a.mean[r], a.mean[r]), rstd2 = make_float2(rstd, rstd), m = sums[r];
+        const float2 c1 = make_float2(-rstd * m.x, -rstd * m.x), c2 = make_float2(-rstd * m.y, -rstd * m.y);
+        const F8 y = unpack<T>(load8<T, VEC>(a.dy + r * a.lddy, seg0, n, lane));
+        const F8 x = unpack<T>(load8<T, VEC>(a.x + r * a.ldx, seg0, n, lane));
+        F8 g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 xh = mul2(sub2(x.p[j], mean2), rstd2);
+            dw.p[j] = fma2(y.p[j], xh, dw.p[j]);
+            db.p[j] = add2(db.p[j], y.p[j]);
+            g.p[j] = fma2(xh, c2, fma2(mul2(y.p[j], w.p[j]), rstd2, c1));
         }
         if constexpr (DROP) {
             if (a.dh) {
-                const Raw8<T> dh = load8<T, VEC>(a.dh + r * a.lddh, seg0, a.cols, lane);
+                const F8 dh = unpack<T>(load8<T, VEC>(a.dh + r * a.lddh, seg0, n, lane));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] += to_f<T>(dh.v[j]);
+                for (int j = 0; j < 4; ++j) g.p[j] = add2(g.p[j], dh.p[j]);
             }
-            store8<T, VEC>(a.dr + r * a.lddr, seg0, a.cols, lane, g);
-            const uint32_t keep = keep_bits<VEC>(a.d.row_offset + (uint64_t)r, seg0, lane, key, a.d.threshold);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = (keep >> j) & 1u ? g[j] * a.d.scale : 0.f;
+            store8<T, VEC>(a.dr + r * a.lddr, seg0, n, lane, g);
+            g = drop8<VEC>(g, a.d.row_offset + (uint64_t)r, seg0, lane, key, a.d);
         }
-        store8<T, VEC>(a.dx + r * a.lddx, seg0, a.cols, lane, g);
+        store8<T, VEC>(a.dx + r * a.lddx, seg0, n, lane, g);
     }
     if (!a.part) return;
     float *part = a.part + (int64_t)blockIdx.y * 2 * a.cols;
-    store8<float, VEC>(part, seg0, a.cols, lane, dw);
-    store8<float, VEC>(part + a.cols, seg0, a.cols, lane, db);
+    store8<float, VEC>(part, seg0, n, lane, dw);
+    store8<float, VEC>(part + a.cols, seg0, n, lane, db);
 }
 
 // dw / db from the `parts` partial sums, in their order: a column's sum does
@@ -533,21 +734,39 @@ __global__ void __launch_bounds__(256) ln_bwd_finish_kernel(const float *part, i
 }
 
 // ---------------------------------------------------------------- launches
+// Segments per thread, warps per row, ring slots and the kernel's shared memory.
 struct Shape {
-    int nch, wpr, threads, rows_per_cta;
+    int nch, wpr, threads, rows_per_cta, depth, smem, per_sm;
 };
-// Segments per thread and warps per row.
-static Shape shape_of(int64_t cols) {
+static Shape shape_of(int64_t cols, int esize, int inputs, bool bwd) {
     const int segs = (int)((cols + SEG - 1) / SEG);
-    if (segs <= 4) return {segs <= 1 ? 1 : (segs <= 2 ? 2 : 4), 1, 256, 8};
-    const int nch = segs <= 16 ? 2 : 4;
-    const int wpr = (segs + nch - 1) / nch;
-    return {nch, wpr, 32 * wpr, 1};
+    Shape s{};
+    if (segs <= 4) {
+        s = {segs <= 1 ? 1 : (segs <= 2 ? 2 : 4), 1, 256, 8, 0, 0, 0};
+    } else {
+        s.nch = segs <= 32 ? 2 : 4;
+        s.wpr = (segs + s.nch - 1) / s.nch;
+        s.threads = 32 * s.wpr;
+        s.rows_per_cta = 1;
+    }
+    const int64_t slot = cols * esize * inputs * s.rows_per_cta;
+    s.per_sm = s.threads <= 256 ? (bwd ? BWD_CTAS : fwd_ctas(s.nch)) : 1;
+    const int64_t room = 220 * 1024 / s.per_sm - 2048;
+    s.depth = (int)(room / slot < MAX_DEPTH ? room / slot : MAX_DEPTH);
+    if (s.depth < 2) {  // the longest rows: one CTA per SM
+        s.per_sm = 1;
+        s.depth = (int)((220 * 1024 - 2048) / slot < MAX_DEPTH ? (220 * 1024 - 2048) / slot : MAX_DEPTH);
+    }
+    s.smem = RING_HEAD + (int)(s.depth * slot);
+    if (bwd && s.wpr == 1) {
+        const int acc = RING_HEAD + (int)(s.rows_per_cta * 2 * cols * 4);
+        if (acc > s.smem) s.smem = acc;
+    }
+    return s;
 }
 static int grid_of(const Shape &s, int64_t rows) {
     const int64_t ctas = (rows + s.rows_per_cta - 1) / s.rows_per_cta;
-    const int per_sm = 1024 / s.threads < 1 ? 1 : 1024 / s.threads;
-    const int64_t cap = (int64_t)num_sms() * per_sm;
+    const int64_t cap = (int64_t)num_sms() * s.per_sm;
     return (int)(ctas < cap ? ctas : cap);
 }
 static int long_parts(int64_t rows, int64_t cols) {
@@ -561,7 +780,8 @@ static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 static size_t bwd_workspace(int64_t rows, int64_t cols) {
     if (is_long(cols)) return up256((size_t)long_parts(rows, cols) * 2 * cols * 4) + up256((size_t)rows * 8);
-    return up256((size_t)grid_of(shape_of(cols), rows) * 2 * cols * 4);
+    const int64_t ctas = cols <= 4 * SEG ? (rows + 7) / 8 : rows, cap = (int64_t)num_sms() * BWD_CTAS;
+    return up256((size_t)(ctas < cap ? ctas : cap) * 2 * cols * 4);
 }
 
 template <typename T, typename W, bool VEC, bool DROP>
@@ -571,20 +791,25 @@ static int fwd_launch(const FwdArgs<T, W> &a, cudaStream_t st) {
         ln_fwd_long_kernel<T, W, VEC, DROP><<<(int)(a.rows < cap ? a.rows : cap), LONG_THREADS, 0, st>>>(a);
         return launch_status();
     }
-    const Shape s = shape_of(a.cols);
+    const Shape s = shape_of(a.cols, sizeof(T), DROP ? 2 : 1, false);
     const int grid = grid_of(s, a.rows);
-    if (s.nch == 1) ln_fwd_kernel<T, W, 1, VEC, DROP><<<grid, s.threads, 0, st>>>(a, s.wpr);
-    else if (s.nch == 2) ln_fwd_kernel<T, W, 2, VEC, DROP><<<grid, s.threads, 0, st>>>(a, s.wpr);
-    else ln_fwd_kernel<T, W, 4, VEC, DROP><<<grid, s.threads, 0, st>>>(a, s.wpr);
-    return launch_status();
+    auto go = [&](auto k) -> int {
+        const int smem = VEC ? s.smem : 0;
+        if (smem > 48 * 1024) ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        k<<<grid, s.threads, smem, st>>>(a, s.wpr, s.depth);
+        return launch_status();
+    };
+    if (s.nch == 1) return go(ln_fwd_kernel<T, W, 1, 256, VEC, DROP>);
+    if (s.nch == 2)
+        return s.threads <= 256 ? go(ln_fwd_kernel<T, W, 2, 256, VEC, DROP>) : go(ln_fwd_kernel<T, W, 2, 512, VEC, DROP>);
+    return s.threads <= 256 ? go(ln_fwd_kernel<T, W, 4, 256, VEC, DROP>) : go(ln_fwd_kernel<T, W, 4, 512, VEC, DROP>);
 }
 
-template <typename T, typename W, int NCH, bool VEC, bool DROP>
+template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP>
 static int bwd_main(const BwdArgs<T, W> &a, const Shape &s, int grid, cudaStream_t st) {
-    auto k = ln_bwd_kernel<T, W, NCH, VEC, DROP>;
-    const int smem = s.wpr == 1 && a.part ? (int)(s.rows_per_cta * 2 * a.cols * 4) : 0;
-    if (smem > 48 * 1024) ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    k<<<grid, s.threads, smem, st>>>(a, s.wpr);
+    auto k = ln_bwd_kernel<T, W, NCH, MAXT, VEC, DROP>;
+    if (s.smem > 48 * 1024) ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem));
+    k<<<grid, s.threads, s.smem, st>>>(a, s.wpr, s.depth);
     return launch_status();
 }
 
@@ -601,11 +826,14 @@ static int bwd_launch(BwdArgs<T, W> a, W *dw, W *db, void *ws, cudaStream_t st) 
         ln_bwd_cols_kernel<T, W, VEC, DROP><<<grid, 128, 0, st>>>(a, sums);
         rc = launch_status();
     } else {
-        const Shape s = shape_of(a.cols);
+        const Shape s = shape_of(a.cols, sizeof(T), DROP ? 3 : 2, true);
         parts = grid_of(s, a.rows);
-        rc = s.nch == 1   ? bwd_main<T, W, 1, VEC, DROP>(a, s, parts, st)
-             : s.nch == 2 ? bwd_main<T, W, 2, VEC, DROP>(a, s, parts, st)
-                          : bwd_main<T, W, 4, VEC, DROP>(a, s, parts, st);
+        const bool small = s.threads <= 256;
+        rc = s.nch == 1   ? bwd_main<T, W, 1, 256, VEC, DROP>(a, s, parts, st)
+             : s.nch == 2 ? (small ? bwd_main<T, W, 2, 256, VEC, DROP>(a, s, parts, st)
+                                   : bwd_main<T, W, 2, 512, VEC, DROP>(a, s, parts, st))
+                          : (small ? bwd_main<T, W, 4, 256, VEC, DROP>(a, s, parts, st)
+                                   : bwd_main<T, W, 4, 512, VEC, DROP>(a, s, parts, st));
     }
     if (rc || !a.part) return rc;
     ln_bwd_finish_kernel<W><<<(unsigned)((2 * a.cols + 31) / 32), 256, 0, st>>>(a.part, parts, a.cols, dw, db);
@@ -650,14 +878,15 @@ extern "C" int actcomp_dropout(const actcomp_drop_args *g, void *stream) {
     ACT_CHECK(aligned(g->x, es) && aligned(g->y, es) && aligned(g->seed_ptr, 8), ACT_E_ALIGN);
     const bool vec = g->cols % 8 == 0 && vec_ok(g->x, g->ldx, es) && vec_ok(g->y, g->ldy, es);
     const int64_t warps = g->rows * ((g->cols + SEG - 1) / SEG);
-    const int64_t cap = (int64_t)num_sms() * 16, ctas = (warps + 7) / 8;
+    const int64_t cap = (int64_t)num_sms() * 8, ctas = (warps + 7) / 8;
     const int grid = (int)(ctas < cap ? ctas : cap);
     cudaStream_t st = as_stream(stream);
     return with_types(g->dtype, 0, [&](auto t, auto) {
         using T = decltype(t);
         DropArgs<T> a{static_cast<const T *>(g->x), static_cast<T *>(g->y), g->rows, g->cols, g->ldx, g->ldy, d};
-        if (vec) dropout_kernel<T, true><<<grid, 256, 0, st>>>(a);
-        else dropout_kernel<T, false><<<grid, 256, 0, st>>>(a);
+        const int64_t segs = (a.cols + SEG - 1) / SEG, step = (int64_t)grid * 8;
+        if (vec) dropout_kernel<T, true><<<grid, 256, 0, st>>>(a, segs, step / segs, step % segs);
+        else dropout_kernel<T, false><<<grid, 256, 0, st>>>(a, segs, step / segs, step % segs);
         return launch_status();
     });
 }

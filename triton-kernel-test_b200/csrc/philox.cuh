@@ -53,8 +53,8 @@ __device__ __forceinline__ uint32_t drop_keep8(uint64_t row, uint32_t block, uin
     uint32_t keep = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        keep |= ((w[j] & 0xffffu) >= threshold ? 1u : 0u) << (2 * j);
-        keep |= ((w[j] >> 16) >= threshold ? 2u : 0u) << (2 * j);
+        if ((w[j] & 0xffffu) >= threshold) keep |= 1u << (2 * j);
+        if ((w[j] >> 16) >= threshold) keep |= 2u << (2 * j);
     }
     return keep;
 }
