@@ -1,11 +1,18 @@
 // mx4_quant.cu -- microscaled 4-bit quantisation (by rows, by columns, or both)
 // and its inverse; the format is stated in include/actcomp.h.
 //
-// HBM-bound: by rows 2 bytes in and 17/32 out per bf16 value.  Four lanes share
-// a block of 32 values, eight consecutive values each: loads and code stores
-// are contiguous over the warp, the block's largest magnitude takes two
-// shuffles, and a warp's 256 values fill two whole scale words.
+// HBM-bound: 2 bytes in and 17/32 out per bf16 value and direction.
+//   rows   a lane takes eight consecutive values, four lanes a block of 32: loads
+//          and code stores are contiguous over the warp, the block's largest
+//          magnitude takes two shuffles, a warp's 256 values fill two scale words.
+//   tiles  by columns, or both ways from one read: a CTA takes 128 x 128 values
+//          through shared memory; the column direction needs 32 rows of a column
+//          in one thread, and whole 64-byte pieces of the output's rows (one K
+//          atom) leave together.
 #include <cuda_fp16.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "mx4.cuh"
 
@@ -20,131 +27,325 @@ template <>
 __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <>
 __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+// Eight values as their words; zero() is eight zeros in every type.
 template <typename T>
-struct alignas(16) Raw8 {
-    T v[8];
+struct Raw8 {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load_vec(const T *p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const uint4 q = reinterpret_cast<const uint4 *>(p)[i];
+            w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+        }
+    }
+    // n of them, the others zero
+    __device__ __forceinline__ void load(const T *p, int n) {
+        zero();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) {
+                if constexpr (sizeof(T) == 4) {
+                    w[j] = reinterpret_cast<const uint32_t *>(p)[j];
+                } else {
+                    w[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[j] << (16 * (j & 1));
+                }
+            }
+    }
+    __device__ __forceinline__ void floats(float (&f)[8]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                    f[2 * j] = __uint_as_float(w[j] << 16);
+                    f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                } else {
+                    __half2 h;
+                    memcpy(&h, &w[j], 4);
+                    const float2 t = __half22float2(h);
+                    f[2 * j] = t.x, f[2 * j + 1] = t.y;
+                }
+            }
+        }
+    }
+    // The largest magnitude's bits: 16-bit types in both halves of the word to
+    // be folded by amax_bits, float32 as it is.
+    __device__ __forceinline__ uint32_t amax() const {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, w[j] & 0x7fffffffu);
+            return m;
+        } else {
+            uint32_t m = __vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu);
+            return __vmaxu2(m, __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+        }
+    }
 };
-
-__device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
-
-// By rows: one warp per 256 columns of a row, rows rounded up to whole atoms.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
-    quant_rows_kernel(const T *x, int64_t rows, int64_t cols, int64_t ldx, uint8_t *codes, uint8_t *scales) {
-    const int lane = threadIdx.x & 31;
-    const int64_t segs = (cols + 255) / 256, nka = atoms_of(cols), rb = row_bytes(cols);
-    const int64_t total = (rows + 127) / 128 * 128 * segs;
-    const int64_t step = (int64_t)gridDim.x * 8;
-    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < total; i += step) {
-        const int64_t r = i / segs, sg = i - r * segs;
-        const int64_t c = sg * 256 + 8 * lane;
-        float v[8] = {};
-        uint32_t m = 0;
-        if (r < rows) {
-            Raw8<T> raw;
-            if (VEC) {
-                uint4 *d = reinterpret_cast<uint4 *>(&raw);
-                const uint4 *s = reinterpret_cast<const uint4 *>(x + r * ldx + c);
-#pragma unroll
-                for (int k = 0; k < (int)sizeof(raw) / 16; ++k) d[k] = c < cols ? s[k] : make_uint4(0, 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) raw.v[j] = c + j < cols ? x[r * ldx + c + j] : from_f<T>(0.f);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = to_f<T>(raw.v[j]);
-                m = max(m, abs_bits(v[j]));
-            }
-        }
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const uint32_t sc = scale_code(m);
-        if (r < rows && c < blocks_of(cols) * BLOCK) {
-            const float inv = inv_scale(sc);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= inv;
-            *reinterpret_cast<uint32_t *>(codes + r * rb + c / 2) = pack8(v);
-        }
-        // four blocks' scale bytes to one word (lanes 0 and 16)
-        uint32_t w = sc;
-        w |= __shfl_down_sync(0xffffffffu, w, 4) << 8;
-        w |= __shfl_down_sync(0xffffffffu, w, 8) << 16;
-        const int64_t ka = sg * 2 + (lane >> 4);
-        if ((lane & 15) == 0 && ka < nka) *reinterpret_cast<uint32_t *>(scales + scale_word(r, ka, nka)) = w;
+template <typename T>
+__device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) return max(a, b);
+    else return __vmaxu2(a, b);
+}
+// Magnitude bits as float32 bits (NaN stays above infinity above the finite).
+template <typename T>
+__device__ __forceinline__ uint32_t amax_bits(uint32_t m) {
+    if constexpr (sizeof(T) == 4) {
+        return m;
+    } else {
+        const uint32_t h = max(m & 0xffffu, m >> 16);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return h << 16;
+        else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
     }
 }
 
-// By columns: a thread takes one column over 32 rows, a row of threads 256
-// neighbouring columns.
-template <typename T>
+// By rows: one warp per 256 columns of a row, two rows at a time; blockIdx.y
+// covers the columns, blockIdx.x strides over the rows, rounded up to atoms.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-    quant_cols_kernel(const T *x, int64_t rows, int64_t cols, int64_t ldx, uint8_t *codes, uint8_t *scales) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;  // over cols rounded up to 128
-    const int64_t nka = atoms_of(rows), rb = row_bytes(rows), nb = blocks_of(rows);
-    if (c >= (cols + 127) / 128 * 128) return;
-    for (int64_t b = blockIdx.y; b < nka * ATOM_BLOCKS; b += gridDim.y) {
-        uint32_t m = 0;
-        float v[32];
+    quant_rows_kernel(const T *x, int64_t rows, int64_t cols, int64_t ldx, uint8_t *codes, uint8_t *scales) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sg = blockIdx.y;
+    const int64_t nka = atoms_of(cols), rb = row_bytes(cols), c = (int64_t)sg * 256 + 8 * lane;
+    const int64_t all = (rows + 127) / 128 * 128, step = (int64_t)gridDim.x * 8;
+    const int n = c >= cols ? 0 : (cols - c < 8 ? (int)(cols - c) : 8);
+    const bool code = c < blocks_of(cols) * BLOCK;
+    const int64_t ka = sg * 2 + (lane >> 4);
+    const bool word = (lane & 15) == 0 && ka < nka;
+    constexpr int UNROLL = 2;
+    for (int64_t r0 = (int64_t)blockIdx.x * 8 + warp; r0 < all; r0 += UNROLL * step) {
+        Raw8<T> raw[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int64_t r = r0 + u * step;
+            if (r < rows && n == 8 && VEC) raw[u].load_vec(x + r * ldx + c);
+            else if (r < rows && n > 0) raw[u].load(x + r * ldx + c, n);
+            else raw[u].zero();
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int64_t r = r0 + u * step;
+            uint32_t m = raw[u].amax();
+            m = max_of<T>(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = max_of<T>(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const uint32_t sc = scale_code(amax_bits<T>(m));
+            if (r < rows && code) {
+                const float inv = inv_scale(sc);
+                float v[8];
+                raw[u].floats(v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= inv;
+                *reinterpret_cast<uint32_t *>(codes + r * rb + c / 2) = pack8(v);
+            }
+            // four blocks' scale bytes to one word (lanes 0 and 16)
+            uint32_t w = sc;
+            w |= __shfl_down_sync(0xffffffffu, w, 4) << 8;
+            w |= __shfl_down_sync(0xffffffffu, w, 8) << 16;
+            if (word && r < all) *reinterpret_cast<uint32_t *>(scales + scale_word(r, ka, nka)) = w;
+        }
+    }
+}
+
+// A CTA's 128 x 128 tile: x rows r0.., columns c0... Shared memory holds it as
+// rows of PITCH values; every thread then takes one column of 32 rows at a time
+// (two neighbouring columns of a 16-bit type: one word a row).
+//   BY_ROWS: the tile's rows are quantised too, from the same read.
+template <typename T, bool VEC, bool BY_ROWS>
+__global__ void __launch_bounds__(256)
+    quant_tile_kernel(const T *x, int64_t rows, int64_t cols, int64_t ldx, uint8_t *codes, uint8_t *scales,
+                      uint8_t *codes_t, uint8_t *scales_t) {
+    constexpr int PITCH = 128 + 16 / (int)sizeof(T);  // 16-byte rows, a shift of four banks from row to row
+    extern __shared__ __align__(16) uint8_t dyn[];
+    T *tile = reinterpret_cast<T *>(dyn);
+    uint32_t *words = reinterpret_cast<uint32_t *>(dyn + 128 * PITCH * sizeof(T));  // 128 columns x 4 scale bytes
+    const int ctiles = (int)((cols + 127) / 128), kr = blockIdx.x / ctiles, kc = blockIdx.x - kr * ctiles;
+    const int64_t r0 = (int64_t)kr * 128, c0 = (int64_t)kc * 128;
+    const int tid = threadIdx.x, lane = tid & 31;
+    // in: sixteen lanes a row, eight values a lane
+    const int64_t nka = atoms_of(cols), rb = row_bytes(cols);
+    const int64_t c = c0 + (tid & 15) * 8;
+    const int n = c >= cols ? 0 : (cols - c < 8 ? (int)(cols - c) : 8);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        Raw8<T> raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t r = r0 + 64 * h + 16 * i + (tid >> 4);
+            if (r < rows && n == 8 && VEC) raw[i].load_vec(x + r * ldx + c);
+            else if (r < rows && n > 0) raw[i].load(x + r * ldx + c, n);
+            else raw[i].zero();
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int lr = 64 * h + 16 * i + (tid >> 4);
+            const int64_t r = r0 + lr;
+            uint4 *d = reinterpret_cast<uint4 *>(tile + lr * PITCH + (tid & 15) * 8);
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+                d[k] = make_uint4(raw[i].w[4 * k], raw[i].w[4 * k + 1], raw[i].w[4 * k + 2], raw[i].w[4 * k + 3]);
+            if constexpr (BY_ROWS) {
+                uint32_t m = raw[i].amax();
+                m = max_of<T>(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max_of<T>(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const uint32_t sc = scale_code(amax_bits<T>(m));
+                if (r < rows && c < blocks_of(cols) * BLOCK) {
+                    const float inv = inv_scale(sc);
+                    float v[8];
+                    raw[i].floats(v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] *= inv;
+                    *reinterpret_cast<uint32_t *>(codes + r * rb + c / 2) = pack8(v);
+                }
+                uint32_t w = sc;
+                w |= __shfl_down_sync(0xffffffffu, w, 4) << 8;
+                w |= __shfl_down_sync(0xffffffffu, w, 8) << 16;
+                if ((lane & 15) == 0) *reinterpret_cast<uint32_t *>(scales + scale_word(r, kc, nka)) = w;
+            }
+        }
+    }
+    __syncthreads();
+    // by columns: warp = (block of 32 rows, half of the columns), two columns a lane
+    const int64_t nka_t = atoms_of(rows), rb_t = row_bytes(rows);
+    const int b = tid >> 6, pair = tid & 63;  // columns 2 pair, 2 pair + 1
+    const bool live = r0 + 32 * b < rows;     // the block exists
+    uint32_t sc2[2];
+    uint32_t code[2][4];
+    if constexpr (sizeof(T) == 2) {
+        uint32_t w[32], m = 0;
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-            const int64_t r = b * 32 + j;
-            v[j] = c < cols && r < rows ? to_f<T>(x[r * ldx + c]) : 0.f;
-            m = max(m, abs_bits(v[j]));
+            w[j] = *reinterpret_cast<const uint32_t *>(tile + (32 * b + j) * PITCH + 2 * pair);
+            m = __vmaxu2(m, w[j] & 0x7fff7fffu);
         }
-        const uint32_t sc = scale_code(m);
-        if (c < cols && b < nb) {
-            const float inv = inv_scale(sc);
-            uint32_t w[4];
+        sc2[0] = scale_code(amax_bits<T>(m & 0xffffu));
+        sc2[1] = scale_code(amax_bits<T>(m >> 16));
+        const float inv[2] = {inv_scale(sc2[0]), inv_scale(sc2[1])};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float lo[8], hi[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t u = w[8 * k + j];
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                    lo[j] = __uint_as_float(u << 16) * inv[0];
+                    hi[j] = __uint_as_float(u & 0xffff0000u) * inv[1];
+                } else {
+                    __half2 h;
+                    memcpy(&h, &u, 4);
+                    const float2 t = __half22float2(h);
+                    lo[j] = t.x * inv[0], hi[j] = t.y * inv[1];
+                }
+            }
+            code[0][k] = pack8(lo);
+            code[1][k] = pack8(hi);
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            float v[32];
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                v[j] = to_f<T>(tile[(32 * b + j) * PITCH + 2 * pair + s]);
+                m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+            }
+            sc2[s] = scale_code(m);
+            const float inv = inv_scale(sc2[s]);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 float t[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) t[j] = v[8 * k + j] * inv;
-                w[k] = pack8(t);
+                code[s][k] = pack8(t);
             }
-            *reinterpret_cast<uint4 *>(codes + c * rb + b * 16) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        scales[scale_word(c, b >> 2, nka) + (b & 3)] = (uint8_t)sc;
     }
+    __syncthreads();  // the tile has been read: its space takes the codes, 128 columns x 64 bytes (and a pad of 16)
+    uint8_t *out = dyn;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const int col = 2 * pair + s;
+        *reinterpret_cast<uint4 *>(out + col * 80 + 16 * b) =
+            make_uint4(code[s][0], code[s][1], code[s][2], code[s][3]);
+        reinterpret_cast<uint8_t *>(words)[col * 4 + b] = live ? (uint8_t)sc2[s] : 0;
+    }
+    __syncthreads();
+    // out: four lanes a column's 64 bytes
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int col = 64 * i + (tid >> 2), q = tid & 3;
+        if (c0 + col < cols && r0 + 32 * q < rows)
+            *reinterpret_cast<uint4 *>(codes_t + (c0 + col) * rb_t + r0 / 2 + 16 * q) =
+                *reinterpret_cast<const uint4 *>(out + col * 80 + 16 * q);
+    }
+    if (tid < 128)
+        *reinterpret_cast<uint32_t *>(scales_t + scale_word(c0 + tid, kr, nka_t)) = words[tid];
 }
 
-// One lane per eight values.
+// By rows like quant_rows_kernel: a lane eight values, a warp 256 columns.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     dequant_kernel(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, T *out, int64_t ldo) {
-    const int64_t per_row = (cols + 7) / 8, nka = atoms_of(cols), rb = row_bytes(cols);
-    const int64_t total = rows * per_row, step = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-        const int64_t r = i / per_row, g = i - r * per_row;
-        uint32_t h[4];
-        unpack8(*reinterpret_cast<const uint32_t *>(codes + r * rb + g * 4), h);
-        const float s = scale_value(scales[scale_word(r, g >> 4, nka) + ((g >> 2) & 3)]);
-        Raw8<T> o;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.y * 256 + 8 * lane;
+    if (c >= cols) return;
+    const int64_t nka = atoms_of(cols), rb = row_bytes(cols), step = (int64_t)gridDim.x * 8;
+    const int n = cols - c < 8 ? (int)(cols - c) : 8;
+    constexpr int UNROLL = 4;
+    for (int64_t r0 = (int64_t)blockIdx.x * 8 + warp; r0 < rows; r0 += UNROLL * step) {
+        uint32_t q[UNROLL];
+        uint8_t sc[UNROLL];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[k]));
-            o.v[2 * k] = from_f<T>(f.x * s);
-            o.v[2 * k + 1] = from_f<T>(f.y * s);
+        for (int u = 0; u < UNROLL; ++u) {
+            const int64_t r = r0 + u * step;
+            q[u] = 0, sc[u] = 0;
+            if (r < rows) {
+                q[u] = *reinterpret_cast<const uint32_t *>(codes + r * rb + c / 2);
+                sc[u] = scales[scale_word(r, c >> 7, nka) + ((c >> 5) & 3)];
+            }
         }
-        T *d = out + r * ldo + g * 8;
-        if (VEC) {
-            const uint4 *src = reinterpret_cast<const uint4 *>(&o);
 #pragma unroll
-            for (int k = 0; k < (int)sizeof(o) / 16; ++k) reinterpret_cast<uint4 *>(d)[k] = src[k];
-        } else {
+        for (int u = 0; u < UNROLL; ++u) {
+            const int64_t r = r0 + u * step;
+            if (r >= rows) break;
+            uint32_t h[4];
+            unpack8(q[u], h);
+            const float s = scale_value(sc[u]);
+            uint32_t w[2 * sizeof(T)];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (g * 8 + j < cols) d[j] = o.v[j];
+            for (int k = 0; k < 4; ++k) {
+                __half2 h2;
+                memcpy(&h2, &h[k], 4);
+                const float2 f = mul2(__half22float2(h2), make_float2(s, s));
+                if constexpr (sizeof(T) == 4) {
+                    w[2 * k] = __float_as_uint(f.x), w[2 * k + 1] = __float_as_uint(f.y);
+                } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                    w[k] = pack_bf16x2(f.x, f.y);
+                } else {
+                    const __half2 o = __float22half2_rn(f);
+                    memcpy(&w[k], &o, 4);
+                }
+            }
+            T *d = out + r * ldo + c;
+            if (VEC && n == 8) {
+#pragma unroll
+                for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+                    reinterpret_cast<uint4 *>(d)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < n) {
+                        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(d)[j] = w[j];
+                        else reinterpret_cast<uint16_t *>(d)[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                    }
+            }
         }
     }
 }
@@ -164,6 +365,16 @@ static int check(const actcomp_mx4 *q) {
     return ACT_OK;
 }
 
+// Grid of the row kernels: y covers the columns, x the rows with enough CTAs to
+// fill the device `waves` times over.
+static bool row_grid(dim3 &g, int64_t rows, int64_t cols, int waves) {
+    const int64_t segs = (cols + 255) / 256, need = (rows + 7) / 8;
+    if (segs > 65535) return false;
+    int64_t x = ((int64_t)num_sms() * waves + segs - 1) / segs;
+    g = dim3((unsigned)(x < need ? x : need), (unsigned)segs);
+    return true;
+}
+
 }  // namespace mx4
 int mx4_check(const actcomp_mx4 *q) { return mx4::check(q); }
 }  // namespace act
@@ -180,6 +391,7 @@ extern "C" int actcomp_mx4_quantize(const void *x, int64_t rows, int64_t cols, i
     using namespace act;
     using namespace act::mx4;
     ACT_CHECK(x && (q || qt) && rows > 0 && cols > 0 && ldx >= cols && dtype >= 0 && dtype <= 2, ACT_E_INVALID);
+    const int64_t tiles = ((cols + 127) / 128) * ((rows + 127) / 128);
     if (q) {
         ACT_CHECK(q->rows == rows && q->cols == cols, ACT_E_INVALID);
         if (int st = check(q)) return st;
@@ -187,28 +399,31 @@ extern "C" int actcomp_mx4_quantize(const void *x, int64_t rows, int64_t cols, i
     if (qt) {
         ACT_CHECK(qt->rows == cols && qt->cols == rows, ACT_E_INVALID);
         if (int st = check(qt)) return st;
+        ACT_CHECK(tiles <= INT32_MAX, ACT_E_UNSUPPORTED);
     }
     const int es = dtype == 0 ? 4 : 2;
     ACT_CHECK(aligned(x, es), ACT_E_ALIGN);
+    const bool vec = aligned(x, 16) && (ldx * es) % 16 == 0;
+    dim3 grid;
+    if (!qt) ACT_CHECK(row_grid(grid, (rows + 127) / 128 * 128, cols, 16), ACT_E_UNSUPPORTED);
     cudaStream_t st = as_stream(stream);
-    return with_type(dtype, [&](auto t) {
+    return with_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
         const T *xs = static_cast<const T *>(x);
-        if (q) {
-            const bool vec = cols % 8 == 0 && aligned(x, 16) && (ldx * es) % 16 == 0;
-            const int64_t warps = (rows + 127) / 128 * 128 * ((cols + 255) / 256);
-            const int64_t cap = (int64_t)num_sms() * 16, ctas = (warps + 7) / 8;
-            const int grid = (int)(ctas < cap ? ctas : cap);
+        if (!qt) {
             if (vec) quant_rows_kernel<T, true><<<grid, 256, 0, st>>>(xs, rows, cols, ldx, q->codes, q->scales);
             else quant_rows_kernel<T, false><<<grid, 256, 0, st>>>(xs, rows, cols, ldx, q->codes, q->scales);
-            if (int rc = launch_status()) return rc;
+            return launch_status();
         }
-        if (qt) {
-            const int64_t nb = atoms_of(rows) * ATOM_BLOCKS;
-            const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)(nb < 65535 ? nb : 65535));
-            quant_cols_kernel<T><<<grid, 256, 0, st>>>(xs, rows, cols, ldx, qt->codes, qt->scales);
-        }
-        return launch_status();
+        const int smem = 128 * (128 + 16 / (int)sizeof(T)) * (int)sizeof(T) + 512;
+        auto go = [&](auto k) -> int {
+            if (smem > 48 * 1024) ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            k<<<(unsigned)tiles, 256, smem, st>>>(xs, rows, cols, ldx, q ? q->codes : nullptr, q ? q->scales : nullptr, qt->codes,
+                                    qt->scales);
+            return launch_status();
+        };
+        if (q) return vec ? go(quant_tile_kernel<T, true, true>) : go(quant_tile_kernel<T, false, true>);
+        return vec ? go(quant_tile_kernel<T, true, false>) : go(quant_tile_kernel<T, false, false>);
     });
 }
 
@@ -219,9 +434,9 @@ extern "C" int actcomp_mx4_dequantize(const actcomp_mx4 *q, void *out, int64_t l
     ACT_CHECK(out && ldo >= q->cols && dtype >= 0 && dtype <= 2, ACT_E_INVALID);
     const int es = dtype == 0 ? 4 : 2;
     ACT_CHECK(aligned(out, es), ACT_E_ALIGN);
-    const bool vec = q->cols % 8 == 0 && aligned(out, 16) && (ldo * es) % 16 == 0;
-    const int64_t ctas = (q->rows * ((q->cols + 7) / 8) + 255) / 256, cap = (int64_t)num_sms() * 16;
-    const int grid = (int)(ctas < cap ? ctas : cap);
+    const bool vec = aligned(out, 16) && (ldo * es) % 16 == 0;
+    dim3 grid;
+    ACT_CHECK(row_grid(grid, q->rows, q->cols, 16), ACT_E_UNSUPPORTED);
     cudaStream_t st = as_stream(stream);
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);

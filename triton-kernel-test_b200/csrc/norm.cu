@@ -213,35 +213,40 @@ template <typename T>
 struct DropArgs {
     const T *x;
     T *y;
-    int64_t rows, cols, ldx, ldy;
+    int64_t cols, ldx, ldy;
     DropParams d;
 };
 
-// One warp per segment of 256 values, two segments in flight; a warp's next
-// segment lies grid-many further on, which is `dr` rows and `ds` segments.
+// One warp per segment of 256 values, grid-stride over `units` = rows x segs
+// segments (32-bit: longer tensors take several launches); row = unit / segs by
+// a multiplication (`mul`, `shift`: exact for 32-bit dividends, or mul 0 for
+// segs == 1).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) dropout_kernel(DropArgs<T> a, int64_t segs, int64_t dr, int64_t ds) {
+__global__ void __launch_bounds__(256) dropout_kernel(DropArgs<T> a, uint32_t units, uint32_t segs, uint32_t mul,
+                                                      uint32_t shift) {
     const int lane = threadIdx.x & 31;
     const uint64_t key = drop_seed(a.d);
-    const int64_t first = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    int64_t r = first / segs, sg = first - r * segs;
-    while (r < a.rows) {
-        int64_t rr[2], s0[2];
-        int n[2];
-        Raw8<T> x[2];
+    const uint32_t step = gridDim.x * 8u;
+    constexpr int UNROLL = 2;
+    for (uint32_t u0 = blockIdx.x * 8u + (threadIdx.x >> 5); u0 < units; u0 += UNROLL * step) {
+        Raw8<T> x[UNROLL];
+        uint32_t row[UNROLL], seg0[UNROLL];
+        int n[UNROLL];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            rr[u] = r, s0[u] = sg * SEG;
-            n[u] = r < a.rows ? count_of<VEC>(s0[u], a.cols, lane) : 0;
-            x[u] = load8<T, VEC>(a.x + r * a.ldx, s0[u], n[u], lane);
-            r += dr, sg += ds;
-            if (sg >= segs) sg -= segs, ++r;
+        for (int k = 0; k < UNROLL; ++k) {
+            const uint32_t u = u0 + k * step;
+            const uint32_t hi = __umulhi(u, mul);
+            row[k] = mul ? (((u - hi) >> 1) + hi) >> shift : u;
+            seg0[k] = (u - row[k] * segs) * SEG;
+            n[k] = u < units && u >= u0 ? count_of<VEC>(seg0[k], a.cols, lane) : 0;
+            x[k] = load8<T, VEC>(a.x + row[k] * a.ldx, seg0[k], n[k], lane);
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const F8 y = drop8<VEC>(unpack<T>(x[u]), a.d.row_offset + (uint64_t)rr[u], s0[u], lane, key, a.d);
-            store8<T, VEC>(a.y + rr[u] * a.ldy, s0[u], n[u], lane, y);
+        for (int k = 0; k < UNROLL; ++k) {
+            const F8 y = drop8<VEC>(unpack<T>(x[k]), a.d.row_offset + row[k], seg0[k], lane, key, a.d);
+            store8<T, VEC>(a.y + row[k] * a.ldy, seg0[k], n[k], lane, y);
         }
+        if (u0 + UNROLL * step < u0) break;
     }
 }
 
@@ -258,19 +263,31 @@ struct FwdArgs {
 };
 
 // Sum of v over the warps that share a row; every thread gets the same value.
+// red: NW entries, zero where there is no warp.
+template <int NW>
 __device__ __forceinline__ float row_sum(float v, float *red, int wpr, int warp, int lane) {
     v = warp_sum(v);
     if (wpr == 1) return v;
     if (lane == 0) red[warp] = v;
     __syncthreads();
-    float s = 0.f;
-    for (int i = 0; i < wpr; ++i) s += red[i];
-    return s;
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NW / 4; ++i) {
+        const float4 q = reinterpret_cast<const float4 *>(red)[i];
+        s = add2(add2(s, make_float2(q.x, q.y)), make_float2(q.z, q.w));
+    }
+    return s.x + s.y;
+}
+// 1 / sqrt(v): the hardware's approximation and one Newton step (the IEEE square
+// root and division cost 40 instructions a row and warp).
+__device__ __forceinline__ float inv_sqrt(float v) {
+    const float r = rsqrtf(v), h = r * __fmaf_rn(-0.5f * v * r, r, 1.5f);
+    return v > 0.f && v < INFINITY ? h : r;
 }
 
-// Resident CTAs of 256 threads that the register use allows.
-__host__ __device__ constexpr int fwd_ctas(int nch) { return nch <= 2 ? 3 : 2; }
-constexpr int BWD_CTAS = 2;
+// Resident CTAs for launches of up to 256 or 512 threads (register use).
+__host__ __device__ constexpr int fwd_ctas(int nch, int maxt) { return maxt > 256 ? 1 : (nch == 1 ? 3 : 2); }
+__host__ __device__ constexpr int bwd_ctas(int maxt) { return maxt > 256 ? 1 : 2; }
 constexpr int MAX_DEPTH = 4;
 constexpr int RING_HEAD = 8 * MAX_DEPTH * 8 + 16;  // barriers of up to eight warps' rings, the abort word
 
@@ -316,9 +333,12 @@ struct RowRing {
 
 // MAXT: the launch's thread count rounded up to 256 or 512.
 template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 ? fwd_ctas(NCH) : 1) ln_fwd_kernel(FwdArgs<T, W> a, int wpr, int depth) {
+__global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdArgs<T, W> a, int wpr, int depth) {
     extern __shared__ __align__(128) uint8_t dyn[];
-    __shared__ float red[2][32];
+    constexpr int NW = MAXT / 32;
+    __shared__ __align__(16) float red[2][NW];
+    if (threadIdx.x < 2 * NW) red[0][threadIdx.x] = 0.f;
+    __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
     const int rpc = wpr == 1 ? nwarps : 1;  // rows a CTA has in hand at once
     const int w0 = wpr == 1 ? 0 : warp, mine = wpr == 1 ? warp : 0;
@@ -367,7 +387,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? fwd_ctas(NCH) : 1) ln_fwd_
 #pragma unroll
             for (int j = 0; j < 4; ++j) s = add2(s, v[i].p[j]);
         }
-        const float mean = row_sum(s.x + s.y, red[0], wpr, warp, lane) * inv_n;
+        const float mean = row_sum<NW>(s.x + s.y, red[0], wpr, warp, lane) * inv_n;
         if constexpr (VEC) {  // every reader of the slot is past its reads
             if (wpr == 1) __syncwarp();
             if (leader) fill(ring.slot, r + depth * step);
@@ -387,8 +407,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? fwd_ctas(NCH) : 1) ln_fwd_
                 if (!VEC || n[i]) q = fma2(v[i].p[j], v[i].p[j], q);
             }
         }
-        const float var = row_sum(q.x + q.y, red[1], wpr, warp, lane) * inv_n;
-        const float rstd = 1.f / sqrtf(var + a.eps);
+        const float var = row_sum<NW>(q.x + q.y, red[1], wpr, warp, lane) * inv_n;
+        const float rstd = inv_sqrt(var + a.eps);
         if (lane == 0 && w0 == 0) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
@@ -411,8 +431,9 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? fwd_ctas(NCH) : 1) ln_fwd_
 // (the later ones mostly from L2).
 template <typename T, typename W, bool VEC, bool DROP>
 __global__ void __launch_bounds__(LONG_THREADS) ln_fwd_long_kernel(FwdArgs<T, W> a) {
-    __shared__ float red[2][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = LONG_THREADS / 32;
+    constexpr int nw = LONG_THREADS / 32;
+    __shared__ __align__(16) float red[2][nw];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float inv_n = 1.f / (float)a.cols;
     const uint64_t key = DROP ? drop_seed(a.d) : 0;
     const int64_t segs = (a.cols + SEG - 1) / SEG;
@@ -433,7 +454,7 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_fwd_long_kernel(FwdArgs<T, W>
             const float2 t = add2(add2(v.p[0], v.p[1]), add2(v.p[2], v.p[3]));
             s += t.x + t.y;
         }
-        const float mean = row_sum(s, red[0], nw, warp, lane) * inv_n;
+        const float mean = row_sum<nw>(s, red[0], nw, warp, lane) * inv_n;
         const float2 mean2 = make_float2(mean, mean);
         float q = 0.f;
         for (int64_t g = warp; g < segs; g += nw) {
@@ -449,8 +470,8 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_fwd_long_kernel(FwdArgs<T, W>
             }
             q += t.x + t.y;
         }
-        const float var = row_sum(q, red[1], nw, warp, lane) * inv_n;
-        const float rstd = 1.f / sqrtf(var + a.eps);
+        const float var = row_sum<nw>(q, red[1], nw, warp, lane) * inv_n;
+        const float rstd = inv_sqrt(var + a.eps);
         if (threadIdx.x == 0) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
@@ -481,6 +502,7 @@ struct BwdArgs {
     DropParams d;
 };
 
+template <int NW>
 __device__ __forceinline__ float2 row_sum2(float u, float v, float2 *red, int wpr, int warp, int lane) {
     u = warp_sum(u);
     v = warp_sum(v);
@@ -488,16 +510,20 @@ __device__ __forceinline__ float2 row_sum2(float u, float v, float2 *red, int wp
     if (lane == 0) red[warp] = make_float2(u, v);
     __syncthreads();
     float2 s = make_float2(0.f, 0.f);
-    for (int i = 0; i < wpr; ++i) {
-        s.x += red[i].x;
-        s.y += red[i].y;
+#pragma unroll
+    for (int i = 0; i < NW / 2; ++i) {
+        const float4 q = reinterpret_cast<const float4 *>(red)[i];
+        s = add2(add2(s, make_float2(q.x, q.y)), make_float2(q.z, q.w));
     }
     return s;
 }
 
 template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 ? BWD_CTAS : 1) ln_bwd_kernel(BwdArgs<T, W> a, int wpr, int depth) {
-    __shared__ float2 red[2][32];
+__global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T, W> a, int wpr, int depth) {
+    constexpr int NW = MAXT / 32;
+    __shared__ __align__(16) float2 red[2][NW];
+    if (threadIdx.x < 2 * NW) red[0][threadIdx.x] = make_float2(0.f, 0.f);
+    __syncthreads();
     extern __shared__ __align__(128) uint8_t dyn[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
     const int rpc = wpr == 1 ? nwarps : 1;
@@ -523,13 +549,15 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? BWD_CTAS : 1) ln_bwd_kerne
     // Up to two segments a thread the row's g and x-hat are held from the sums to
     // the output, past that they are computed again from the slot (registers).
     constexpr bool HOLD = NCH <= 2;
-    Raw8<W> wv[NCH];
+    // four segments: their sums fill the registers, the weights are read again too
+    constexpr bool WREG = NCH <= 2;
+    Raw8<W> wv[WREG ? NCH : 1];
     F8 dw[NCH], db[NCH];
     int n[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         n[i] = count_of<VEC>((w0 + i * wpr) * SEG, a.cols, lane);
-        wv[i] = load8_or<W, VEC>(a.w, 1.f, (w0 + i * wpr) * SEG, n[i], lane);
+        if constexpr (WREG) wv[i] = load8_or<W, VEC>(a.w, 1.f, (w0 + i * wpr) * SEG, n[i], lane);
 #pragma unroll
         for (int j = 0; j < 4; ++j) dw[i].p[j] = db[i].p[j] = make_float2(0.f, 0.f);
     }
@@ -544,6 +572,14 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? BWD_CTAS : 1) ln_bwd_kerne
         float2 s1 = make_float2(0.f, 0.f), s2 = s1;
         F8 gh[HOLD ? NCH : 1], xh[HOLD ? NCH : 1];
         if constexpr (VEC) ring.wait(dyn);
+        auto weights = [&](int i) {
+            if constexpr (WREG) {
+                stay_packed(wv[i]);
+                return unpack<W>(wv[i]);
+            } else {
+                return unpack<W>(load8_or<W, VEC>(a.w, 1.f, (w0 + i * wpr) * SEG, n[i], lane));
+            }
+        };
         auto values = [&](int i, F8 &dy, F8 &x) {  // dy and x-hat
             const int seg0 = (w0 + i * wpr) * SEG;
             dy = unpack<T>(load8<T, VEC>(yr, seg0, n[i], lane));
@@ -555,8 +591,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? BWD_CTAS : 1) ln_bwd_kerne
         for (int i = 0; i < NCH; ++i) {
             F8 dy, x;
             values(i, dy, x);
-            stay_packed(wv[i]);
-            const F8 w = unpack<W>(wv[i]);
+            const F8 w = weights(i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {  // dy is 0 past the row's end
                 const float2 g = mul2(dy.p[j], w.p[j]);
@@ -567,7 +602,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? BWD_CTAS : 1) ln_bwd_kerne
                 if constexpr (HOLD) gh[i].p[j] = g, xh[i].p[j] = x.p[j];
             }
         }
-        const float2 s = row_sum2(s1.x + s1.y, s2.x + s2.y, red[turn & 1], wpr, warp, lane);
+        const float2 s = row_sum2<NW>(s1.x + s1.y, s2.x + s2.y, red[turn & 1], wpr, warp, lane);
         if constexpr (VEC) {  // the row before this one has been read by all
             if (wpr == 1) __syncwarp();
             if (leader && turn > 0) fill(ring.slot == 0 ? depth - 1 : ring.slot - 1, r + (depth - 1) * step);
@@ -583,8 +618,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? BWD_CTAS : 1) ln_bwd_kerne
                 g = gh[i], x = xh[i];
             } else {
                 values(i, g, x);
-                stay_packed(wv[i]);
-                const F8 w = unpack<W>(wv[i]);
+                const F8 w = weights(i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) g.p[j] = mul2(g.p[j], w.p[j]);
             }
@@ -634,8 +668,9 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? BWD_CTAS : 1) ln_bwd_kerne
 // Rows longer than MAX_SEGS segments, first kernel: the row's two sums.
 template <typename T, typename W, bool VEC>
 __global__ void __launch_bounds__(LONG_THREADS) ln_bwd_sums_kernel(BwdArgs<T, W> a, float2 *sums) {
-    __shared__ float2 red[2][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = LONG_THREADS / 32;
+    constexpr int nw = LONG_THREADS / 32;
+    __shared__ __align__(16) float2 red[2][nw];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float inv_n = 1.f / (float)a.cols;
     const int64_t segs = (a.cols + SEG - 1) / SEG;
     int turn = 0;
@@ -658,7 +693,7 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_bwd_sums_kernel(BwdArgs<T, W>
             s1 += t1.x + t1.y;
             s2 += t2.x + t2.y;
         }
-        const float2 s = row_sum2(s1, s2, red[turn], nw, warp, lane);
+        const float2 s = row_sum2<nw>(s1, s2, red[turn], nw, warp, lane);
         turn ^= 1;
         if (threadIdx.x == 0) sums[r] = make_float2(s.x * inv_n, s.y * inv_n);
     }
@@ -744,13 +779,13 @@ static Shape shape_of(int64_t cols, int esize, int inputs, bool bwd) {
     if (segs <= 4) {
         s = {segs <= 1 ? 1 : (segs <= 2 ? 2 : 4), 1, 256, 8, 0, 0, 0};
     } else {
-        s.nch = segs <= 32 ? 2 : 4;
+        s.nch = bwd ? (segs <= 32 ? 2 : 4) : (segs <= 8 ? 1 : segs <= 16 ? 2 : segs <= 24 ? 3 : 4);
         s.wpr = (segs + s.nch - 1) / s.nch;
         s.threads = 32 * s.wpr;
         s.rows_per_cta = 1;
     }
     const int64_t slot = cols * esize * inputs * s.rows_per_cta;
-    s.per_sm = s.threads <= 256 ? (bwd ? BWD_CTAS : fwd_ctas(s.nch)) : 1;
+    s.per_sm = bwd ? bwd_ctas(s.threads) : fwd_ctas(s.nch, s.threads);
     const int64_t room = 220 * 1024 / s.per_sm - 2048;
     s.depth = (int)(room / slot < MAX_DEPTH ? room / slot : MAX_DEPTH);
     if (s.depth < 2) {  // the longest rows: one CTA per SM
@@ -780,7 +815,7 @@ static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 static size_t bwd_workspace(int64_t rows, int64_t cols) {
     if (is_long(cols)) return up256((size_t)long_parts(rows, cols) * 2 * cols * 4) + up256((size_t)rows * 8);
-    const int64_t ctas = cols <= 4 * SEG ? (rows + 7) / 8 : rows, cap = (int64_t)num_sms() * BWD_CTAS;
+    const int64_t ctas = cols <= 4 * SEG ? (rows + 7) / 8 : rows, cap = (int64_t)num_sms() * 2;
     return up256((size_t)(ctas < cap ? ctas : cap) * 2 * cols * 4);
 }
 
@@ -800,8 +835,8 @@ static int fwd_launch(const FwdArgs<T, W> &a, cudaStream_t st) {
         return launch_status();
     };
     if (s.nch == 1) return go(ln_fwd_kernel<T, W, 1, 256, VEC, DROP>);
-    if (s.nch == 2)
-        return s.threads <= 256 ? go(ln_fwd_kernel<T, W, 2, 256, VEC, DROP>) : go(ln_fwd_kernel<T, W, 2, 512, VEC, DROP>);
+    if (s.nch == 2) return go(ln_fwd_kernel<T, W, 2, 256, VEC, DROP>);
+    if (s.nch == 3) return go(ln_fwd_kernel<T, W, 3, 256, VEC, DROP>);
     return s.threads <= 256 ? go(ln_fwd_kernel<T, W, 4, 256, VEC, DROP>) : go(ln_fwd_kernel<T, W, 4, 512, VEC, DROP>);
 }
 
@@ -877,17 +912,29 @@ extern "C" int actcomp_dropout(const actcomp_drop_args *g, void *stream) {
     const int es = g->dtype == 0 ? 4 : 2;
     ACT_CHECK(aligned(g->x, es) && aligned(g->y, es) && aligned(g->seed_ptr, 8), ACT_E_ALIGN);
     const bool vec = g->cols % 8 == 0 && vec_ok(g->x, g->ldx, es) && vec_ok(g->y, g->ldy, es);
-    const int64_t warps = g->rows * ((g->cols + SEG - 1) / SEG);
-    const int64_t cap = (int64_t)num_sms() * 8, ctas = (warps + 7) / 8;
-    const int grid = (int)(ctas < cap ? ctas : cap);
+    // division by segs: quotient of a 32-bit u = (((u - h) >> 1) + h) >> (l - 1), h = umulhi(u, mul),
+    // l = ceil(log2 segs), mul = floor(2^32 (2^l - segs) / segs) + 1
+    const uint32_t segs = (uint32_t)((g->cols + SEG - 1) / SEG);
+    uint32_t l = 0;
+    while (((uint64_t)1 << l) < segs) ++l;
+    const uint32_t mul = segs > 1 ? (uint32_t)((((((uint64_t)1 << l) - segs) << 32) / segs) + 1) : 0;
+    const int64_t most = 0x7fffffff / segs;  // rows a launch
     cudaStream_t st = as_stream(stream);
     return with_types(g->dtype, 0, [&](auto t, auto) {
         using T = decltype(t);
-        DropArgs<T> a{static_cast<const T *>(g->x), static_cast<T *>(g->y), g->rows, g->cols, g->ldx, g->ldy, d};
-        const int64_t segs = (a.cols + SEG - 1) / SEG, step = (int64_t)grid * 8;
-        if (vec) dropout_kernel<T, true><<<grid, 256, 0, st>>>(a, segs, step / segs, step % segs);
-        else dropout_kernel<T, false><<<grid, 256, 0, st>>>(a, segs, step / segs, step % segs);
-        return launch_status();
+        for (int64_t r = 0; r < g->rows; r += most) {
+            const int64_t rows = g->rows - r < most ? g->rows - r : most;
+            DropArgs<T> a{static_cast<const T *>(g->x) + r * g->ldx, static_cast<T *>(g->y) + r * g->ldy, g->cols,
+                          g->ldx, g->ldy, d};
+            a.d.row_offset += (uint64_t)r;
+            const uint32_t units = (uint32_t)(rows * segs);
+            const int64_t cap = (int64_t)num_sms() * 8, ctas = ((int64_t)units + 7) / 8;
+            const int grid = (int)(ctas < cap ? ctas : cap);
+            if (vec) dropout_kernel<T, true><<<grid, 256, 0, st>>>(a, units, segs, mul, l - 1);
+            else dropout_kernel<T, false><<<grid, 256, 0, st>>>(a, units, segs, mul, l - 1);
+            if (int rc = launch_status()) return rc;
+        }
+        return (int)ACT_OK;
     });
 }
 
