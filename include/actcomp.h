@@ -466,6 +466,15 @@ int actcomp_mx4_dequantize(const actcomp_mx4 *q, void *out, int64_t ldo, int32_t
  * accumulation on the tensor cores; c_dtype 0 = float32, 1 = bf16, 2 = fp16. */
 int actcomp_mx4_gemm(const actcomp_mx4 *a, const actcomp_mx4 *b, void *c, int64_t ldc, int32_t c_dtype, void *stream);
 
+/* c = x . w^T (tokens x w->rows) for up to ACTCOMP_MX4_LINEAR_TOKENS tokens in one
+ * kernel: x (tokens x w->cols, dtype as above, row stride ldx) is quantised by
+ * rows on the way.  c_dtype: dtype or 0.  ACT_E_UNSUPPORTED for more tokens, or
+ * where 36 bytes per token and block of 32 columns pass 160 KiB (quantise, then
+ * actcomp_mx4_gemm). */
+#define ACTCOMP_MX4_LINEAR_TOKENS 4
+int actcomp_mx4_linear(const void *x, int64_t tokens, int64_t cols, int64_t ldx, int32_t dtype, const actcomp_mx4 *w,
+                       void *c, int64_t ldc, int32_t c_dtype, void *stream);
+
 /* Error statistics of a reconstruction against its original (n bf16 values):
  * out[0] += sum (a-b)^2, out[1] += sum b^2, out[2] = max(out[2], max|a-b|),
  * out[3] += count(a != b); out: 4 doubles of device memory (accumulated into,

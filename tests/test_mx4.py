@@ -98,6 +98,12 @@ def test_sizes_and_validation_without_gpu():
     assert gemm(d(), d(64, 128)) == _lib.ACT_E_INVALID and gemm(d(), d(), ld=63) == _lib.ACT_E_INVALID
     assert gemm(d(), d(), dt=5) == _lib.ACT_E_INVALID and gemm(d(), d(), c=P + 1) == _lib.ACT_E_ALIGN
     assert gemm(d(), d(0, 96)) == _lib.ACT_E_INVALID
+    lin = lambda t=1, k=96, ld=96, x=P, w=None, o=1: lib.actcomp_mx4_linear(  # noqa: E731
+        x, t, k, ld, 1, w or d(), P, 64, o, None)
+    assert lin(0) == _lib.ACT_E_INVALID and lin(k=64) == _lib.ACT_E_INVALID and lin(ld=8) == _lib.ACT_E_INVALID
+    assert lin(o=2) == _lib.ACT_E_INVALID and lin(x=P + 1) == _lib.ACT_E_ALIGN
+    assert lin(_lib.MX4_LINEAR_TOKENS + 1) == _lib.ACT_E_UNSUPPORTED
+    assert lin(4, 1 << 20, 1 << 20, w=d(64, 1 << 20)) == _lib.ACT_E_UNSUPPORTED  # x outgrows shared memory
     assert lib.actcomp_mx4_dequantize(d(), P, 95, 1, None) == _lib.ACT_E_INVALID
     assert lib.actcomp_mx4_dequantize(d(1 << 31), P, 96, 1, None) == _lib.ACT_E_UNSUPPORTED
 
@@ -252,6 +258,43 @@ def test_linear_step(tokens, k, n):
         assert got.shape == ref.shape
         assert not ((got.double() - ref).abs() > 2.0 ** -8 * ref.abs() + a.shape[1] * 2.0 ** -22 * mag).any()
     assert mx4.linear(x.view(1, tokens, k), wq).shape == (1, tokens, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("n,k", [(1, 1), (40, 96), (129, 1000), (300, 33), (64, 16384), (1000, 2080), (4096, 4096)])
+def test_few_tokens(tokens, n, k):
+    """The few-token kernel (and, at five tokens, the tensor cores) on the same operands."""
+    from actcomp import mx4
+
+    w = mx4.quantize(data(n, k, torch.bfloat16, n).cuda())
+    for dt in DTYPES:
+        x = data(tokens, k, dt, k)
+        for xs in (x.cuda(), torch.nn.functional.pad(x, (3, 6)).cuda()[:, 3:3 + k]):
+            q = values(mx4.quantize(x.cuda())).cuda()
+            for out in {dt, torch.float32}:
+                got = mx4.linear(xs, w, out)
+                ref, mag = q @ values(w).cuda().t(), q.abs() @ values(w).abs().cuda().t()
+                assert got.shape == ref.shape and got.dtype == out
+                ok = (got.double() - ref).abs() <= U[out] * ref.abs() + k * 2.0 ** -23 * mag * (1 + U[out]) + 1e-7
+                if out == torch.float16:
+                    ok |= got.isinf() & (torch.sign(got) == torch.sign(ref)) & (ref.abs() + k * 2.0 ** -23 * mag >= 65520)
+                assert ok.all(), (dt, out, int((~ok).sum()))
+
+
+@pytest.mark.gpu
+def test_few_tokens_extreme_scales():
+    """Block scales near both ends of float32's range: products that are in range come out exactly."""
+    from actcomp import mx4
+
+    x, w = torch.zeros(2, 64), torch.zeros(3, 64)
+    x[0, 0], x[1, 32] = 6 * 2.0 ** 124, 1.5 * 2.0 ** -127
+    w[0, 0], w[1, 32], w[2, 0] = 1.5 * 2.0 ** -120, 3 * 2.0 ** 120, 4 * 2.0 ** -126
+    want = x.double() @ w.double().t()
+    assert torch.equal(mx4.linear(x.cuda(), mx4.quantize(w.cuda())).double().cpu(), want)
+    x[0, 1] = float("inf")
+    y = mx4.linear(x.cuda(), mx4.quantize(w.cuda())).cpu()
+    assert y[0].isnan().all() and torch.equal(y[1].double(), want[1])
 
 
 @pytest.mark.gpu

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -40,6 +41,9 @@ ACT_RC_HALF_EVEN = 2
 ACT_RC_SCALE_BATCH = 4
 ACT_RC_ROW_PACK = 8
 ACT_RC_OUTLIER_BF16 = 16
+
+
+MX4_LINEAR_TOKENS = 4  # ACTCOMP_MX4_LINEAR_TOKENS
 
 
 class CgDesc(ctypes.Structure):
@@ -113,6 +117,19 @@ class Mx4Desc(ctypes.Structure):
     _fields_ = [("rows", c_i64), ("cols", c_i64), ("codes", c_vp), ("scales", c_vp)]
 
 
+_CODES = {c_i64: "q", ctypes.c_uint64: "Q", c_i32: "i", c_vp: "P", ctypes.c_double: "d", ctypes.c_float: "f"}
+
+
+def packer(cls) -> struct.Struct:
+    """``cls``'s layout as a struct.Struct (native alignment): packing a dozen
+    fields takes a quarter of the time of building the ctypes structure, which
+    counts where a call's host time is most of it."""
+    st = struct.Struct("@" + "".join(_CODES[t] for _, t in cls._fields_))
+    if st.size != ctypes.sizeof(cls):
+        raise ImportError(f"{cls.__name__}: packed layout differs from the C layout")
+    return st
+
+
 #: entry point -> (restype, argtypes); mirrors include/actcomp.h
 SIGNATURES = {
     "actcomp_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -156,6 +173,8 @@ SIGNATURES = {
     "actcomp_mx4_quantize": (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_i32, ctypes.POINTER(Mx4Desc),
                                             ctypes.POINTER(Mx4Desc), c_vp]),
     "actcomp_mx4_dequantize": (ctypes.c_int, [ctypes.POINTER(Mx4Desc), c_vp, c_i64, c_i32, c_vp]),
+    "actcomp_mx4_linear": (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_i32, ctypes.POINTER(Mx4Desc), c_vp, c_i64,
+                                          c_i32, c_vp]),
     "actcomp_mx4_gemm": (ctypes.c_int, [ctypes.POINTER(Mx4Desc), ctypes.POINTER(Mx4Desc), c_vp, c_i64, c_i32, c_vp]),
 }
 
@@ -198,6 +217,16 @@ class ActcompError(RuntimeError):
 def check(fn: str, status: int) -> None:
     if status != ACT_OK:
         raise ActcompError(fn, status)
+
+
+def entry(name: str):
+    """The entry point as a function object of its own that takes structures as
+    packed bytes (any pointer argument takes bytes or an address)."""
+    res, args = SIGNATURES[name]
+    fn = load()[name]
+    fn.restype = res
+    fn.argtypes = [c_vp if isinstance(t, type) and issubclass(t, ctypes._Pointer) else t for t in args]
+    return fn
 
 
 def call(name: str, *args) -> None:

@@ -20,16 +20,21 @@ the weight gradient contracts dy and x over tokens, both quantised by columns.
 """
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass
 from typing import Optional
 
 import torch
 
 from . import _lib
-from ._lib import Mx4Desc, call
-from .core import _need_cuda, _stream
+from .core import _launch, _need_cuda
 from .norm import _DT, _dtype
+
+_desc_args = _lib.packer(_lib.Mx4Desc).pack
+_quant_fn, _dequant_fn = _lib.entry("actcomp_mx4_quantize"), _lib.entry("actcomp_mx4_dequantize")
+_gemm_fn, _linear_fn = _lib.entry("actcomp_mx4_gemm"), _lib.entry("actcomp_mx4_linear")
+
+#: x's values and scales in a few-token product, bytes of shared memory
+_SMALL_BYTES = 160 * 1024
 
 BLOCK = 32
 
@@ -57,14 +62,15 @@ class Mx4:
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
 
-    def desc(self) -> Mx4Desc:
-        return Mx4Desc(self.rows, self.cols, self.codes.data_ptr(), self.scales.data_ptr())
+    def desc(self) -> bytes:
+        """The packed actcomp_mx4 structure."""
+        return _desc_args(self.rows, self.cols, self.codes.data_ptr(), self.scales.data_ptr())
 
 
-def _empty(rows: int, cols: int, dtype: torch.dtype, device) -> Mx4:
-    codes = torch.empty((rows, (cols + 31) // 32 * 16), dtype=torch.uint8, device=device)
-    scales = torch.empty(((rows + 127) // 128 * ((cols + 127) // 128) * 512,), dtype=torch.uint8, device=device)
-    return Mx4(rows, cols, codes, scales, dtype)
+def _empty(x: torch.Tensor, rows: int, cols: int) -> Mx4:
+    codes = x.new_empty((rows, (cols + 31) // 32 * 16), dtype=torch.uint8)
+    scales = x.new_empty(((rows + 127) // 128 * ((cols + 127) // 128) * 512,), dtype=torch.uint8)
+    return Mx4(rows, cols, codes, scales, x.dtype)
 
 
 def _matrix(x: torch.Tensor) -> torch.Tensor:
@@ -82,11 +88,10 @@ def _quantize(x: torch.Tensor, by_rows: bool, by_cols: bool) -> tuple[Optional[M
     dt = _dtype(x)
     x2 = _matrix(x)
     rows, cols = x2.shape
-    q = _empty(rows, cols, x.dtype, x.device) if by_rows else None
-    qt = _empty(cols, rows, x.dtype, x.device) if by_cols else None
-    with torch.cuda.device(x.device):
-        call("actcomp_mx4_quantize", x2.data_ptr(), rows, cols, max(x2.stride(0), cols), dt,
-             ctypes.byref(q.desc()) if by_rows else None, ctypes.byref(qt.desc()) if by_cols else None, _stream(x))
+    q = _empty(x, rows, cols) if by_rows else None
+    qt = _empty(x, cols, rows) if by_cols else None
+    _launch("actcomp_mx4_quantize", _quant_fn, x.device, x2.data_ptr(), rows, cols, max(x2.stride(0), cols), dt,
+            q.desc() if by_rows else None, qt.desc() if by_cols else None)
     return q, qt
 
 
@@ -109,9 +114,8 @@ def dequantize(q: Mx4, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     dtype = dtype or q.dtype
     if dtype not in _DT:
         raise TypeError(f"float32, bfloat16 or float16 expected, got {dtype}")
-    out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.device)
-    with torch.cuda.device(q.device):
-        call("actcomp_mx4_dequantize", ctypes.byref(q.desc()), out.data_ptr(), q.cols, _DT[dtype], _stream(out))
+    out = q.codes.new_empty((q.rows, q.cols), dtype=dtype)
+    _launch("actcomp_mx4_dequantize", _dequant_fn, out.device, q.desc(), out.data_ptr(), q.cols, _DT[dtype])
     return out
 
 
@@ -125,18 +129,38 @@ def matmul(a: Mx4, b: Mx4, out_dtype: Optional[torch.dtype] = None) -> torch.Ten
         raise ValueError(f"inner dimensions differ: {a.cols} vs {b.cols}")
     if a.device != b.device:
         raise ValueError(f"operands on {a.device} and {b.device}")
-    out = torch.empty((a.rows, b.rows), dtype=dtype, device=a.device)
-    with torch.cuda.device(a.device):
-        call("actcomp_mx4_gemm", ctypes.byref(a.desc()), ctypes.byref(b.desc()), out.data_ptr(), b.rows, _DT[dtype],
-             _stream(out))
+    out = a.codes.new_empty((a.rows, b.rows), dtype=dtype)
+    _launch("actcomp_mx4_gemm", _gemm_fn, out.device, a.desc(), b.desc(), out.data_ptr(), b.rows, _DT[dtype])
+    return out
+
+
+def _few_tokens(x: torch.Tensor, w: Mx4, out_dtype: Optional[torch.dtype]) -> bool:
+    tokens = x.numel() // w.cols
+    return (0 < tokens <= _lib.MX4_LINEAR_TOKENS and tokens * ((w.cols + 31) // 32) * 36 <= _SMALL_BYTES
+            and (out_dtype is None or out_dtype is x.dtype or out_dtype is torch.float32))
+
+
+def _linear_few(x: torch.Tensor, w: Mx4, out_dtype: Optional[torch.dtype]) -> torch.Tensor:
+    _need_cuda(x)
+    dt = _dtype(x)
+    if x.device != w.device:
+        raise ValueError(f"operands on {x.device} and {w.device}")
+    x2 = _matrix(x)
+    dtype = out_dtype or x.dtype
+    out = x.new_empty(x.shape[:-1] + (w.rows,), dtype=dtype)
+    _launch("actcomp_mx4_linear", _linear_fn, x.device, x2.data_ptr(), x2.shape[0], w.cols, max(x2.stride(0), w.cols),
+            dt, w.desc(), out.data_ptr(), w.rows, _DT[dtype])
     return out
 
 
 def linear(x: torch.Tensor, w: Mx4, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x . w^T for x (..., K) and w (N, K) in 4 bits: x is quantised by rows on
-    the way; (..., N) of ``out_dtype`` (default: x's)."""
+    the way; (..., N) of ``out_dtype`` (default: x's).  Up to four tokens take one
+    kernel that reads the weight at memory speed, more the tensor cores."""
     if x.shape[-1] != w.cols:
         raise ValueError(f"x has {x.shape[-1]} columns, the weight {w.cols}")
+    if _few_tokens(x, w, out_dtype):
+        return _linear_few(x, w, out_dtype)
     return matmul(quantize(x), w, out_dtype).view(x.shape[:-1] + (w.rows,))
 
 
@@ -145,6 +169,8 @@ def linear_forward(x: torch.Tensor, w: Mx4, out_dtype: Optional[torch.dtype] = N
     weight gradient needs of it."""
     if x.shape[-1] != w.cols:
         raise ValueError(f"x has {x.shape[-1]} columns, the weight {w.cols}")
+    if _few_tokens(x, w, out_dtype):
+        return _linear_few(x, w, out_dtype), quantize(x, transpose=True)
     q, saved = quantize_pair(x)
     return matmul(q, w, out_dtype).view(x.shape[:-1] + (w.rows,)), saved
 

@@ -22,17 +22,25 @@ masks); ``p`` is held to 16 bits (``round(p * 65536) / 65536``) and the scale
 uses the held value."""
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Union
 
 import torch
 
 from . import _lib
-from ._lib import DropArgs, LnArgs, LnBwdArgs, call
-from .core import _need_cuda, _ptr, _stream
+from .core import _launch, _need_cuda, _ptr
 
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 Seed = Union[int, torch.Tensor]
+
+_drop_fn, _drop_args = _lib.entry("actcomp_dropout"), _lib.packer(_lib.DropArgs).pack
+_ln_fn, _ln_args = _lib.entry("actcomp_layer_norm"), _lib.packer(_lib.LnArgs).pack
+_bwd_fn, _bwd_args = _lib.entry("actcomp_layer_norm_bwd"), _lib.packer(_lib.LnBwdArgs).pack
+_bwd_workspace = _lib.entry("actcomp_layer_norm_bwd_workspace")
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of x's shape (a third of torch.empty's host time)."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _dtype(x: torch.Tensor) -> int:
@@ -42,15 +50,13 @@ def _dtype(x: torch.Tensor) -> int:
     return dt
 
 
-def _rows2d(x: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """x as rows x cols with unit column stride, and its row stride; copied
+def _rows2d(x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
+    """x as rows of ``cols`` with unit column stride, and its row stride; copied
     only if the leading dimensions have no common stride."""
-    cols = x.shape[-1]
     if x.is_contiguous():
         return x, cols
     if x.dim() == 1:
-        x = x.contiguous()
-        return x, cols
+        return x.contiguous(), cols
     try:
         x2 = x.view(-1, cols) if x.dim() != 2 else x
     except RuntimeError:
@@ -76,16 +82,16 @@ def _same(x: torch.Tensor, **others: Optional[torch.Tensor]) -> None:
                              f"({tuple(x.shape)} {x.dtype}), got {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
-def _affine(x: torch.Tensor, **vectors: Optional[torch.Tensor]) -> int:
-    """Checks weight-like vectors; returns their dtype code."""
+def _affine(x: torch.Tensor, cols: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor] = None) -> int:
+    """Checks weight and bias; returns their dtype code."""
     wdt = None
-    for name, t in vectors.items():
+    for t in (weight, bias):
         if t is None:
             continue
-        if t.shape != x.shape[-1:] or t.device != x.device:
-            raise ValueError(f"{name} must be a vector of {x.shape[-1]} values on {x.device}")
+        if t.dim() != 1 or t.numel() != cols or t.device != x.device:
+            raise ValueError(f"weight and bias must be vectors of {cols} values on {x.device}")
         if t.dtype != x.dtype and t.dtype != torch.float32:
-            raise TypeError(f"{name} must be {x.dtype} or float32, got {t.dtype}")
+            raise TypeError(f"weight and bias must be {x.dtype} or float32, got {t.dtype}")
         if wdt is not None and t.dtype != wdt:
             raise TypeError("weight and bias must have one dtype")
         wdt = t.dtype
@@ -129,15 +135,14 @@ def dropout(x: torch.Tensor, p: float, seed: Seed, row_offset: int = 0,
     rows, cols = _geometry(x)
     seed, seed_ptr, row_offset = _draw(x, p, seed, row_offset)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _like(x)
     else:
         _same(x, out=out)
         if not out.is_contiguous():
             raise ValueError("out must be contiguous")
-    x2, ldx = _rows2d(x)
-    a = DropArgs(rows, cols, x2.data_ptr(), ldx, out.data_ptr(), cols, dt, 0, p, seed, seed_ptr, row_offset)
-    with torch.cuda.device(x.device):
-        call("actcomp_dropout", ctypes.byref(a), _stream(x))
+    x2, ldx = _rows2d(x, cols)
+    _launch("actcomp_dropout", _drop_fn, x.device,
+            _drop_args(rows, cols, x2.data_ptr(), ldx, out.data_ptr(), cols, dt, 0, p, seed, seed_ptr, row_offset))
     return out
 
 
@@ -149,23 +154,22 @@ def dropout_backward(dy: torch.Tensor, p: float, seed: Seed, row_offset: int = 0
 
 def _forward(x, res, weight, bias, eps, p, draw):
     dt = _dtype(x)
-    wdt = _affine(x, weight=weight, bias=bias)
     rows, cols = _geometry(x)
+    wdt = _affine(x, cols, weight, bias)
     if cols == 0:
         raise ValueError("layer norm over an empty last dimension")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    x2, ldx = _rows2d(x)
-    r2, ldr = _rows2d(res) if res is not None else (None, 0)
+    x2, ldx = _rows2d(x, cols)
+    r2, ldr = _rows2d(res, cols) if res is not None else (None, 0)
     weight, bias = _vec(weight), _vec(bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if res is not None else None
-    stats = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
-    a = LnArgs(rows, cols, x2.data_ptr(), ldx, _ptr(r2), ldr, _ptr(weight), _ptr(bias), y.data_ptr(), cols, _ptr(h),
-               cols, mean.data_ptr(), rstd.data_ptr(), dt, wdt, eps, 0, p, *draw)
-    with torch.cuda.device(x.device):
-        call("actcomp_layer_norm", ctypes.byref(a), _stream(x))
+    y = _like(x)
+    h = _like(x) if res is not None else None
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    _launch("actcomp_layer_norm", _ln_fn, x.device,
+            _ln_args(rows, cols, x2.data_ptr(), ldx, _ptr(r2), ldr, _ptr(weight), _ptr(bias), y.data_ptr(), cols,
+                     _ptr(h), cols, mean.data_ptr(), rstd.data_ptr(), dt, wdt, eps, 0, p, *draw))
     return y, h, mean, rstd
 
 
@@ -191,27 +195,28 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Opti
 
 def _backward(dy, x, weight, mean, rstd, p, draw, dh, fused, bias_grad):
     dt = _dtype(x)
-    wdt = _affine(x, weight=weight)
     rows, cols = _geometry(x)
+    wdt = _affine(x, cols, weight)
     if cols == 0:
         raise ValueError("layer norm over an empty last dimension")
     mean, rstd = _stats(rows, x, mean=mean, rstd=rstd)
-    dy2, lddy = _rows2d(dy)
-    x2, ldx = _rows2d(x)
-    dh2, lddh = _rows2d(dh) if dh is not None else (None, 0)
+    dy2, lddy = _rows2d(dy, cols)
+    x2, ldx = _rows2d(x, cols)
+    dh2, lddh = _rows2d(dh, cols) if dh is not None else (None, 0)
     weight = _vec(weight)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dr = torch.empty(x.shape, dtype=x.dtype, device=x.device) if fused else None
-    wt = x.dtype if weight is None else weight.dtype
-    dw = torch.empty((cols,), dtype=wt, device=x.device) if weight is not None else None
-    db = torch.empty((cols,), dtype=wt, device=x.device) if bias_grad else None
-    with torch.cuda.device(x.device):
-        need = _lib.load().actcomp_layer_norm_bwd_workspace(rows, cols)
-        ws = torch.empty((max(need, 1),), dtype=torch.uint8, device=x.device)
-        a = LnBwdArgs(rows, cols, dy2.data_ptr(), lddy, x2.data_ptr(), ldx, _ptr(dh2), lddh, _ptr(weight),
+    dx = _like(x)
+    dr = _like(x) if fused else None
+    dw = torch.empty_like(weight) if weight is not None else None
+    db = None
+    if bias_grad:
+        db = torch.empty_like(weight) if weight is not None else x.new_empty((cols,))
+    need = _bwd_workspace(rows, cols)
+    ws = x.new_empty((max(need, 1),), dtype=torch.uint8)
+    _launch("actcomp_layer_norm_bwd", _bwd_fn, x.device,
+            _bwd_args(rows, cols, dy2.data_ptr(), lddy, x2.data_ptr(), ldx, _ptr(dh2), lddh, _ptr(weight),
                       mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), cols, _ptr(dr), cols, _ptr(dw), _ptr(db), dt,
-                      wdt, p, *draw)
-        call("actcomp_layer_norm_bwd", ctypes.byref(a), ws.data_ptr(), need, _stream(x))
+                      wdt, p, *draw),
+            ws.data_ptr(), need)
     return dx, dr, dw, db
 
 

@@ -2,6 +2,11 @@
 // positions and the conversions of one value group.
 #pragma once
 
+#include <cuda_fp16.h>
+#include <string.h>
+
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace act {
@@ -37,24 +42,124 @@ __device__ __forceinline__ float scale_value(uint32_t code) {
 }
 
 // Eight scaled values to eight e2m1 codes, value j in nibble j (nearest, ties
-// to even, saturating).
-__device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
-    uint32_t r;
-    asm("{\n .reg .b8 a, b, c, d;\n"
-        " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
-        " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
-        " mov.b32 %0, {a, b, c, d};\n}"
-        : "=r"(r)
-        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+// to even, saturating).  Each byte leaves its asm block by itself: four of them
+// packed inside one block came out as zeros in some kernels (nvcc 12.9).
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint16_t r;
+    asm("{\n .reg .b8 t;\n cvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n mov.b16 %0, {t, 0};\n}" : "=h"(r) : "f"(lo), "f"(hi));
     return r;
 }
-// Eight codes to four pairs of fp16 (exact).
-__device__ __forceinline__ void unpack8(uint32_t codes, uint32_t (&h)[4]) {
-    asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
-        " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n cvt.rn.f16x2.e2m1x2 %2, c;\n"
-        " cvt.rn.f16x2.e2m1x2 %3, d;\n}"
-        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-        : "r"(codes));
+__device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
+    return pack2(v[0], v[1]) | pack2(v[2], v[3]) << 8 | pack2(v[4], v[5]) << 16 | pack2(v[6], v[7]) << 24;
+}
+// Codes j and j + 4 of a word as a pair of fp16 times 2^-14 (exact): the sign to
+// bit 15, exponent and mantissa to bits 11..9.  With fp16's bias of 15 against
+// e2m1's 1 that is the value times 2^-14, and e2m1's subnormal (exponent 0) is an
+// fp16 subnormal.  (The conversion instruction from e2m1 pairs takes the wrong
+// byte of the word in some kernels when nvcc 12.9 folds the shift into it.)
+template <int J>
+__device__ __forceinline__ uint32_t tiny_pair(uint32_t codes) {
+    const uint32_t m = J < 3 ? codes << (J < 3 ? 9 - 4 * J : 0) : codes >> 3;
+    return ((codes << (12 - 4 * J)) & 0x80008000u) | (m & 0x0e000e00u);
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t v) {
+    __half2 h;
+    memcpy(&h, &v, 4);
+    return h;
+}
+// The pairs (0, 4), (1, 5), (2, 6), (3, 7) times 2^-14.
+__device__ __forceinline__ void tiny8(uint32_t codes, __half2 (&h)[4]) {
+    h[0] = as_half2(tiny_pair<0>(codes));
+    h[1] = as_half2(tiny_pair<1>(codes));
+    h[2] = as_half2(tiny_pair<2>(codes));
+    h[3] = as_half2(tiny_pair<3>(codes));
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+
+// Eight values as their words; zero() is eight zeros in every type.
+template <typename T>
+struct Raw8 {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load_vec(const T *p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const uint4 q = reinterpret_cast<const uint4 *>(p)[i];
+            w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+        }
+    }
+    // n of them, the others zero
+    __device__ __forceinline__ void load(const T *p, int n) {
+        zero();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) {
+                if constexpr (sizeof(T) == 4) {
+                    w[j] = reinterpret_cast<const uint32_t *>(p)[j];
+                } else {
+                    w[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[j] << (16 * (j & 1));
+                }
+            }
+    }
+    __device__ __forceinline__ void floats(float (&f)[8]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                    f[2 * j] = __uint_as_float(w[j] << 16);
+                    f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                } else {
+                    __half2 h;
+                    memcpy(&h, &w[j], 4);
+                    const float2 t = __half22float2(h);
+                    f[2 * j] = t.x, f[2 * j + 1] = t.y;
+                }
+            }
+        }
+    }
+    // The largest magnitude's bits: 16-bit types in both halves of the word to
+    // be folded by amax_bits, float32 as it is.
+    __device__ __forceinline__ uint32_t amax() const {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, w[j] & 0x7fffffffu);
+            return m;
+        } else {
+            uint32_t m = __vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu);
+            return __vmaxu2(m, __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+        }
+    }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) return max(a, b);
+    else return __vmaxu2(a, b);
+}
+// Magnitude bits as float32 bits (NaN stays above infinity above the finite).
+template <typename T>
+__device__ __forceinline__ uint32_t amax_bits(uint32_t m) {
+    if constexpr (sizeof(T) == 4) {
+        return m;
+    } else {
+        const uint32_t h = max(m & 0xffffu, m >> 16);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return h << 16;
+        else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+    }
 }
 
 }  // namespace mx4

@@ -9,102 +9,10 @@
 //          through shared memory; the column direction needs 32 rows of a column
 //          in one thread, and whole 64-byte pieces of the output's rows (one K
 //          atom) leave together.
-#include <cuda_fp16.h>
-#include <string.h>
-
-#include <type_traits>
-
 #include "mx4.cuh"
 
 namespace act {
 namespace mx4 {
-
-template <typename T>
-__device__ __forceinline__ float to_f(T v);
-template <>
-__device__ __forceinline__ float to_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <>
-__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
-
-// Eight values as their words; zero() is eight zeros in every type.
-template <typename T>
-struct Raw8 {
-    uint32_t w[2 * sizeof(T)];
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < 2 * (int)sizeof(T); ++i) w[i] = 0;
-    }
-    __device__ __forceinline__ void load_vec(const T *p) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-            const uint4 q = reinterpret_cast<const uint4 *>(p)[i];
-            w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
-        }
-    }
-    // n of them, the others zero
-    __device__ __forceinline__ void load(const T *p, int n) {
-        zero();
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < n) {
-                if constexpr (sizeof(T) == 4) {
-                    w[j] = reinterpret_cast<const uint32_t *>(p)[j];
-                } else {
-                    w[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[j] << (16 * (j & 1));
-                }
-            }
-    }
-    __device__ __forceinline__ void floats(float (&f)[8]) const {
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                    f[2 * j] = __uint_as_float(w[j] << 16);
-                    f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-                } else {
-                    __half2 h;
-                    memcpy(&h, &w[j], 4);
-                    const float2 t = __half22float2(h);
-                    f[2 * j] = t.x, f[2 * j + 1] = t.y;
-                }
-            }
-        }
-    }
-    // The largest magnitude's bits: 16-bit types in both halves of the word to
-    // be folded by amax_bits, float32 as it is.
-    __device__ __forceinline__ uint32_t amax() const {
-        if constexpr (sizeof(T) == 4) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, w[j] & 0x7fffffffu);
-            return m;
-        } else {
-            uint32_t m = __vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu);
-            return __vmaxu2(m, __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-        }
-    }
-};
-template <typename T>
-__device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) {
-    if constexpr (sizeof(T) == 4) return max(a, b);
-    else return __vmaxu2(a, b);
-}
-// Magnitude bits as float32 bits (NaN stays above infinity above the finite).
-template <typename T>
-__device__ __forceinline__ uint32_t amax_bits(uint32_t m) {
-    if constexpr (sizeof(T) == 4) {
-        return m;
-    } else {
-        const uint32_t h = max(m & 0xffffu, m >> 16);
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) return h << 16;
-        else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
-    }
-}
 
 // By rows: one warp per 256 columns of a row, two rows at a time; blockIdx.y
 // covers the columns, blockIdx.x strides over the rows, rounded up to atoms.
@@ -294,10 +202,10 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     dequant_kernel(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, T *out, int64_t ldo) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ __align__(16) uint8_t turn[VEC ? 1 : 8][VEC ? 16 : 256 * sizeof(T)];
     const int64_t c = (int64_t)blockIdx.y * 256 + 8 * lane;
-    if (c >= cols) return;
     const int64_t nka = atoms_of(cols), rb = row_bytes(cols), step = (int64_t)gridDim.x * 8;
-    const int n = cols - c < 8 ? (int)(cols - c) : 8;
+    const int n = c >= cols ? 0 : (cols - c < 8 ? (int)(cols - c) : 8);
     constexpr int UNROLL = 4;
     for (int64_t r0 = (int64_t)blockIdx.x * 8 + warp; r0 < rows; r0 += UNROLL * step) {
         uint32_t q[UNROLL];
@@ -306,7 +214,7 @@ __global__ void __launch_bounds__(256)
         for (int u = 0; u < UNROLL; ++u) {
             const int64_t r = r0 + u * step;
             q[u] = 0, sc[u] = 0;
-            if (r < rows) {
+            if (r < rows && n > 0) {
                 q[u] = *reinterpret_cast<const uint32_t *>(codes + r * rb + c / 2);
                 sc[u] = scales[scale_word(r, c >> 7, nka) + ((c >> 5) & 3)];
             }
@@ -315,21 +223,24 @@ __global__ void __launch_bounds__(256)
         for (int u = 0; u < UNROLL; ++u) {
             const int64_t r = r0 + u * step;
             if (r >= rows) break;
-            uint32_t h[4];
-            unpack8(q[u], h);
+            __half2 h[4];
+            tiny8(q[u], h);
             const float s = scale_value(sc[u]);
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 t = mul2(__half22float2(__hmul2(h[k], __float2half2_rn(16384.f))), make_float2(s, s));
+                f[k] = t.x, f[k + 4] = t.y;
+            }
             uint32_t w[2 * sizeof(T)];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                __half2 h2;
-                memcpy(&h2, &h[k], 4);
-                const float2 f = mul2(__half22float2(h2), make_float2(s, s));
                 if constexpr (sizeof(T) == 4) {
-                    w[2 * k] = __float_as_uint(f.x), w[2 * k + 1] = __float_as_uint(f.y);
+                    w[2 * k] = __float_as_uint(f[2 * k]), w[2 * k + 1] = __float_as_uint(f[2 * k + 1]);
                 } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                    w[k] = pack_bf16x2(f.x, f.y);
+                    w[k] = pack_bf16x2(f[2 * k], f[2 * k + 1]);
                 } else {
-                    const __half2 o = __float22half2_rn(f);
+                    const __half2 o = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
                     memcpy(&w[k], &o, 4);
                 }
             }
@@ -338,13 +249,26 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
                 for (int k = 0; k < (int)sizeof(T) / 2; ++k)
                     reinterpret_cast<uint4 *>(d)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-            } else {
+            } else if (VEC) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (j < n) {
                         if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(d)[j] = w[j];
                         else reinterpret_cast<uint16_t *>(d)[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
                     }
+            } else {  // through shared memory, so that neighbouring lanes store neighbouring values
+                uint4 *mine = reinterpret_cast<uint4 *>(turn[warp]) + lane * (sizeof(T) / 2);
+#pragma unroll
+                for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+                    mine[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                __syncwarp();
+                T *row = out + r * ldo + (c - 8 * lane);
+                const int left = (int)(cols - (c - 8 * lane) < 256 ? cols - (c - 8 * lane) : 256);
+                const T *src = reinterpret_cast<const T *>(turn[warp]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (32 * j + lane < left) row[32 * j + lane] = src[32 * j + lane];
+                __syncwarp();
             }
         }
     }
