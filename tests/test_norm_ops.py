@@ -217,7 +217,7 @@ def test_dropout_keeps_the_stated_share():
 
 # ---------------------------------------------------------------- layer norm forward
 SHAPES = [(1, 1), (3, 5), (9, 64), (4, 257), (2, 1000), (5, 1024), (3, 2048), (7, 4096), (2, 4100), (300, 1032),
-          (3, 11008), (2, 16384), (2, 16385), (3, 20000)]
+          (3, 11008), (2, 16384), (2, 16385), (3, 20000), (1300, 4096), (900, 4095), (600, 16383), (4000, 130)]
 
 
 def bound_rows(x, rstd):
@@ -325,7 +325,8 @@ def check_backward(dtype, rows, cols, wide, fused, p=0.25, with_dh=True, view=No
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols", SHAPES + [(1500, 40), (777, 1001), (1200, 2056)])
+@pytest.mark.parametrize("rows,cols", SHAPES + [(1500, 40), (777, 1001), (1200, 2056), (400, 11008), (330, 13002),
+                                                  (320, 16384)])
 def test_layer_norm_backward(dtype, rows, cols):
     check_backward(dtype, rows, cols, wide=(rows + cols) % 2 == 0, fused=False)
 
@@ -333,7 +334,8 @@ def test_layer_norm_backward(dtype, rows, cols):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 5), (9, 64), (300, 1032), (2, 1001), (7, 4096), (3, 11008),
-                                       (2, 16385), (3, 20000), (520, 5120)])
+                                       (2, 16385), (3, 20000), (520, 5120), (320, 9001), (310, 9600),
+                                       (320, 16384), (3000, 33), (1300, 515)])
 def test_branch_backward(dtype, rows, cols):
     check_backward(dtype, rows, cols, wide=rows % 2 == 0, fused=True, with_dh=cols != 64)
 
@@ -399,7 +401,7 @@ def test_gradients_against_differences(cols):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 5), (9, 64), (300, 1032), (2, 1001), (7, 4096), (3, 11008),
-                                       (2, 16385), (3, 20000)])
+                                       (2, 16385), (3, 20000), (700, 4097), (640, 9001), (620, 16384), (5000, 19)])
 def test_branch_forward(dtype, rows, cols):
     import actcomp
 

@@ -40,6 +40,7 @@ namespace norm {
 constexpr int SEG = 256;            // values of a warp's segment
 constexpr int MAX_SEGS = 64;        // longest row held in registers: 16384 values
 constexpr int LONG_THREADS = 512;
+constexpr int SLOT_ROOM = 218 * 1024;  // shared memory for row slots
 
 // ---------------------------------------------------------------- types
 template <typename T>
@@ -264,19 +265,32 @@ struct FwdArgs {
 
 // Sum of v over the warps that share a row; every thread gets the same value.
 // red: NW entries, zero where there is no warp.
-template <int NW>
-__device__ __forceinline__ float row_sum(float v, float *red, int wpr, int warp, int lane) {
-    v = warp_sum(v);
-    if (wpr == 1) return v;
-    if (lane == 0) red[warp] = v;
-    __syncthreads();
-    float2 s = make_float2(0.f, 0.f);
+template <int NW, int R>
+__device__ __forceinline__ void row_sums(float (&v)[R], float (*red)[NW], int wpr, int warp, int lane) {
 #pragma unroll
-    for (int i = 0; i < NW / 4; ++i) {
-        const float4 q = reinterpret_cast<const float4 *>(red)[i];
-        s = add2(add2(s, make_float2(q.x, q.y)), make_float2(q.z, q.w));
+    for (int i = 0; i < R; ++i) v[i] = warp_sum(v[i]);
+    if (wpr == 1) return;
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) red[i][warp] = v[i];
     }
-    return s.x + s.y;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < NW / 4; ++i) {
+            const float4 q = reinterpret_cast<const float4 *>(red[k])[i];
+            s = add2(add2(s, make_float2(q.x, q.y)), make_float2(q.z, q.w));
+        }
+        v[k] = s.x + s.y;
+    }
+}
+template <int NW>
+__device__ __forceinline__ float row_sum(float v, float (*red)[NW], int wpr, int warp, int lane) {
+    float a[1] = {v};
+    row_sums<NW, 1>(a, red, wpr, warp, lane);
+    return a[0];
 }
 // 1 / sqrt(v): the hardware's approximation and one Newton step (the IEEE square
 // root and division cost 40 instructions a row and warp).
@@ -290,24 +304,39 @@ __host__ __device__ constexpr int fwd_ctas(int nch, int maxt) { return maxt > 25
 __host__ __device__ constexpr int bwd_ctas(int maxt) { return maxt > 256 ? 1 : 2; }
 constexpr int MAX_DEPTH = 4;
 constexpr int RING_HEAD = 8 * MAX_DEPTH * 8 + 16;  // barriers of up to eight warps' rings, the abort word
+// Bytes of a row in a slot.
+__host__ __device__ __forceinline__ uint32_t row_pitch(int64_t cols, int esize, bool vec) {
+    return (uint32_t)(vec ? cols * esize : (cols * esize + 15) / 16 * 16);
+}
+
+// One input's current row: values lo <= c < hi lie at s[c] in shared memory,
+// the others (a ragged row's ends) at g[c] in global memory.
+template <typename T>
+struct RowView {
+    const T *s, *g;
+    int lo, hi;
+};
 
 // The rows a CTA (or, with one warp per row, a warp) works through, brought to
-// shared memory ahead of their use: DEPTH slots, one bulk copy per input and
+// shared memory ahead of their use: `depth` slots, one bulk copy per input and
 // row, issued by one thread.  A slot is filled again once every reader has
-// passed the barrier that follows its last read.
-template <typename T, int INPUTS>
+// passed the barrier that follows its last read.  A bulk copy takes whole
+// 16-byte pieces: of a row that is not aligned so (VEC false) the pieces inside
+// it, which leaves up to seven 16-bit values at either end to plain loads.
+template <typename T, int INPUTS, bool VEC>
 struct RowRing {
     uint8_t *slots;
     uint64_t *bars;
-    uint32_t bytes;  // of one input's row
-    int depth, slot;
+    uint32_t pitch;  // of one input's row in a slot
+    int cols, depth, slot;
     uint32_t phase;
 
     // dyn: barriers of up to eight rings, the abort word, then the slots.
-    __device__ __forceinline__ void init(uint8_t *dyn, int which, uint32_t row_bytes, int d, bool leader) {
-        bytes = row_bytes, depth = d, slot = 0, phase = 0;
+    __device__ __forceinline__ void init(uint8_t *dyn, int which, int n, int d, bool leader) {
+        cols = n, depth = d, slot = 0, phase = 0;
+        pitch = row_pitch(n, sizeof(T), VEC);
         bars = reinterpret_cast<uint64_t *>(dyn) + which * MAX_DEPTH;
-        slots = dyn + RING_HEAD + (size_t)which * d * INPUTS * row_bytes;
+        slots = dyn + RING_HEAD + (size_t)which * d * INPUTS * pitch;
         if (threadIdx.x == 0) *abort_word(dyn) = 0;
         if (leader) {
             for (int i = 0; i < d; ++i) tc::mbar_init(&bars[i], 1);
@@ -318,26 +347,85 @@ struct RowRing {
     __device__ __forceinline__ static volatile int *abort_word(uint8_t *dyn) {
         return reinterpret_cast<volatile int *>(dyn + RING_HEAD - 16);
     }
-    __device__ __forceinline__ void fill(int s, int k, const T *row) {
-        if (k == 0) tc::mbar_arrive_expect_tx(&bars[s], bytes * INPUTS);
-        tc::bulk_load(slots + (s * INPUTS + k) * bytes, row, bytes, &bars[s]);
+    // Values before the row's first whole 16-byte piece, and up to the end of its last.
+    __device__ __forceinline__ void inside(const T *row, int &lo, int &hi) const {
+        const uint32_t a = (uint32_t)reinterpret_cast<uintptr_t>(row);
+        lo = (int)((0u - a) & 15u) / (int)sizeof(T);
+        hi = cols - (int)((a + (uint32_t)cols * (uint32_t)sizeof(T)) & 15u) / (int)sizeof(T);
+        if (hi <= lo) lo = hi = 0;
     }
-    __device__ __forceinline__ void wait(uint8_t *dyn) { tc::mbar_wait(&bars[slot], phase, abort_word(dyn)); }
-    __device__ __forceinline__ const T *row(int k) const {
-        return reinterpret_cast<const T *>(slots + (slot * INPUTS + k) * bytes);
+    __device__ __forceinline__ void fill(int s, const T *const (&row)[INPUTS]) {
+        if constexpr (VEC) {
+            tc::mbar_arrive_expect_tx(&bars[s], pitch * INPUTS);
+#pragma unroll
+            for (int k = 0; k < INPUTS; ++k)
+                tc::bulk_load(slots + (s * INPUTS + k) * pitch, row[k], pitch, &bars[s]);
+        } else {
+            int lo[INPUTS], hi[INPUTS];
+            uint32_t bytes = 0;
+#pragma unroll
+            for (int k = 0; k < INPUTS; ++k) {
+                inside(row[k], lo[k], hi[k]);
+                bytes += (uint32_t)(hi[k] - lo[k]) * (uint32_t)sizeof(T);
+            }
+            tc::mbar_arrive_expect_tx(&bars[s], bytes);
+#pragma unroll
+            for (int k = 0; k < INPUTS; ++k)
+                if (hi[k] > lo[k])
+                    tc::bulk_load(slots + (s * INPUTS + k) * pitch, row[k] + lo[k],
+                                  (uint32_t)(hi[k] - lo[k]) * (uint32_t)sizeof(T), &bars[s]);
+        }
+    }
+    // `ahead` (0 or 1): the row after the current one
+    __device__ __forceinline__ void wait(uint8_t *dyn, int ahead = 0) {
+        const bool wrap = slot + ahead >= depth;
+        tc::mbar_wait(&bars[wrap ? 0 : slot + ahead], phase ^ (wrap ? 1u : 0u), abort_word(dyn));
+    }
+    __device__ __forceinline__ RowView<T> view(int k, const T *row, int ahead = 0) const {
+        const int s = slot + ahead >= depth ? 0 : slot + ahead;
+        RowView<T> v{reinterpret_cast<const T *>(slots + (s * INPUTS + k) * pitch), row, 0, cols};
+        if constexpr (!VEC) {
+            inside(row, v.lo, v.hi);
+            v.s -= v.lo;
+        }
+        return v;
     }
     __device__ __forceinline__ void next() {
         if (++slot == depth) slot = 0, phase ^= 1;
     }
 };
 
+// A lane's values of a segment of the row.
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw8<T> load8(const RowView<T> &row, int seg0, int count, int lane) {
+    if constexpr (VEC) {
+        return load8<T, true>(row.s, seg0, count, lane);
+    } else {
+        Raw8<T> r;
+        if (seg0 >= row.lo && seg0 + SEG <= row.hi) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r.v[j] = row.s[seg0 + 32 * j + lane];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int c = seg0 + 32 * j + lane;
+                r.v[j] = from_f<T>(0.f);
+                if (j < count) r.v[j] = c >= row.lo && c < row.hi ? row.s[c] : row.g[c];
+            }
+        }
+        return r;
+    }
+}
+
 // MAXT: the launch's thread count rounded up to 256 or 512.
 template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP>
 __global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdArgs<T, W> a, int wpr, int depth) {
     extern __shared__ __align__(128) uint8_t dyn[];
     constexpr int NW = MAXT / 32;
-    __shared__ __align__(16) float red[2][NW];
-    if (threadIdx.x < 2 * NW) red[0][threadIdx.x] = 0.f;
+    // rows in hand at once: the reductions of two rows overlap and share their barriers
+    constexpr int R = NCH <= 2 && sizeof(T) == 2 ? 2 : 1;
+    __shared__ __align__(16) float red[2][R][NW];
+    if (threadIdx.x < 2 * R * NW) red[0][0][threadIdx.x] = 0.f;
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
     const int rpc = wpr == 1 ? nwarps : 1;  // rows a CTA has in hand at once
@@ -345,19 +433,19 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdAr
     const float inv_n = 1.f / (float)a.cols;
     const uint64_t key = DROP ? drop_seed(a.d) : 0;
     constexpr int IN = DROP ? 2 : 1;
-    RowRing<T, IN> ring;
+    RowRing<T, IN, VEC> ring;
     const bool leader = wpr == 1 ? lane == 0 : threadIdx.x == 0;
     const int64_t r0 = (int64_t)blockIdx.x * rpc + mine, step = (int64_t)gridDim.x * rpc;
     auto fill = [&](int s, int64_t row) {
         if (row >= a.rows) return;
-        ring.fill(s, 0, a.x + row * a.ldx);
-        if constexpr (DROP) ring.fill(s, 1, a.res + row * a.ldr);
+        const T *src[IN];
+        src[0] = a.x + row * a.ldx;
+        if constexpr (DROP) src[1] = a.res + row * a.ldr;
+        ring.fill(s, src);
     };
-    if constexpr (VEC) {
-        ring.init(dyn, mine, (uint32_t)(a.cols * sizeof(T)), depth, leader);
-        if (leader)
-            for (int i = 0; i < depth; ++i) fill(i, r0 + i * step);
-    }
+    ring.init(dyn, mine, (int)a.cols, depth, leader);
+    if (leader)
+        for (int i = 0; i < depth; ++i) fill(i, r0 + i * step);
     Raw8<W> wv[NCH], bv[NCH];
     int n[NCH];
 #pragma unroll
@@ -367,62 +455,82 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdAr
         wv[i] = load8_or<W, VEC>(a.w, 1.f, seg0, n[i], lane);
         bv[i] = load8_or<W, VEC>(a.b, 0.f, seg0, n[i], lane);
     }
-    for (int64_t r = r0; r < a.rows; r += step) {
-        F8 v[NCH];
-        float2 s = make_float2(0.f, 0.f);
-        if constexpr (VEC) ring.wait(dyn);
-        const T *xr = VEC ? ring.row(0) : a.x + r * a.ldx;
-        const T *rr = DROP ? (VEC ? ring.row(IN - 1) : a.res + r * a.ldr) : nullptr;
+    for (int64_t r = r0; r < a.rows; r += R * step) {
+        F8 v[R][NCH];
+        float s[R];
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int seg0 = (w0 + i * wpr) * SEG;
-            v[i] = unpack<T>(load8<T, VEC>(xr, seg0, n[i], lane));
-            if constexpr (DROP) {
-                const F8 res = unpack<T>(load8<T, VEC>(rr, seg0, n[i], lane));
-                const F8 d = drop8<VEC>(v[i], a.d.row_offset + (uint64_t)r, seg0, lane, key, a.d);
+        for (int k = 0; k < R; ++k) {
+            const int64_t rk = r + k * step;
+            const bool live = k == 0 || rk < a.rows;  // the same for all that share the row
+            float2 t = make_float2(0.f, 0.f);
+            if (live) ring.wait(dyn, k);
+            const RowView<T> xr = ring.view(0, a.x + rk * a.ldx, k);
+            const RowView<T> rr = ring.view(IN - 1, DROP ? a.res + rk * a.ldr : a.x + rk * a.ldx, k);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[i].p[j] = add2(d.p[j], res.p[j]);
-                store8<T, VEC>(a.h + r * a.ldh, seg0, n[i], lane, v[i]);
+            for (int i = 0; i < NCH; ++i) {
+                const int seg0 = (w0 + i * wpr) * SEG, nk = live ? n[i] : 0;
+                v[k][i] = unpack<T>(load8<T, VEC>(xr, seg0, nk, lane));
+                if constexpr (DROP) {
+                    const F8 res = unpack<T>(load8<T, VEC>(rr, seg0, nk, lane));
+                    const F8 d = drop8<VEC>(v[k][i], a.d.row_offset + (uint64_t)rk, seg0, lane, key, a.d);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[k][i].p[j] = add2(d.p[j], res.p[j]);
+                    store8<T, VEC>(a.h + rk * a.ldh, seg0, nk, lane, v[k][i]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) t = add2(t, v[k][i].p[j]);
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s = add2(s, v[i].p[j]);
+            s[k] = t.x + t.y;
         }
-        const float mean = row_sum<NW>(s.x + s.y, red[0], wpr, warp, lane) * inv_n;
-        if constexpr (VEC) {  // every reader of the slot is past its reads
-            if (wpr == 1) __syncwarp();
-            if (leader) fill(ring.slot, r + depth * step);
+        row_sums<NW, R>(s, red[0], wpr, warp, lane);
+        // every reader of the slots is past its reads
+        if (wpr == 1) __syncwarp();
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            if (leader) fill(ring.slot, r + (depth + k) * step);
             ring.next();
         }
-        const float2 mean2 = make_float2(mean, mean);
-        float2 q = make_float2(0.f, 0.f);
+        float mean[R], q[R];
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
+        for (int k = 0; k < R; ++k) {
+            mean[k] = s[k] * inv_n;
+            const float2 mean2 = make_float2(mean[k], mean[k]);
+            float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[i].p[j] = sub2(v[i].p[j], mean2);
-                if constexpr (!VEC) {
-                    if (2 * j >= n[i]) v[i].p[j].x = 0.f;
-                    if (2 * j + 1 >= n[i]) v[i].p[j].y = 0.f;
+            for (int i = 0; i < NCH; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float2 &p = v[k][i].p[j];
+                    p = sub2(p, mean2);
+                    if constexpr (!VEC) {
+                        if (2 * j >= n[i]) p.x = 0.f;
+                        if (2 * j + 1 >= n[i]) p.y = 0.f;
+                    }
+                    if (!VEC || n[i]) t = fma2(p, p, t);
                 }
-                if (!VEC || n[i]) q = fma2(v[i].p[j], v[i].p[j], q);
             }
+            q[k] = t.x + t.y;
         }
-        const float var = row_sum<NW>(q.x + q.y, red[1], wpr, warp, lane) * inv_n;
-        const float rstd = inv_sqrt(var + a.eps);
-        if (lane == 0 && w0 == 0) {
-            a.mean[r] = mean;
-            a.rstd[r] = rstd;
-        }
-        const float2 rstd2 = make_float2(rstd, rstd);
+        row_sums<NW, R>(q, red[1], wpr, warp, lane);
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int seg0 = (w0 + i * wpr) * SEG;
-            stay_packed(wv[i]);
-            stay_packed(bv[i]);
-            const F8 w = unpack<W>(wv[i]), b = unpack<W>(bv[i]);
+        for (int k = 0; k < R; ++k) {
+            const int64_t rk = r + k * step;
+            if (k > 0 && rk >= a.rows) break;
+            const float rstd = inv_sqrt(__fmaf_rn(q[k], inv_n, a.eps));
+            if (lane == 0 && w0 == 0) {
+                a.mean[rk] = mean[k];
+                a.rstd[rk] = rstd;
+            }
+            const float2 rstd2 = make_float2(rstd, rstd);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[i].p[j] = fma2(mul2(v[i].p[j], rstd2), w.p[j], b.p[j]);
-            store8<T, VEC>(a.y + r * a.ldy, seg0, n[i], lane, v[i]);
+            for (int i = 0; i < NCH; ++i) {
+                stay_packed(wv[i]);
+                stay_packed(bv[i]);
+                const F8 w = unpack<W>(wv[i]), b = unpack<W>(bv[i]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[k][i].p[j] = fma2(mul2(v[k][i].p[j], rstd2), w.p[j], b.p[j]);
+                store8<T, VEC>(a.y + rk * a.ldy, (w0 + i * wpr) * SEG, n[i], lane, v[k][i]);
+            }
         }
     }
 }
@@ -454,7 +562,7 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_fwd_long_kernel(FwdArgs<T, W>
             const float2 t = add2(add2(v.p[0], v.p[1]), add2(v.p[2], v.p[3]));
             s += t.x + t.y;
         }
-        const float mean = row_sum<nw>(s, red[0], nw, warp, lane) * inv_n;
+        const float mean = row_sum<nw>(s, red, nw, warp, lane) * inv_n;
         const float2 mean2 = make_float2(mean, mean);
         float q = 0.f;
         for (int64_t g = warp; g < segs; g += nw) {
@@ -470,7 +578,7 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_fwd_long_kernel(FwdArgs<T, W>
             }
             q += t.x + t.y;
         }
-        const float var = row_sum<nw>(q, red[1], nw, warp, lane) * inv_n;
+        const float var = row_sum<nw>(q, red + 1, nw, warp, lane) * inv_n;
         const float rstd = inv_sqrt(var + a.eps);
         if (threadIdx.x == 0) {
             a.mean[r] = mean;
@@ -531,21 +639,21 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
     const float inv_n = 1.f / (float)a.cols;
     const uint64_t key = DROP ? drop_seed(a.d) : 0;
     constexpr int IN = DROP ? 3 : 2;
-    RowRing<T, IN> ring;
+    RowRing<T, IN, VEC> ring;
     const bool leader = wpr == 1 ? lane == 0 : threadIdx.x == 0;
     const int64_t r0 = (int64_t)blockIdx.x * rpc + mine, step = (int64_t)gridDim.x * rpc;
     auto fill = [&](int s, int64_t row) {
         if (row >= a.rows) return;
-        ring.fill(s, 0, a.dy + row * a.lddy);
-        ring.fill(s, 1, a.x + row * a.ldx);
+        const T *src[IN];
+        src[0] = a.dy + row * a.lddy;
+        src[1] = a.x + row * a.ldx;
         // without dh its slot holds dy again and is not read
-        if constexpr (DROP) ring.fill(s, 2, a.dh ? a.dh + row * a.lddh : a.dy + row * a.lddy);
+        if constexpr (DROP) src[2] = a.dh ? a.dh + row * a.lddh : src[0];
+        ring.fill(s, src);
     };
-    if constexpr (VEC) {
-        ring.init(dyn, mine, (uint32_t)(a.cols * sizeof(T)), depth, leader);
-        if (leader)
-            for (int i = 0; i < depth; ++i) fill(i, r0 + i * step);
-    }
+    ring.init(dyn, mine, (int)a.cols, depth, leader);
+    if (leader)
+        for (int i = 0; i < depth; ++i) fill(i, r0 + i * step);
     // Up to two segments a thread the row's g and x-hat are held from the sums to
     // the output, past that they are computed again from the slot (registers).
     constexpr bool HOLD = NCH <= 2;
@@ -567,11 +675,10 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
         const float2 mean2 = make_float2(mean, mean), rstd2 = make_float2(rstd, rstd);
         const float rs = rstd;
         if (r + step < a.rows) mean = a.mean[r + step], rstd = a.rstd[r + step];
-        const T *yr = VEC ? ring.row(0) : a.dy + r * a.lddy;
-        const T *xr = VEC ? ring.row(1) : a.x + r * a.ldx;
+        const RowView<T> yr = ring.view(0, a.dy + r * a.lddy), xr = ring.view(1, a.x + r * a.ldx);
         float2 s1 = make_float2(0.f, 0.f), s2 = s1;
         F8 gh[HOLD ? NCH : 1], xh[HOLD ? NCH : 1];
-        if constexpr (VEC) ring.wait(dyn);
+        ring.wait(dyn);
         auto weights = [&](int i) {
             if constexpr (WREG) {
                 stay_packed(wv[i]);
@@ -603,10 +710,9 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
             }
         }
         const float2 s = row_sum2<NW>(s1.x + s1.y, s2.x + s2.y, red[turn & 1], wpr, warp, lane);
-        if constexpr (VEC) {  // the row before this one has been read by all
-            if (wpr == 1) __syncwarp();
-            if (leader && turn > 0) fill(ring.slot == 0 ? depth - 1 : ring.slot - 1, r + (depth - 1) * step);
-        }
+        // the row before this one has been read by all
+        if (wpr == 1) __syncwarp();
+        if (leader && turn > 0) fill(ring.slot == 0 ? depth - 1 : ring.slot - 1, r + (depth - 1) * step);
         // dx = rstd g - rstd mean(g) - x-hat rstd mean(g x-hat)
         const float c1 = -rs * (s.x * inv_n), c2 = -rs * (s.y * inv_n);
         const float2 c1_2 = make_float2(c1, c1), c2_2 = make_float2(c2, c2);
@@ -627,7 +733,7 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
             if constexpr (DROP) {
                 if (a.dh) {
                     const F8 dh = unpack<T>(
-                        load8<T, VEC>(VEC ? ring.row(IN - 1) : a.dh + r * a.lddh, seg0, n[i], lane));
+                        load8<T, VEC>(ring.view(IN - 1, a.dh + r * a.lddh), seg0, n[i], lane));
 #pragma unroll
                     for (int j = 0; j < 4; ++j) g.p[j] = add2(g.p[j], dh.p[j]);
                 }
@@ -636,7 +742,7 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
             }
             store8<T, VEC>(a.dx + r * a.lddx, seg0, n[i], lane, g);
         }
-        if constexpr (VEC) ring.next();
+        ring.next();
     }
     if (!a.part) return;
     float *part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
@@ -773,24 +879,33 @@ __global__ void __launch_bounds__(256) ln_bwd_finish_kernel(const float *part, i
 struct Shape {
     int nch, wpr, threads, rows_per_cta, depth, smem, per_sm;
 };
-static Shape shape_of(int64_t cols, int esize, int inputs, bool bwd) {
+static Shape shape_of(int64_t cols, int esize, bool drop, bool bwd, bool vec) {
     const int segs = (int)((cols + SEG - 1) / SEG);
     Shape s{};
     if (segs <= 4) {
         s = {segs <= 1 ? 1 : (segs <= 2 ? 2 : 4), 1, 256, 8, 0, 0, 0};
     } else {
-        s.nch = bwd ? (segs <= 32 ? 2 : 4) : (segs <= 8 ? 1 : segs <= 16 ? 2 : segs <= 24 ? 3 : 4);
+        // Fewer, fuller warps spend less on a row's reductions: 16384 x 4096 bf16
+        // forward in 52 us with four segments a thread, 56 with two, 86 with one; the
+        // dropout's and float32's registers allow two, the backward's sums two.
+        const bool full = !drop && esize == 2;
+        s.nch = bwd         ? (segs <= 32 ? 2 : 4)
+                : segs <= 8 ? (full ? 2 : 1)
+                : segs <= 16 ? (full ? 4 : 2)
+                : segs <= 24 ? 3
+                             : 4;
         s.wpr = (segs + s.nch - 1) / s.nch;
         s.threads = 32 * s.wpr;
         s.rows_per_cta = 1;
     }
-    const int64_t slot = cols * esize * inputs * s.rows_per_cta;
-    s.per_sm = bwd ? bwd_ctas(s.threads) : fwd_ctas(s.nch, s.threads);
-    const int64_t room = 220 * 1024 / s.per_sm - 2048;
+    const int inputs = (bwd ? 2 : 1) + (drop ? 1 : 0);
+    const int64_t slot = (int64_t)row_pitch(cols, esize, vec) * inputs * s.rows_per_cta;
+    s.per_sm = (bwd ? bwd_ctas(s.threads) : fwd_ctas(s.nch, s.threads)) * (s.threads <= 128 ? 2 : 1);
+    const int64_t room = SLOT_ROOM / s.per_sm;
     s.depth = (int)(room / slot < MAX_DEPTH ? room / slot : MAX_DEPTH);
     if (s.depth < 2) {  // the longest rows: one CTA per SM
         s.per_sm = 1;
-        s.depth = (int)((220 * 1024 - 2048) / slot < MAX_DEPTH ? (220 * 1024 - 2048) / slot : MAX_DEPTH);
+        s.depth = (int)(SLOT_ROOM / slot < MAX_DEPTH ? SLOT_ROOM / slot : MAX_DEPTH);
     }
     s.smem = RING_HEAD + (int)(s.depth * slot);
     if (bwd && s.wpr == 1) {
@@ -810,28 +925,40 @@ static int long_parts(int64_t rows, int64_t cols) {
     if (y > rows) y = rows;
     return (int)(y < 1 ? 1 : (y > 65535 ? 65535 : y));
 }
-static bool is_long(int64_t cols) { return cols > (int64_t)MAX_SEGS * SEG; }
+// Rows that go through the re-reading kernels: more than the registers hold, or
+// (backward) than leaves two ring slots in shared memory.
+static bool is_long(int64_t cols, int esize, bool drop, bool bwd) {
+    if (cols > (int64_t)MAX_SEGS * SEG) return true;
+    return bwd && 2 * (int64_t)row_pitch(cols, esize, false) * (drop ? 3 : 2) > SLOT_ROOM;
+}
 static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 static size_t bwd_workspace(int64_t rows, int64_t cols) {
-    if (is_long(cols)) return up256((size_t)long_parts(rows, cols) * 2 * cols * 4) + up256((size_t)rows * 8);
-    const int64_t ctas = cols <= 4 * SEG ? (rows + 7) / 8 : rows, cap = (int64_t)num_sms() * 2;
-    return up256((size_t)(ctas < cap ? ctas : cap) * 2 * cols * 4);
+    size_t need = 0;
+    if (cols <= (int64_t)MAX_SEGS * SEG) {
+        const int64_t ctas = cols <= 4 * SEG ? (rows + 7) / 8 : rows, cap = (int64_t)num_sms() * 4;
+        need = up256((size_t)(ctas < cap ? ctas : cap) * 2 * cols * 4);
+    }
+    if (is_long(cols, 4, true, true)) {  // for some type or form
+        const size_t l = up256((size_t)long_parts(rows, cols) * 2 * cols * 4) + up256((size_t)rows * 8);
+        if (l > need) need = l;
+    }
+    return need;
 }
 
 template <typename T, typename W, bool VEC, bool DROP>
 static int fwd_launch(const FwdArgs<T, W> &a, cudaStream_t st) {
-    if (is_long(a.cols)) {
+    if (is_long(a.cols, sizeof(T), DROP, false)) {
         const int64_t cap = (int64_t)num_sms() * 4;
         ln_fwd_long_kernel<T, W, VEC, DROP><<<(int)(a.rows < cap ? a.rows : cap), LONG_THREADS, 0, st>>>(a);
         return launch_status();
     }
-    const Shape s = shape_of(a.cols, sizeof(T), DROP ? 2 : 1, false);
+    const Shape s = shape_of(a.cols, sizeof(T), DROP, false, VEC);
     const int grid = grid_of(s, a.rows);
     auto go = [&](auto k) -> int {
-        const int smem = VEC ? s.smem : 0;
-        if (smem > 48 * 1024) ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        k<<<grid, s.threads, smem, st>>>(a, s.wpr, s.depth);
+        if (s.smem > 48 * 1024)
+            ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem));
+        k<<<grid, s.threads, s.smem, st>>>(a, s.wpr, s.depth);
         return launch_status();
     };
     if (s.nch == 1) return go(ln_fwd_kernel<T, W, 1, 256, VEC, DROP>);
@@ -852,7 +979,7 @@ template <typename T, typename W, bool VEC, bool DROP>
 static int bwd_launch(BwdArgs<T, W> a, W *dw, W *db, void *ws, cudaStream_t st) {
     int parts, rc;
     a.part = dw || db ? static_cast<float *>(ws) : nullptr;
-    if (is_long(a.cols)) {
+    if (is_long(a.cols, sizeof(T), DROP, true)) {
         parts = long_parts(a.rows, a.cols);
         float2 *sums = reinterpret_cast<float2 *>(static_cast<uint8_t *>(ws) + up256((size_t)parts * 2 * a.cols * 4));
         const int64_t cap = (int64_t)num_sms() * 4;
@@ -861,7 +988,7 @@ static int bwd_launch(BwdArgs<T, W> a, W *dw, W *db, void *ws, cudaStream_t st) 
         ln_bwd_cols_kernel<T, W, VEC, DROP><<<grid, 128, 0, st>>>(a, sums);
         rc = launch_status();
     } else {
-        const Shape s = shape_of(a.cols, sizeof(T), DROP ? 3 : 2, true);
+        const Shape s = shape_of(a.cols, sizeof(T), DROP, true, VEC);
         parts = grid_of(s, a.rows);
         const bool small = s.threads <= 256;
         rc = s.nch == 1   ? bwd_main<T, W, 1, 256, VEC, DROP>(a, s, parts, st)
