@@ -469,9 +469,10 @@ int actcomp_mx4_gemm(const actcomp_mx4 *a, const actcomp_mx4 *b, void *c, int64_
 /* c = x . w^T (tokens x w->rows) for up to ACTCOMP_MX4_LINEAR_TOKENS tokens in one
  * kernel: x (tokens x w->cols, dtype as above, row stride ldx) is quantised by
  * rows on the way.  c_dtype: dtype or 0.  ACT_E_UNSUPPORTED for more tokens, or
- * where 36 bytes per token and block of 32 columns pass 160 KiB (quantise, then
- * actcomp_mx4_gemm). */
+ * where 36 bytes per token and block of 32 columns pass
+ * ACTCOMP_MX4_LINEAR_BYTES (quantise, then actcomp_mx4_gemm). */
 #define ACTCOMP_MX4_LINEAR_TOKENS 4
+#define ACTCOMP_MX4_LINEAR_BYTES (160 * 1024)
 int actcomp_mx4_linear(const void *x, int64_t tokens, int64_t cols, int64_t ldx, int32_t dtype, const actcomp_mx4 *w,
                        void *c, int64_t ldc, int32_t c_dtype, void *stream);
 

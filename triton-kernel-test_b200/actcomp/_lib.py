@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -117,19 +116,6 @@ class Mx4Desc(ctypes.Structure):
     _fields_ = [("rows", c_i64), ("cols", c_i64), ("codes", c_vp), ("scales", c_vp)]
 
 
-_CODES = {c_i64: "q", ctypes.c_uint64: "Q", c_i32: "i", c_vp: "P", ctypes.c_double: "d", ctypes.c_float: "f"}
-
-
-def packer(cls) -> struct.Struct:
-    """``cls``'s layout as a struct.Struct (native alignment): packing a dozen
-    fields takes a quarter of the time of building the ctypes structure, which
-    counts where a call's host time is most of it."""
-    st = struct.Struct("@" + "".join(_CODES[t] for _, t in cls._fields_))
-    if st.size != ctypes.sizeof(cls):
-        raise ImportError(f"{cls.__name__}: packed layout differs from the C layout")
-    return st
-
-
 #: entry point -> (restype, argtypes); mirrors include/actcomp.h
 SIGNATURES = {
     "actcomp_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -219,14 +205,18 @@ def check(fn: str, status: int) -> None:
         raise ActcompError(fn, status)
 
 
-def entry(name: str):
-    """The entry point as a function object of its own that takes structures as
-    packed bytes (any pointer argument takes bytes or an address)."""
-    res, args = SIGNATURES[name]
-    fn = load()[name]
-    fn.restype = res
-    fn.argtypes = [c_vp if isinstance(t, type) and issubclass(t, ctypes._Pointer) else t for t in args]
-    return fn
+def host():
+    """The extension module that runs the host side of :mod:`actcomp.norm` and
+    :mod:`actcomp.mx4` (csrc/host.cpp), bound to the loaded library."""
+    lib = load()
+    path = os.path.join(_HERE, "_host.so")
+    if not os.path.exists(path):
+        raise ImportError(f"{path} is missing: build it with `python triton-kernel-test_b200/actcomp/build.py`")
+    from . import _host
+
+    _host.bind({name: ctypes.cast(getattr(lib, name), c_vp).value for name in SIGNATURES
+                if name.startswith(("actcomp_dropout", "actcomp_layer_norm", "actcomp_mx4_"))})
+    return _host
 
 
 def call(name: str, *args) -> None:

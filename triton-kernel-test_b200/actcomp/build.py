@@ -23,6 +23,8 @@ LIB = os.path.join(PKG, "libactcomp.so")
 # the bounds-checked build (-DACT_BOUNDS_CHECK): device-side index checks that
 # record a bit in the device error word instead of trapping; tests only
 LIB_BC = os.path.join(PKG, "libactcomp_bc.so")
+# the host side of actcomp.norm and actcomp.mx4 (csrc/host.cpp), a Python extension module
+HOST = os.path.join(PKG, "_host.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -58,10 +60,35 @@ def stale(lib: str = LIB) -> bool:
     return any(os.path.getmtime(p) > t for p in _deps())
 
 
+def build_host(force: bool = False) -> str:
+    """Compile (if stale) csrc/host.cpp against torch's headers and return the
+    path of _host.so."""
+    import sysconfig
+
+    src = os.path.join(CSRC, "host.cpp")
+    deps = [src, os.path.join(os.path.dirname(ROOT), "include", "actcomp.h")]
+    if not force and os.path.exists(HOST) and all(os.path.getmtime(p) <= os.path.getmtime(HOST) for p in deps):
+        return HOST
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], cuda]
+    tmp = HOST + ".tmp"
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", src, "-o", tmp,
+                    *[f"-I{i}" for i in inc], f"-L{os.path.join(base, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+                    "-ltorch", "-ltorch_python", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"],
+                   check=True)
+    os.replace(tmp, HOST)
+    return HOST
+
+
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None, bounds_check: bool = False) -> str:
     """Compile (if stale) and return the path of libactcomp.so (libactcomp_bc.so
     with bounds_check)."""
     lib = LIB_BC if bounds_check else LIB
+    build_host(force and not bounds_check)
     if not force and not stale(lib):
         return lib
     exe = nvcc()

@@ -23,19 +23,6 @@ def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-def _launch(name: str, fn, device: torch.device, *args) -> None:
-    """Call a status-returning entry point (from ``_lib.entry``) on the current
-    stream of ``device``, with that device current."""
-    index = device.index
-    if index == torch._C._cuda_getDevice():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status:
-        _lib.check(name, status)
-
-
 def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 

@@ -24,7 +24,7 @@ int mx4_check(const actcomp_mx4 *q);
 namespace mx4 {
 
 constexpr int MAX_TOKENS = ACTCOMP_MX4_LINEAR_TOKENS;
-constexpr int MAX_X_BYTES = 160 * 1024;  // shared memory for x
+constexpr int MAX_X_BYTES = ACTCOMP_MX4_LINEAR_BYTES;  // shared memory for x
 constexpr int DEPTH = 2, STAGE = 5 * 512;  // a warp's stages: four rows' pieces of 512 bytes and the scale words
 
 struct LinArgs {
