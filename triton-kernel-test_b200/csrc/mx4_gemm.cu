@@ -205,22 +205,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             auto put = [&](int g, const uint32_t (&r)[32]) {
                 const int col = n0 + g * 32;
                 if (row0 >= p.M || col >= p.N) return;
-                if (p.tma_out) {
-                    uint8_t *dst = stage + buf * 4096;
-                    tc::bulk_wait_read<1>();  // lane 0's store before the last has left this buffer
-                    __syncwarp();
+                uint8_t *dst = stage + buf * 4096;
+                tc::bulk_wait_read<1>();  // lane 0's store before the last has left this buffer
+                __syncwarp();
 #pragma unroll
-                    for (int c = 0; c < 2 * ES; ++c) {  // 16-byte chunks of a row
-                        uint4 v;
-                        if constexpr (ES == 4) {
-                            v = make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
-                        } else {
-                            const auto F = [&](int j) { return __uint_as_float(r[8 * c + j]); };
-                            v = make_uint4(pack2<TOut>(F(0), F(1)), pack2<TOut>(F(2), F(3)), pack2<TOut>(F(4), F(5)),
-                                           pack2<TOut>(F(6), F(7)));
-                        }
-                        *reinterpret_cast<uint4 *>(dst + kmajor_swz<32 * ES>(lane, c)) = v;
+                for (int c = 0; c < 2 * ES; ++c) {  // 16-byte chunks of a row
+                    uint4 v;
+                    if constexpr (ES == 4) {
+                        v = make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+                    } else {
+                        const auto F = [&](int j) { return __uint_as_float(r[8 * c + j]); };
+                        v = make_uint4(pack2<TOut>(F(0), F(1)), pack2<TOut>(F(2), F(3)), pack2<TOut>(F(4), F(5)),
+                                       pack2<TOut>(F(6), F(7)));
                     }
+                    *reinterpret_cast<uint4 *>(dst + kmajor_swz<32 * ES>(lane, c)) = v;
+                }
+                if (p.tma_out) {
                     tc::fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
@@ -228,13 +228,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         tc::bulk_commit();
                     }
                     buf ^= 1;
-                } else {
-                    if (row0 + lane < p.M) {
-                        TOut *d = static_cast<TOut *>(p.C) + (int64_t)(row0 + lane) * p.ldc + col;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (col + j < p.N) d[j] = cvt_out<TOut>(__uint_as_float(r[j]));
-                    }
+                } else {  // a row at a time, neighbouring lanes neighbouring columns
+                    __syncwarp();
+                    constexpr int PER = 16 / ES;
+                    const int rows = p.M - row0 < 32 ? p.M - row0 : 32;
+                    TOut *d = static_cast<TOut *>(p.C) + (int64_t)row0 * p.ldc + col + lane;
+                    if (col + lane < p.N)
+                        for (int i = 0; i < rows; ++i, d += p.ldc)
+                            *d = *reinterpret_cast<const TOut *>(dst + kmajor_swz<32 * ES>(i, lane / PER) +
+                                                                 lane % PER * ES);
                     __syncwarp();
                 }
             };

@@ -406,11 +406,12 @@ __device__ __forceinline__ Raw8<T> load8(const RowView<T> &row, int seg0, int co
 #pragma unroll
             for (int j = 0; j < 8; ++j) r.v[j] = row.s[seg0 + 32 * j + lane];
         } else {
+            // one generic load each, no branch between them: their latencies overlap
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int c = seg0 + 32 * j + lane;
-                r.v[j] = from_f<T>(0.f);
-                if (j < count) r.v[j] = c >= row.lo && c < row.hi ? row.s[c] : row.g[c];
+                const T *p = c >= row.lo && c < row.hi ? row.s + c : row.g + c;
+                r.v[j] = j < count ? *p : from_f<T>(0.f);
             }
         }
         return r;
@@ -610,23 +611,32 @@ struct BwdArgs {
     DropParams d;
 };
 
-template <int NW>
-__device__ __forceinline__ float2 row_sum2(float u, float v, float2 *red, int wpr, int warp, int lane) {
+// Sums of u and v over the warps that share a row (`w0`: this one's place).  red:
+// NW entries, zero where there is no warp.  MULTI: several groups of warps share the
+// CTA, each with two or four entries.
+template <int NW, bool MULTI>
+__device__ __forceinline__ float2 row_sum2(float u, float v, float2 *red, int wpr, int group, int w0, int lane) {
     u = warp_sum(u);
     v = warp_sum(v);
-    if (wpr == 1) return make_float2(u, v);
-    if (lane == 0) red[warp] = make_float2(u, v);
-    __syncthreads();
+    if (MULTI && wpr == 1) return make_float2(u, v);
+    const int room = wpr <= 2 ? 2 : 4;
+    if (MULTI) red += group * room;
+    if (lane == 0) red[w0] = make_float2(u, v);
+    if (MULTI) tc::named_bar(1 + group, 32 * wpr);
+    else __syncthreads();
     float2 s = make_float2(0.f, 0.f);
+    const float4 *p = reinterpret_cast<const float4 *>(red);
+    if constexpr (!MULTI) {
 #pragma unroll
-    for (int i = 0; i < NW / 2; ++i) {
-        const float4 q = reinterpret_cast<const float4 *>(red)[i];
-        s = add2(add2(s, make_float2(q.x, q.y)), make_float2(q.z, q.w));
+        for (int i = 0; i < NW / 2; ++i) s = add2(add2(s, make_float2(p[i].x, p[i].y)), make_float2(p[i].z, p[i].w));
+    } else {
+        for (int i = 0; i < room / 2; ++i) s = add2(add2(s, make_float2(p[i].x, p[i].y)), make_float2(p[i].z, p[i].w));
     }
     return s;
 }
 
-template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP>
+// MULTI: a CTA has several rows in hand, each a group of `wpr` warps; else one.
+template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP, bool MULTI>
 __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T, W> a, int wpr, int depth) {
     constexpr int NW = MAXT / 32;
     __shared__ __align__(16) float2 red[2][NW];
@@ -634,13 +644,13 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
     __syncthreads();
     extern __shared__ __align__(128) uint8_t dyn[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
-    const int rpc = wpr == 1 ? nwarps : 1;
-    const int w0 = wpr == 1 ? 0 : warp, mine = wpr == 1 ? warp : 0;
+    const int rpc = MULTI ? nwarps / wpr : 1;  // rows a CTA has in hand at once
+    const int mine = MULTI ? warp / wpr : 0, w0 = warp - mine * wpr;
     const float inv_n = 1.f / (float)a.cols;
     const uint64_t key = DROP ? drop_seed(a.d) : 0;
     constexpr int IN = DROP ? 3 : 2;
     RowRing<T, IN, VEC> ring;
-    const bool leader = wpr == 1 ? lane == 0 : threadIdx.x == 0;
+    const bool leader = w0 == 0 && lane == 0;
     const int64_t r0 = (int64_t)blockIdx.x * rpc + mine, step = (int64_t)gridDim.x * rpc;
     auto fill = [&](int s, int64_t row) {
         if (row >= a.rows) return;
@@ -709,9 +719,9 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
                 if constexpr (HOLD) gh[i].p[j] = g, xh[i].p[j] = x.p[j];
             }
         }
-        const float2 s = row_sum2<NW>(s1.x + s1.y, s2.x + s2.y, red[turn & 1], wpr, warp, lane);
+        const float2 s = row_sum2<NW, MULTI>(s1.x + s1.y, s2.x + s2.y, red[turn & 1], wpr, mine, w0, lane);
         // the row before this one has been read by all
-        if (wpr == 1) __syncwarp();
+        if (MULTI && wpr == 1) __syncwarp();
         if (leader && turn > 0) fill(ring.slot == 0 ? depth - 1 : ring.slot - 1, r + (depth - 1) * step);
         // dx = rstd g - rstd mean(g) - x-hat rstd mean(g x-hat)
         const float c1 = -rs * (s.x * inv_n), c2 = -rs * (s.y * inv_n);
@@ -746,19 +756,19 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
     }
     if (!a.part) return;
     float *part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
-    if (wpr == 1) {
-        // the warps' sums, over the ring's space once every warp is done with it
+    if constexpr (MULTI) {
+        // the groups' sums, over the rings' space once every warp is done with it
         __syncthreads();
-        float *acc = reinterpret_cast<float *>(dyn + RING_HEAD), *own = acc + (int64_t)warp * 2 * a.cols;
+        float *acc = reinterpret_cast<float *>(dyn + RING_HEAD), *own = acc + (int64_t)mine * 2 * a.cols;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            store8<float, VEC>(own, i * SEG, n[i], lane, dw[i]);
-            store8<float, VEC>(own + a.cols, i * SEG, n[i], lane, db[i]);
+            store8<float, VEC>(own, (w0 + i * wpr) * SEG, n[i], lane, dw[i]);
+            store8<float, VEC>(own + a.cols, (w0 + i * wpr) * SEG, n[i], lane, db[i]);
         }
         __syncthreads();
         for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) {
             float s = 0.f;
-            for (int i = 0; i < nwarps; ++i) s += acc[(int64_t)i * 2 * a.cols + c];
+            for (int i = 0; i < rpc; ++i) s += acc[(int64_t)i * 2 * a.cols + c];
             part[c] = s;
         }
         return;
@@ -799,7 +809,7 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_bwd_sums_kernel(BwdArgs<T, W>
             s1 += t1.x + t1.y;
             s2 += t2.x + t2.y;
         }
-        const float2 s = row_sum2<nw>(s1, s2, red[turn], nw, warp, lane);
+        const float2 s = row_sum2<nw, false>(s1, s2, red[turn], nw, 0, warp, lane);
         turn ^= 1;
         if (threadIdx.x == 0) sums[r] = make_float2(s.x * inv_n, s.y * inv_n);
     }
@@ -849,20 +859,32 @@ __global__ void __launch_bounds__(128) ln_bwd_cols_kernel(BwdArgs<T, W> a, const
     store8<float, VEC>(part + a.cols, seg0, n, lane, db);
 }
 
-// dw / db from the `parts` partial sums, in their order: a column's sum does
+// dw / db from the `parts` partial sums, in a fixed order: a column's sum does
 // not depend on timing.  A warp takes 32 columns, the CTA's eight warps every
-// eighth partial.
+// eighth partial, eight loads in flight.  Launched under the kernel before it
+// (programmatic dependence): it waits for that kernel's end before it reads.
 template <typename W>
 __global__ void __launch_bounds__(256) ln_bwd_finish_kernel(const float *part, int parts, int64_t cols, W *dw, W *db) {
     __shared__ float red[8][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + lane;  // of 2 * cols
+    const int64_t n = 2 * cols, c = (int64_t)blockIdx.x * 32 + lane;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     float s = 0.f;
-    if (c < 2 * cols)
-        for (int i = warp; i < parts; i += 8) s += part[(int64_t)i * 2 * cols + c];
+    if (c < n) {
+        const float *p = part + c;
+        int i = warp;
+        for (; i + 56 < parts; i += 64) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = __ldcg(p + (int64_t)(i + 8 * k) * n);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += v[k];
+        }
+        for (; i < parts; i += 8) s += __ldcg(p + (int64_t)i * n);
+    }
     red[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && c < 2 * cols) {
+    if (warp == 0 && c < n) {
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += red[i][lane];
@@ -882,25 +904,27 @@ struct Shape {
 static Shape shape_of(int64_t cols, int esize, bool drop, bool bwd, bool vec) {
     const int segs = (int)((cols + SEG - 1) / SEG);
     Shape s{};
-    if (segs <= 4) {
+    if (bwd) {
+        // two segments a thread (its sums' registers); short rows several to a CTA
+        s.nch = segs <= 1 ? 1 : (segs <= 32 ? 2 : 4);
+        s.wpr = (segs + s.nch - 1) / s.nch;
+        s.rows_per_cta = s.wpr <= 4 ? 8 / s.wpr : 1;  // two or more
+        s.threads = 32 * s.wpr * s.rows_per_cta;
+    } else if (segs <= 4) {
         s = {segs <= 1 ? 1 : (segs <= 2 ? 2 : 4), 1, 256, 8, 0, 0, 0};
     } else {
         // Fewer, fuller warps spend less on a row's reductions: 16384 x 4096 bf16
-        // forward in 52 us with four segments a thread, 56 with two, 86 with one; the
-        // dropout's and float32's registers allow two, the backward's sums two.
+        // in 52 us with four segments a thread, 56 with two, 86 with one; the
+        // dropout's and float32's registers allow two.
         const bool full = !drop && esize == 2;
-        s.nch = bwd         ? (segs <= 32 ? 2 : 4)
-                : segs <= 8 ? (full ? 2 : 1)
-                : segs <= 16 ? (full ? 4 : 2)
-                : segs <= 24 ? 3
-                             : 4;
+        s.nch = segs <= 8 ? (full ? 2 : 1) : segs <= 16 ? (full ? 4 : 2) : segs <= 24 ? 3 : 4;
         s.wpr = (segs + s.nch - 1) / s.nch;
         s.threads = 32 * s.wpr;
         s.rows_per_cta = 1;
     }
     const int inputs = (bwd ? 2 : 1) + (drop ? 1 : 0);
     const int64_t slot = (int64_t)row_pitch(cols, esize, vec) * inputs * s.rows_per_cta;
-    s.per_sm = (bwd ? bwd_ctas(s.threads) : fwd_ctas(s.nch, s.threads)) * (s.threads <= 128 ? 2 : 1);
+    s.per_sm = bwd ? bwd_ctas(s.threads) : fwd_ctas(s.nch, s.threads) * (s.threads <= 128 ? 2 : 1);
     const int64_t room = SLOT_ROOM / s.per_sm;
     s.depth = (int)(room / slot < MAX_DEPTH ? room / slot : MAX_DEPTH);
     if (s.depth < 2) {  // the longest rows: one CTA per SM
@@ -908,7 +932,7 @@ static Shape shape_of(int64_t cols, int esize, bool drop, bool bwd, bool vec) {
         s.depth = (int)(SLOT_ROOM / slot < MAX_DEPTH ? SLOT_ROOM / slot : MAX_DEPTH);
     }
     s.smem = RING_HEAD + (int)(s.depth * slot);
-    if (bwd && s.wpr == 1) {
+    if (bwd && s.rows_per_cta > 1) {
         const int acc = RING_HEAD + (int)(s.rows_per_cta * 2 * cols * 4);
         if (acc > s.smem) s.smem = acc;
     }
@@ -936,8 +960,8 @@ static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 static size_t bwd_workspace(int64_t rows, int64_t cols) {
     size_t need = 0;
     if (cols <= (int64_t)MAX_SEGS * SEG) {
-        const int64_t ctas = cols <= 4 * SEG ? (rows + 7) / 8 : rows, cap = (int64_t)num_sms() * 4;
-        need = up256((size_t)(ctas < cap ? ctas : cap) * 2 * cols * 4);
+        const Shape s = shape_of(cols, 2, false, true, false);  // the largest grid of the forms
+        need = up256((size_t)grid_of(s, rows) * 2 * cols * 4);
     }
     if (is_long(cols, 4, true, true)) {  // for some type or form
         const size_t l = up256((size_t)long_parts(rows, cols) * 2 * cols * 4) + up256((size_t)rows * 8);
@@ -967,9 +991,9 @@ static int fwd_launch(const FwdArgs<T, W> &a, cudaStream_t st) {
     return s.threads <= 256 ? go(ln_fwd_kernel<T, W, 4, 256, VEC, DROP>) : go(ln_fwd_kernel<T, W, 4, 512, VEC, DROP>);
 }
 
-template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP>
+template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP, bool MULTI>
 static int bwd_main(const BwdArgs<T, W> &a, const Shape &s, int grid, cudaStream_t st) {
-    auto k = ln_bwd_kernel<T, W, NCH, MAXT, VEC, DROP>;
+    auto k = ln_bwd_kernel<T, W, NCH, MAXT, VEC, DROP, MULTI>;
     if (s.smem > 48 * 1024) ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem));
     k<<<grid, s.threads, s.smem, st>>>(a, s.wpr, s.depth);
     return launch_status();
@@ -990,16 +1014,25 @@ static int bwd_launch(BwdArgs<T, W> a, W *dw, W *db, void *ws, cudaStream_t st) 
     } else {
         const Shape s = shape_of(a.cols, sizeof(T), DROP, true, VEC);
         parts = grid_of(s, a.rows);
-        const bool small = s.threads <= 256;
-        rc = s.nch == 1   ? bwd_main<T, W, 1, 256, VEC, DROP>(a, s, parts, st)
-             : s.nch == 2 ? (small ? bwd_main<T, W, 2, 256, VEC, DROP>(a, s, parts, st)
-                                   : bwd_main<T, W, 2, 512, VEC, DROP>(a, s, parts, st))
-                          : (small ? bwd_main<T, W, 4, 256, VEC, DROP>(a, s, parts, st)
-                                   : bwd_main<T, W, 4, 512, VEC, DROP>(a, s, parts, st));
+        const bool multi = s.rows_per_cta > 1;
+        rc = s.nch == 1           ? bwd_main<T, W, 1, 256, VEC, DROP, true>(a, s, parts, st)
+             : s.nch == 4         ? bwd_main<T, W, 4, 512, VEC, DROP, false>(a, s, parts, st)
+             : multi              ? bwd_main<T, W, 2, 256, VEC, DROP, true>(a, s, parts, st)
+             : s.threads <= 256   ? bwd_main<T, W, 2, 256, VEC, DROP, false>(a, s, parts, st)
+                                  : bwd_main<T, W, 2, 512, VEC, DROP, false>(a, s, parts, st);
     }
     if (rc || !a.part) return rc;
-    ln_bwd_finish_kernel<W><<<(unsigned)((2 * a.cols + 31) / 32), 256, 0, st>>>(a.part, parts, a.cols, dw, db);
-    return launch_status();
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((2 * a.cols + 31) / 32));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    ACT_CUDA_TRY(cudaLaunchKernelEx(&cfg, ln_bwd_finish_kernel<W>, (const float *)a.part, parts, a.cols, dw, db));
+    return ACT_OK;
 }
 
 // f(T tag, W tag) for the run-time types; wide: float32 weights.
