@@ -244,8 +244,25 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropArgs<T> a, uint32_t un
         }
 #pragma unroll
         for (int k = 0; k < UNROLL; ++k) {
-            const F8 y = drop8<VEC>(unpack<T>(x[k]), a.d.row_offset + row[k], seg0[k], lane, key, a.d);
-            store8<T, VEC>(a.y + row[k] * a.ldy, seg0[k], n[k], lane, y);
+            if constexpr (VEC && sizeof(T) == 2) {
+                // the rounded pairs under a mask of their halves
+                const uint4 r = philox4x32_10((seg0[k] >> 3) + lane, (uint32_t)(a.d.row_offset + row[k]),
+                                              (uint32_t)((a.d.row_offset + row[k]) >> 32), key);
+                const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+                F8 f = unpack<T>(x[k]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f.p[j] = mul2(f.p[j], make_float2(a.d.scale, a.d.scale));
+                Raw8<T> y = pack<T>(f);
+                uint32_t q[4];
+                memcpy(q, &y, 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q[j] &= keep_halves(w[j], a.d.threshold);
+                if (n[k]) *reinterpret_cast<uint4 *>(a.y + row[k] * a.ldy + seg0[k] + 8 * lane) =
+                    make_uint4(q[0], q[1], q[2], q[3]);
+            } else {
+                const F8 y = drop8<VEC>(unpack<T>(x[k]), a.d.row_offset + row[k], seg0[k], lane, key, a.d);
+                store8<T, VEC>(a.y + row[k] * a.ldy, seg0[k], n[k], lane, y);
+            }
         }
         if (u0 + UNROLL * step < u0) break;
     }
@@ -263,13 +280,13 @@ struct FwdArgs {
     DropParams d;
 };
 
-// Sum of v over the warps that share a row; every thread gets the same value.
-// red: NW entries, zero where there is no warp.
-template <int NW, int R>
-__device__ __forceinline__ void row_sums(float (&v)[R], float (*red)[NW], int wpr, int warp, int lane) {
+// Sums over the warps that share a row (ONE: one warp), for R rows; every thread
+// gets the same values.  red: NW entries a row, zero where there is no warp.
+template <int NW, int R, bool ONE>
+__device__ __forceinline__ void row_sums(float (&v)[R], float (*red)[NW], int warp, int lane) {
 #pragma unroll
     for (int i = 0; i < R; ++i) v[i] = warp_sum(v[i]);
-    if (wpr == 1) return;
+    if (ONE) return;
     if (lane == 0) {
 #pragma unroll
         for (int i = 0; i < R; ++i) red[i][warp] = v[i];
@@ -287,9 +304,9 @@ __device__ __forceinline__ void row_sums(float (&v)[R], float (*red)[NW], int wp
     }
 }
 template <int NW>
-__device__ __forceinline__ float row_sum(float v, float (*red)[NW], int wpr, int warp, int lane) {
+__device__ __forceinline__ float row_sum(float v, float (*red)[NW], int warp, int lane) {
     float a[1] = {v};
-    row_sums<NW, 1>(a, red, wpr, warp, lane);
+    row_sums<NW, 1, false>(a, red, warp, lane);
     return a[0];
 }
 // 1 / sqrt(v): the hardware's approximation and one Newton step (the IEEE square
@@ -419,8 +436,10 @@ __device__ __forceinline__ Raw8<T> load8(const RowView<T> &row, int seg0, int co
 }
 
 // MAXT: the launch's thread count rounded up to 256 or 512.
-template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP>
-__global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdArgs<T, W> a, int wpr, int depth) {
+// ONE: a warp per row, else a CTA.
+template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP, bool ONE>
+__global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdArgs<T, W> a, int warps, int depth) {
+    const int wpr = ONE ? 1 : warps;  // warps per row
     extern __shared__ __align__(128) uint8_t dyn[];
     constexpr int NW = MAXT / 32;
     // rows in hand at once: the reductions of two rows overlap and share their barriers
@@ -429,13 +448,13 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdAr
     if (threadIdx.x < 2 * R * NW) red[0][0][threadIdx.x] = 0.f;
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
-    const int rpc = wpr == 1 ? nwarps : 1;  // rows a CTA has in hand at once
-    const int w0 = wpr == 1 ? 0 : warp, mine = wpr == 1 ? warp : 0;
+    const int rpc = ONE ? nwarps : 1;  // rows a CTA has in hand at once
+    const int w0 = ONE ? 0 : warp, mine = ONE ? warp : 0;
     const float inv_n = 1.f / (float)a.cols;
     const uint64_t key = DROP ? drop_seed(a.d) : 0;
     constexpr int IN = DROP ? 2 : 1;
     RowRing<T, IN, VEC> ring;
-    const bool leader = wpr == 1 ? lane == 0 : threadIdx.x == 0;
+    const bool leader = ONE ? lane == 0 : threadIdx.x == 0;
     const int64_t r0 = (int64_t)blockIdx.x * rpc + mine, step = (int64_t)gridDim.x * rpc;
     auto fill = [&](int s, int64_t row) {
         if (row >= a.rows) return;
@@ -483,9 +502,9 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdAr
             }
             s[k] = t.x + t.y;
         }
-        row_sums<NW, R>(s, red[0], wpr, warp, lane);
+        row_sums<NW, R, ONE>(s, red[0], warp, lane);
         // every reader of the slots is past its reads
-        if (wpr == 1) __syncwarp();
+        if (ONE) __syncwarp();
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             if (leader) fill(ring.slot, r + (depth + k) * step);
@@ -512,7 +531,7 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdAr
             }
             q[k] = t.x + t.y;
         }
-        row_sums<NW, R>(q, red[1], wpr, warp, lane);
+        row_sums<NW, R, ONE>(q, red[1], warp, lane);
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             const int64_t rk = r + k * step;
@@ -563,7 +582,7 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_fwd_long_kernel(FwdArgs<T, W>
             const float2 t = add2(add2(v.p[0], v.p[1]), add2(v.p[2], v.p[3]));
             s += t.x + t.y;
         }
-        const float mean = row_sum<nw>(s, red, nw, warp, lane) * inv_n;
+        const float mean = row_sum<nw>(s, red, warp, lane) * inv_n;
         const float2 mean2 = make_float2(mean, mean);
         float q = 0.f;
         for (int64_t g = warp; g < segs; g += nw) {
@@ -579,7 +598,7 @@ __global__ void __launch_bounds__(LONG_THREADS) ln_fwd_long_kernel(FwdArgs<T, W>
             }
             q += t.x + t.y;
         }
-        const float var = row_sum<nw>(q, red + 1, nw, warp, lane) * inv_n;
+        const float var = row_sum<nw>(q, red + 1, warp, lane) * inv_n;
         const float rstd = inv_sqrt(var + a.eps);
         if (threadIdx.x == 0) {
             a.mean[r] = mean;
@@ -985,10 +1004,15 @@ static int fwd_launch(const FwdArgs<T, W> &a, cudaStream_t st) {
         k<<<grid, s.threads, s.smem, st>>>(a, s.wpr, s.depth);
         return launch_status();
     };
-    if (s.nch == 1) return go(ln_fwd_kernel<T, W, 1, 256, VEC, DROP>);
-    if (s.nch == 2) return go(ln_fwd_kernel<T, W, 2, 256, VEC, DROP>);
-    if (s.nch == 3) return go(ln_fwd_kernel<T, W, 3, 256, VEC, DROP>);
-    return s.threads <= 256 ? go(ln_fwd_kernel<T, W, 4, 256, VEC, DROP>) : go(ln_fwd_kernel<T, W, 4, 512, VEC, DROP>);
+    if (s.wpr == 1) {
+        if (s.nch == 1) return go(ln_fwd_kernel<T, W, 1, 256, VEC, DROP, true>);
+        return s.nch == 2 ? go(ln_fwd_kernel<T, W, 2, 256, VEC, DROP, true>) : go(ln_fwd_kernel<T, W, 4, 256, VEC, DROP, true>);
+    }
+    if (s.nch == 1) return go(ln_fwd_kernel<T, W, 1, 256, VEC, DROP, false>);
+    if (s.nch == 2) return go(ln_fwd_kernel<T, W, 2, 256, VEC, DROP, false>);
+    if (s.nch == 3) return go(ln_fwd_kernel<T, W, 3, 256, VEC, DROP, false>);
+    return s.threads <= 256 ? go(ln_fwd_kernel<T, W, 4, 256, VEC, DROP, false>)
+                            : go(ln_fwd_kernel<T, W, 4, 512, VEC, DROP, false>);
 }
 
 template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP, bool MULTI>
