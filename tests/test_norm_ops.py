@@ -441,3 +441,79 @@ def test_refusals():
                 lambda: A.layer_norm(x.half(), w, w.half())):
         with pytest.raises(TypeError):
             bad()
+
+
+# ---------------------------------------------------------------- custom ops and the example
+def test_custom_ops_have_fake_forms():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import actcomp.ops  # noqa: F401
+
+    with FakeTensorMode():
+        x, w, seed = torch.empty(6, 40), torch.empty(40), torch.empty(1, dtype=torch.int64)
+        o = torch.ops.actcomp
+        assert o.dropout(x, 0.1, seed, 0).shape == (6, 40)
+        y, m, r = o.layer_norm(x, w, w, 1e-5)
+        assert m.shape == r.shape == (6,) and m.dtype == torch.float32
+        assert [t.shape for t in o.layer_norm_backward(x, x, w, m, r)] == [(6, 40), (40,), (40,)]
+        assert len(o.dropout_add_layer_norm(x, x, w, w, 0.1, seed, 0, 1e-5)) == 4
+        assert o.dropout_add_layer_norm_backward(x, x, w, m, r, 0.1, seed, 0, None)[2].shape == (40,)
+        c, s = o.mx4_quantize(x, True)
+        assert c.shape == (40, 16) and s.shape == (512,)
+        c, s = o.mx4_quantize(x, False)
+        assert o.mx4_linear(x, c, s, torch.bfloat16).shape == (6, 6)
+
+
+@pytest.mark.gpu
+def test_custom_ops_run_the_operators():
+    import actcomp
+    import actcomp.ops  # noqa: F401
+    from actcomp import mx4
+
+    o = torch.ops.actcomp
+    x, w = data(64, 256, torch.bfloat16, 1).cuda(), data(1, 256, torch.bfloat16, 2).cuda()[0]
+    seed = torch.tensor([5], device="cuda")
+    assert torch.equal(o.dropout(x, 0.2, seed, 3), actcomp.dropout(x, 0.2, 5, 3))
+    for a, b in zip(o.dropout_add_layer_norm(x, x, w, w, 0.2, seed, 0, 1e-5),
+                    actcomp.dropout_add_layer_norm(x, x, w, w, 0.2, 5)):
+        assert torch.equal(a, b)
+    y, m, r = o.layer_norm(x, w, w, 1e-5)
+    for a, b in zip(o.dropout_add_layer_norm_backward(y, x, w, m, r, 0.2, seed, 0, x),
+                    actcomp.dropout_add_layer_norm_backward(y, x, w, m, r, 0.2, 5, dh=x)):
+        assert torch.equal(a, b)
+    c, s = o.mx4_quantize(x, False)
+    assert torch.equal(o.mx4_linear(x, c, s, torch.bfloat16), mx4.linear(x, mx4.quantize(x)))
+
+
+@pytest.mark.gpu
+def test_captured_graph_draws_new_masks_from_a_seed_tensor():
+    import actcomp
+
+    x, seed = data(32, 512, torch.bfloat16, 1).cuda(), torch.tensor([7], device="cuda")
+    actcomp.dropout(x, 0.3, seed)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = actcomp.dropout(x, 0.3, seed)
+    for s in (7, 8):
+        seed.fill_(s)
+        g.replay()
+        assert torch.equal(y, actcomp.dropout(x, 0.3, s))
+
+
+@pytest.mark.gpu
+def test_residual_step_example():
+    """Against the float32 step.  e2m1 has one mantissa bit: rounding to it is off
+    by at most 1/4 of a value above a block's smallest step, saturation by 1/4, and
+    the step itself bounds small values: under 0.15 of a block's norm for normal
+    values, so under 0.25 for a product of two such operands (errors add in squares:
+    0.15 sqrt 2 = 0.21).  What needs no 4-bit gradient input is far closer."""
+    import importlib.util
+
+    path = os.path.join(ROOT, "triton-kernel-test_b200", "examples", "residual_step.py")
+    spec = importlib.util.spec_from_file_location("residual_step", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    r = m.main(tokens=512, channels=256, out=384)
+    for rep in r.values():
+        assert all(v < 0.25 for k, v in rep.items() if k != "bytes"), rep
+    assert r[True]["bytes"] < 0.75 * r[False]["bytes"]

@@ -10,7 +10,7 @@ from typing import Optional
 
 import torch
 
-from . import core, refcompat
+from . import core, mx4, norm, refcompat
 
 _U8, _F32, _BF = torch.uint8, torch.float32, torch.bfloat16
 
@@ -128,3 +128,94 @@ def _(a, b, out_dtype, activation):
         batch = max(a.shape[0] if a.dim() == 3 else 1, b.shape[0] if b.dim() == 3 else 1)
         return a.new_empty((batch, a.shape[-2], b.shape[-1]), dtype=out_dtype)
     return a.new_empty((a.shape[0], b.shape[1]), dtype=out_dtype)
+
+
+# ---------------------------------------------------------------- residual branch
+@torch.library.custom_op("actcomp::dropout", mutates_args=())
+def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, row_offset: int) -> torch.Tensor:
+    """norm.dropout with the seed as a one-element int64 tensor (its backward is itself, on the gradient)."""
+    return norm.dropout(x, p, seed, row_offset)
+
+
+@dropout.register_fake
+def _(x, p, seed, row_offset):
+    return _empty(x.shape, x.dtype, x)
+
+
+@torch.library.custom_op("actcomp::layer_norm", mutates_args=())
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+               eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return norm.layer_norm(x, weight, bias, eps)
+
+
+@layer_norm.register_fake
+def _(x, weight, bias, eps):
+    return _empty(x.shape, x.dtype, x), _empty(x.shape[:-1], _F32, x), _empty(x.shape[:-1], _F32, x)
+
+
+@torch.library.custom_op("actcomp::layer_norm_backward", mutates_args=())
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor,
+                        rstd: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return norm.layer_norm_backward(dy, x, weight, mean, rstd)
+
+
+@layer_norm_backward.register_fake
+def _(dy, x, weight, mean, rstd):
+    return _empty(x.shape, x.dtype, x), _empty(weight.shape, weight.dtype, x), _empty(weight.shape, weight.dtype, x)
+
+
+@torch.library.custom_op("actcomp::dropout_add_layer_norm", mutates_args=())
+def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor],
+                           bias: Optional[torch.Tensor], p: float, seed: torch.Tensor, row_offset: int,
+                           eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return norm.dropout_add_layer_norm(x, residual, weight, bias, p, seed, row_offset, eps)
+
+
+@dropout_add_layer_norm.register_fake
+def _(x, residual, weight, bias, p, seed, row_offset, eps):
+    return (_empty(x.shape, x.dtype, x), _empty(x.shape, x.dtype, x), _empty(x.shape[:-1], _F32, x),
+            _empty(x.shape[:-1], _F32, x))
+
+
+@torch.library.custom_op("actcomp::dropout_add_layer_norm_backward", mutates_args=())
+def dropout_add_layer_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor,
+                                    rstd: torch.Tensor, p: float, seed: torch.Tensor, row_offset: int,
+                                    dh: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor,
+                                                                         torch.Tensor]:
+    return norm.dropout_add_layer_norm_backward(dy, h, weight, mean, rstd, p, seed, row_offset, dh)
+
+
+@dropout_add_layer_norm_backward.register_fake
+def _(dy, h, weight, mean, rstd, p, seed, row_offset, dh):
+    return (_empty(h.shape, h.dtype, h), _empty(h.shape, h.dtype, h), _empty(weight.shape, weight.dtype, h),
+            _empty(weight.shape, weight.dtype, h))
+
+
+# ---------------------------------------------------------------- microscaled 4-bit
+def _mx4_shapes(rows, cols):
+    return (rows, (cols + 31) // 32 * 16), ((rows + 127) // 128 * ((cols + 127) // 128) * 512,)
+
+
+@torch.library.custom_op("actcomp::mx4_quantize", mutates_args=())
+def mx4_quantize(x: torch.Tensor, transpose: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of mx4.quantize."""
+    q = mx4.quantize(x, transpose)
+    return q.codes, q.scales
+
+
+@mx4_quantize.register_fake
+def _(x, transpose):
+    rows, cols = x.numel() // x.shape[-1], x.shape[-1]
+    c, s = _mx4_shapes(cols, rows) if transpose else _mx4_shapes(rows, cols)
+    return _empty(c, _U8, x), _empty(s, _U8, x)
+
+
+@torch.library.custom_op("actcomp::mx4_linear", mutates_args=())
+def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
+    """mx4.linear with the weight's buffers (codes: (N, K / 2 rounded up to blocks))."""
+    return mx4.linear(x, mx4.Mx4(codes.shape[0], x.shape[-1], codes, scales, x.dtype), out_dtype)
+
+
+@mx4_linear.register_fake
+def _(x, codes, scales, out_dtype):
+    return _empty(x.shape[:-1] + (codes.shape[0],), out_dtype, x)

@@ -244,25 +244,8 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropArgs<T> a, uint32_t un
         }
 #pragma unroll
         for (int k = 0; k < UNROLL; ++k) {
-            if constexpr (VEC && sizeof(T) == 2) {
-                // the rounded pairs under a mask of their halves
-                const uint4 r = philox4x32_10((seg0[k] >> 3) + lane, (uint32_t)(a.d.row_offset + row[k]),
-                                              (uint32_t)((a.d.row_offset + row[k]) >> 32), key);
-                const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-                F8 f = unpack<T>(x[k]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) f.p[j] = mul2(f.p[j], make_float2(a.d.scale, a.d.scale));
-                Raw8<T> y = pack<T>(f);
-                uint32_t q[4];
-                memcpy(q, &y, 16);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) q[j] &= keep_halves(w[j], a.d.threshold);
-                if (n[k]) *reinterpret_cast<uint4 *>(a.y + row[k] * a.ldy + seg0[k] + 8 * lane) =
-                    make_uint4(q[0], q[1], q[2], q[3]);
-            } else {
-                const F8 y = drop8<VEC>(unpack<T>(x[k]), a.d.row_offset + row[k], seg0[k], lane, key, a.d);
-                store8<T, VEC>(a.y + row[k] * a.ldy, seg0[k], n[k], lane, y);
-            }
+            const F8 y = drop8<VEC>(unpack<T>(x[k]), a.d.row_offset + row[k], seg0[k], lane, key, a.d);
+            store8<T, VEC>(a.y + row[k] * a.ldy, seg0[k], n[k], lane, y);
         }
         if (u0 + UNROLL * step < u0) break;
     }

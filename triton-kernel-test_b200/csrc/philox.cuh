@@ -46,20 +46,6 @@ __device__ __forceinline__ uint4 philox4x32_10(uint32_t c0, uint32_t c2, uint32_
     return make_uint4(c0, c1, c2, c3);
 }
 
-// 0xffff in each half of the word that is kept (>= threshold), else 0.  Two halves
-// at a time: with t = threshold mod 2^15 the top bit of (h | 2^15) - t says whether
-// h's low 15 bits reach t, and no half borrows from the other; with h's own top
-// bit it is an OR below 2^15, an AND above (three-input majority with the flag).
-__device__ __forceinline__ uint32_t keep_halves(uint32_t w, uint32_t threshold) {
-    const uint32_t low = threshold <= 0x8000u ? 0xffffffffu : 0u;
-    const uint32_t t = threshold <= 0x8000u ? threshold : threshold - 0x8000u;
-    const uint32_t d = (w | 0x80008000u) - (t | t << 16);
-    const uint32_t k = (w & d) | ((w | d) & low);
-    uint32_t m;
-    asm("prmt.b32 %0, %1, 0, 0xBB99;" : "=r"(m) : "r"(k));  // the sign of bytes 1, 1, 3, 3
-    return m;
-}
-
 // Bit j of the result: whether value 8 * block + j of the row is kept.
 __device__ __forceinline__ uint32_t drop_keep8(uint64_t row, uint32_t block, uint64_t key, uint32_t threshold) {
     const uint4 r = philox4x32_10(block, (uint32_t)row, (uint32_t)(row >> 32), key);
