@@ -50,7 +50,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return r;
 }
 __device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
-    return pack2(v[0], v[1]) | pack2(v[2], v[3]) << 8 | pack2(v[4], v[5]) << 16 | pack2(v[6], v[7]) << 24;
+    const uint32_t lo = __byte_perm(pack2(v[0], v[1]), pack2(v[2], v[3]), 0x0040);
+    const uint32_t hi = __byte_perm(pack2(v[4], v[5]), pack2(v[6], v[7]), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
 }
 // Codes j and j + 4 of a word as a pair of fp16 times 2^-14 (exact): the sign to
 // bit 15, exponent and mantissa to bits 11..9.  With fp16's bias of 15 against

@@ -14,50 +14,63 @@
 namespace act {
 namespace mx4 {
 
-// By rows: one warp per 256 columns of a row, two rows at a time; blockIdx.y
-// covers the columns, blockIdx.x strides over the rows, rounded up to atoms.
+// The 4 x 4 bytes of a, b, c, d (rows) transposed.
+__device__ __forceinline__ uint4 transpose_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);  // a0 b0 a1 b1 | a2 b2 a3 b3
+    const uint32_t cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
+    return make_uint4(__byte_perm(ab0, cd0, 0x5410), __byte_perm(ab0, cd0, 0x7632), __byte_perm(ab1, cd1, 0x5410),
+                      __byte_perm(ab1, cd1, 0x7632));
+}
+
+// By rows: a warp takes 256 columns of the four rows r0, r0 + 32, r0 + 64,
+// r0 + 96 of a scale atom, whose four scale words lie in one 16-byte piece;
+// blockIdx.y covers the columns, blockIdx.x strides over the rows' groups.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-    quant_rows_kernel(const T *x, int64_t rows, int64_t cols, int64_t ldx, uint8_t *codes, uint8_t *scales) {
+    quant_rows_kernel(const T *x, int rows, int cols, int64_t ldx, uint8_t *codes, uint8_t *scales) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int sg = blockIdx.y;
-    const int64_t nka = atoms_of(cols), rb = row_bytes(cols), c = (int64_t)sg * 256 + 8 * lane;
-    const int64_t all = (rows + 127) / 128 * 128, step = (int64_t)gridDim.x * 8;
-    const int n = c >= cols ? 0 : (cols - c < 8 ? (int)(cols - c) : 8);
-    const bool code = c < blocks_of(cols) * BLOCK;
-    const int64_t ka = sg * 2 + (lane >> 4);
+    const int sg = blockIdx.y, c = sg * 256 + 8 * lane;
+    const int nka = (int)atoms_of(cols);
+    const int64_t rb = row_bytes(cols);
+    const int groups = (rows + 127) / 128 * 32, step = gridDim.x * 8;
+    const int n = c >= cols ? 0 : (cols - c < 8 ? cols - c : 8);
+    const bool code = c < (int)blocks_of(cols) * BLOCK;
+    const int ka = sg * 2 + (lane >> 4);
     const bool word = (lane & 15) == 0 && ka < nka;
-    constexpr int UNROLL = 2;
-    for (int64_t r0 = (int64_t)blockIdx.x * 8 + warp; r0 < all; r0 += UNROLL * step) {
-        Raw8<T> raw[UNROLL];
+    for (int g = blockIdx.x * 8 + warp; g < groups; g += step) {
+        const int r0 = (g >> 5) * 128 + (g & 31);
+        const T *src = x + r0 * ldx + c;
+        Raw8<T> raw[4];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int64_t r = r0 + u * step;
-            if (r < rows && n == 8 && VEC) raw[u].load_vec(x + r * ldx + c);
-            else if (r < rows && n > 0) raw[u].load(x + r * ldx + c, n);
-            else raw[u].zero();
+        for (int j = 0; j < 4; ++j) {
+            const bool live = r0 + 32 * j < rows;
+            if (VEC && live && n == 8) raw[j].load_vec(src + 32 * j * ldx);
+            else raw[j].load(src + 32 * j * ldx, live ? n : 0);
         }
+        uint8_t *dst = codes + r0 * rb + c / 2;
+        uint32_t sc4 = 0;
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int64_t r = r0 + u * step;
-            uint32_t m = raw[u].amax();
+        for (int j = 0; j < 4; ++j) {
+            uint32_t m = raw[j].amax();
             m = max_of<T>(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = max_of<T>(m, __shfl_xor_sync(0xffffffffu, m, 2));
             const uint32_t sc = scale_code(amax_bits<T>(m));
-            if (r < rows && code) {
+            sc4 |= sc << (8 * j);
+            if (code && r0 + 32 * j < rows) {
                 const float inv = inv_scale(sc);
                 float v[8];
-                raw[u].floats(v);
+                raw[j].floats(v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] *= inv;
-                *reinterpret_cast<uint32_t *>(codes + r * rb + c / 2) = pack8(v);
+                for (int k = 0; k < 8; ++k) v[k] *= inv;
+                *reinterpret_cast<uint32_t *>(dst + 32 * j * rb) = pack8(v);
             }
-            // four blocks' scale bytes to one word (lanes 0 and 16)
-            uint32_t w = sc;
-            w |= __shfl_down_sync(0xffffffffu, w, 4) << 8;
-            w |= __shfl_down_sync(0xffffffffu, w, 8) << 16;
-            if (word && r < all) *reinterpret_cast<uint32_t *>(scales + scale_word(r, ka, nka)) = w;
         }
+        // four blocks x four rows of scale bytes (lanes 0 and 16)
+        const uint32_t b1 = __shfl_down_sync(0xffffffffu, sc4, 4), b2 = __shfl_down_sync(0xffffffffu, sc4, 8),
+                       b3 = __shfl_down_sync(0xffffffffu, sc4, 12);
+        if (word)
+            *reinterpret_cast<uint4 *>(scales + ((int64_t)(g >> 5) * nka + ka) * ATOM_BYTES + (g & 31) * 16) =
+                transpose_bytes(sc4, b1, b2, b3);
     }
 }
 
@@ -197,35 +210,38 @@ __global__ void __launch_bounds__(256)
         *reinterpret_cast<uint32_t *>(scales_t + scale_word(c0 + tid, kr, nka_t)) = words[tid];
 }
 
-// By rows like quant_rows_kernel: a lane eight values, a warp 256 columns.
+// Rows and columns as in quant_rows_kernel: one 16-byte load brings a lane the
+// scales of its four rows.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-    dequant_kernel(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, T *out, int64_t ldo) {
+    dequant_kernel(const uint8_t *codes, const uint8_t *scales, int rows, int cols, T *out, int64_t ldo) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     __shared__ __align__(16) uint8_t turn[VEC ? 1 : 8][VEC ? 16 : 256 * sizeof(T)];
-    const int64_t c = (int64_t)blockIdx.y * 256 + 8 * lane;
-    const int64_t nka = atoms_of(cols), rb = row_bytes(cols), step = (int64_t)gridDim.x * 8;
-    const int n = c >= cols ? 0 : (cols - c < 8 ? (int)(cols - c) : 8);
-    constexpr int UNROLL = 4;
-    for (int64_t r0 = (int64_t)blockIdx.x * 8 + warp; r0 < rows; r0 += UNROLL * step) {
-        uint32_t q[UNROLL];
-        uint8_t sc[UNROLL];
+    const int c0 = blockIdx.y * 256, c = c0 + 8 * lane;
+    const int nka = (int)atoms_of(cols), groups = (rows + 127) / 128 * 32, step = gridDim.x * 8;
+    const int64_t rb = row_bytes(cols);
+    const int n = c >= cols ? 0 : (cols - c < 8 ? cols - c : 8);
+    const int sh = 8 * ((c >> 5) & 3);
+    for (int g = blockIdx.x * 8 + warp; g < groups; g += step) {
+        const int r0 = (g >> 5) * 128 + (g & 31);
+        if (r0 >= rows) continue;  // the same for the warp
+        const uint8_t *src = codes + r0 * rb + c / 2;
+        uint32_t q[4] = {};
+        uint4 s4 = make_uint4(0, 0, 0, 0);
+        if (n > 0) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int64_t r = r0 + u * step;
-            q[u] = 0, sc[u] = 0;
-            if (r < rows && n > 0) {
-                q[u] = *reinterpret_cast<const uint32_t *>(codes + r * rb + c / 2);
-                sc[u] = scales[scale_word(r, c >> 7, nka) + ((c >> 5) & 3)];
-            }
+            for (int j = 0; j < 4; ++j)
+                if (r0 + 32 * j < rows) q[j] = *reinterpret_cast<const uint32_t *>(src + 32 * j * rb);
+            s4 = *reinterpret_cast<const uint4 *>(scales + ((int64_t)(g >> 5) * nka + (c >> 7)) * ATOM_BYTES +
+                                                  (g & 31) * 16);
         }
+        const uint32_t sc[4] = {(s4.x >> sh) & 255u, (s4.y >> sh) & 255u, (s4.z >> sh) & 255u, (s4.w >> sh) & 255u};
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int64_t r = r0 + u * step;
-            if (r >= rows) break;
+        for (int j = 0; j < 4; ++j) {
+            if (r0 + 32 * j >= rows) break;
             __half2 h[4];
-            tiny8(q[u], h);
-            const float s = scale_value(sc[u]);
+            tiny8(q[j], h);
+            const float s = scale_value(sc[j]);
             float f[8];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -244,17 +260,18 @@ __global__ void __launch_bounds__(256)
                     memcpy(&w[k], &o, 4);
                 }
             }
-            T *d = out + r * ldo + c;
+            T *row = out + (r0 + 32 * j) * ldo + c0;
             if (VEC && n == 8) {
 #pragma unroll
                 for (int k = 0; k < (int)sizeof(T) / 2; ++k)
-                    reinterpret_cast<uint4 *>(d)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                    reinterpret_cast<uint4 *>(row + 8 * lane)[k] =
+                        make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
             } else if (VEC) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j < n) {
-                        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(d)[j] = w[j];
-                        else reinterpret_cast<uint16_t *>(d)[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                for (int k = 0; k < 8; ++k)
+                    if (k < n) {
+                        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(row)[8 * lane + k] = w[k];
+                        else reinterpret_cast<uint16_t *>(row)[8 * lane + k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
                     }
             } else {  // through shared memory, so that neighbouring lanes store neighbouring values
                 uint4 *mine = reinterpret_cast<uint4 *>(turn[warp]) + lane * (sizeof(T) / 2);
@@ -262,12 +279,11 @@ __global__ void __launch_bounds__(256)
                 for (int k = 0; k < (int)sizeof(T) / 2; ++k)
                     mine[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
                 __syncwarp();
-                T *row = out + r * ldo + (c - 8 * lane);
-                const int left = (int)(cols - (c - 8 * lane) < 256 ? cols - (c - 8 * lane) : 256);
-                const T *src = reinterpret_cast<const T *>(turn[warp]);
+                const int left = cols - c0 < 256 ? cols - c0 : 256;
+                const T *v = reinterpret_cast<const T *>(turn[warp]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (32 * j + lane < left) row[32 * j + lane] = src[32 * j + lane];
+                for (int k = 0; k < 8; ++k)
+                    if (32 * k + lane < left) row[32 * k + lane] = v[32 * k + lane];
                 __syncwarp();
             }
         }
@@ -292,7 +308,7 @@ static int check(const actcomp_mx4 *q) {
 // Grid of the row kernels: y covers the columns, x the rows with enough CTAs to
 // fill the device `waves` times over.
 static bool row_grid(dim3 &g, int64_t rows, int64_t cols, int waves) {
-    const int64_t segs = (cols + 255) / 256, need = (rows + 7) / 8;
+    const int64_t segs = (cols + 255) / 256, need = (rows + 127) / 128 * 4;  // eight warps a CTA, four rows a warp
     if (segs > 65535) return false;
     int64_t x = ((int64_t)num_sms() * waves + segs - 1) / segs;
     g = dim3((unsigned)(x < need ? x : need), (unsigned)segs);
@@ -329,14 +345,14 @@ extern "C" int actcomp_mx4_quantize(const void *x, int64_t rows, int64_t cols, i
     ACT_CHECK(aligned(x, es), ACT_E_ALIGN);
     const bool vec = aligned(x, 16) && (ldx * es) % 16 == 0;
     dim3 grid;
-    if (!qt) ACT_CHECK(row_grid(grid, (rows + 127) / 128 * 128, cols, 16), ACT_E_UNSUPPORTED);
+    if (!qt) ACT_CHECK(row_grid(grid, rows, cols, 16), ACT_E_UNSUPPORTED);
     cudaStream_t st = as_stream(stream);
     return with_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
         const T *xs = static_cast<const T *>(x);
         if (!qt) {
-            if (vec) quant_rows_kernel<T, true><<<grid, 256, 0, st>>>(xs, rows, cols, ldx, q->codes, q->scales);
-            else quant_rows_kernel<T, false><<<grid, 256, 0, st>>>(xs, rows, cols, ldx, q->codes, q->scales);
+            if (vec) quant_rows_kernel<T, true><<<grid, 256, 0, st>>>(xs, (int)rows, (int)cols, ldx, q->codes, q->scales);
+            else quant_rows_kernel<T, false><<<grid, 256, 0, st>>>(xs, (int)rows, (int)cols, ldx, q->codes, q->scales);
             return launch_status();
         }
         const int smem = 128 * (128 + 16 / (int)sizeof(T)) * (int)sizeof(T) + 512;
@@ -365,8 +381,8 @@ extern "C" int actcomp_mx4_dequantize(const actcomp_mx4 *q, void *out, int64_t l
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
         T *o = static_cast<T *>(out);
-        if (vec) dequant_kernel<T, true><<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols, o, ldo);
-        else dequant_kernel<T, false><<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols, o, ldo);
+        if (vec) dequant_kernel<T, true><<<grid, 256, 0, st>>>(q->codes, q->scales, (int)q->rows, (int)q->cols, o, ldo);
+        else dequant_kernel<T, false><<<grid, 256, 0, st>>>(q->codes, q->scales, (int)q->rows, (int)q->cols, o, ldo);
         return launch_status();
     });
 }
