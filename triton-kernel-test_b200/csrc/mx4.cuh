@@ -86,6 +86,17 @@ __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return _
 template <>
 __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
 
+// Larger magnitude of each 16-bit half of m (magnitudes) and v; NaN stays.
+template <typename T>
+__device__ __forceinline__ uint32_t absmax2(uint32_t m, uint32_t v) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm("{\n .reg .b32 t;\n abs.bf16x2 t, %2;\n max.NaN.bf16x2 %0, %1, t;\n}" : "=r"(r) : "r"(m), "r"(v));
+    else
+        asm("{\n .reg .b32 t;\n abs.f16x2 t, %2;\n max.NaN.f16x2 %0, %1, t;\n}" : "=r"(r) : "r"(m), "r"(v));
+    return r;
+}
+
 // Eight values as their words; zero() is eight zeros in every type.
 template <typename T>
 struct Raw8 {
@@ -142,8 +153,7 @@ struct Raw8 {
             for (int j = 0; j < 8; ++j) m = max(m, w[j] & 0x7fffffffu);
             return m;
         } else {
-            uint32_t m = __vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu);
-            return __vmaxu2(m, __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+            return absmax2<T>(absmax2<T>(absmax2<T>(absmax2<T>(0u, w[0]), w[1]), w[2]), w[3]);
         }
     }
 };

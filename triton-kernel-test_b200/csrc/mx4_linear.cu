@@ -1,9 +1,9 @@
 // mx4_linear.cu -- x . w^T for a few tokens: x is quantised by rows on the way,
 // w is a microscaled 4-bit matrix.
 //
-// What bounds it is the weight's 17/32 byte a value, read once, and the latency
-// of one launch; the tensor cores' 128-row tiles would be nearly empty and the
-// separate quantisation a second launch.  Every CTA quantises all of x (it is
+// It cannot do without the weight's 17/32 byte a value, read once, and one launch;
+// the tensor cores' 128-row tiles would be nearly empty and the quantisation a
+// launch of its own (16.0 us for both at 1 x 4096 x 11008, 8.9 us here).  Every CTA quantises all of x (it is
 // small) into shared memory as 8-bit integers (twice the e2m1 value: 0, 1, 2, 3,
 // 4, 6, 8, 12 and their negatives), one scale per block.
 //   warp  the four rows r0, r0 + 32, r0 + 64, r0 + 96 of a scale atom, whose
@@ -14,9 +14,8 @@
 // one of eight table bytes, the fourth (the sign) replaces it by its sign bit,
 // 0; the codes with their signs flipped give the negative ones' magnitudes.
 // Few rows: a CTA's warps share rows and split their blocks (KS).
-// Decoding and __dp4a bound it (three quarters of the time), not the weight's
-// bytes: fp16 pairs and HFMA2 instead took 10.8 us where this takes 9.0
-// (1 x 4096 x 11008).
+// Decoding and __dp4a bound it, not the weight's bytes (24 MB, 3.7 us): each
+// further token adds 3.2 us.  fp16 pairs and HFMA2 instead took 10.8 us.
 #include "mx4.cuh"
 
 namespace act {

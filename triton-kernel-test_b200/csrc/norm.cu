@@ -20,12 +20,23 @@
 //
 // Work split.  A warp holds a row in segments of 256 values, eight a lane: a
 // lane's own eight consecutive values where 16-byte access is possible (VEC),
-// else values lane, lane + 32, ... of the segment, so that narrow loads still
+// else values lane, lane + 32, ... of the segment, so that narrow accesses still
 // coalesce; the lane then makes the generator call of block `lane` of the
-// segment and the keep bits travel by shuffle.  Rows of up to 1024 values take
-// a warp each, rows of up to 16384 a CTA each (both persistent: weights and
-// the weight-gradient sums stay in registers from row to row); longer rows go
+// segment and the keep bits travel by shuffle.  Rows arrive ahead of their use
+// by bulk copies into shared memory (RowRing).  Persistent CTAs: weights and the
+// weight-gradient sums stay in registers from row to row.  Short rows take a warp
+// or a group of warps each, rows of up to 16384 values a CTA; longer ones go
 // through kernels that re-read the row.
+//
+// Measured on a B200, 16384 x 4096 bf16 (share of the copy rate, 6.47 TB/s):
+//   dropout                 60 us  4.5 TB/s  70 %  (the generator's multiplies; float32 87 us, 95 %)
+//   forward                 47 us  5.7 TB/s  88 %
+//   backward                70 us  5.7 TB/s  89 %
+//   branch forward          98 us  5.5 TB/s  85 %
+//   branch backward        121 us  5.5 TB/s  86 %
+// Before the ring (loads in the row's own time) forward took 123 us and backward
+// 245; value by value instead of in pairs 90 and 112.  Ragged rows (16384 x 4097)
+// take 91 and 198 us: two-byte accesses, four times the instructions.
 #include <cuda_fp16.h>
 #include <string.h>
 

@@ -7,12 +7,12 @@
 //   counter = (column >> 3, 0, row's low 32 bits, row's high 32 bits), key = seed;
 //   the four output words are eight 16-bit halves, half column & 7 decides:
 //   kept iff half >= threshold, threshold = round(p * 2^16) in 0 .. 2^16.
-// Sixteen bits a value: one generator call serves eight values (one 16-byte
-// load of a 16-bit type), which keeps the integer pipes below the memory time
-// (at 32 bits a value the 20 wide products a call would be the bound: about
-// 1.6e12 values/s pass through HBM); the scale uses the held probability
-// threshold / 2^16, so the expectation is exact.  Rows count from row_offset:
-// a token shard that passes its first row draws the same mask as the whole.
+// Sixteen bits a value: one generator call serves eight values, one 16-byte load
+// of a 16-bit type.  The 20 wide products of a call are then a fifth of a bf16
+// dropout's time (16384 x 4096: 60 us, with one round instead of ten 50 us); at 32
+// bits a value there would be twice as many.  The scale uses the held probability
+// threshold / 2^16, so the expectation is exact.  Rows count from row_offset: a
+// token shard that passes its first row draws the same mask as the whole.
 #pragma once
 
 #include <stdint.h>
