@@ -242,14 +242,15 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropArgs<T> a, uint32_t un
     constexpr int UNROLL = 2;
     for (uint32_t u0 = blockIdx.x * 8u + (threadIdx.x >> 5); u0 < units; u0 += UNROLL * step) {
         Raw8<T> x[UNROLL];
-        uint32_t row[UNROLL], seg0[UNROLL];
+        uint32_t row[UNROLL];
+        int64_t seg0[UNROLL];
         int n[UNROLL];
 #pragma unroll
         for (int k = 0; k < UNROLL; ++k) {
             const uint32_t u = u0 + k * step;
             const uint32_t hi = __umulhi(u, mul);
             row[k] = mul ? (((u - hi) >> 1) + hi) >> shift : u;
-            seg0[k] = (u - row[k] * segs) * SEG;
+            seg0[k] = (int64_t)(u - row[k] * segs) * SEG;
             n[k] = u < units && u >= u0 ? count_of<VEC>(seg0[k], a.cols, lane) : 0;
             x[k] = load8<T, VEC>(a.x + row[k] * a.ldx, seg0[k], n[k], lane);
         }
