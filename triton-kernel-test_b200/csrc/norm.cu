@@ -311,9 +311,9 @@ __device__ __forceinline__ float inv_sqrt(float v) {
     return v > 0.f && v < INFINITY ? h : r;
 }
 
-// Resident CTAs for launches of up to 256 or 512 threads (register use).
+// Resident CTAs for launches of up to 256, 320 or 512 threads (register use).
 __host__ __device__ constexpr int fwd_ctas(int nch, int maxt) { return maxt > 256 ? 1 : (nch == 1 ? 3 : 2); }
-__host__ __device__ constexpr int bwd_ctas(int maxt) { return maxt > 256 ? 1 : 2; }
+__host__ __device__ constexpr int bwd_ctas(int maxt) { return maxt > 320 ? 1 : 2; }
 constexpr int MAX_DEPTH = 4;
 constexpr int RING_HEAD = 8 * MAX_DEPTH * 8 + 16;  // barriers of up to eight warps' rings, the abort word
 // Bytes of a row in a slot.
@@ -430,7 +430,7 @@ __device__ __forceinline__ Raw8<T> load8(const RowView<T> &row, int seg0, int co
     }
 }
 
-// MAXT: the launch's thread count rounded up to 256 or 512.
+// MAXT: the launch's thread count rounded up to 256, 320 or 512.
 // ONE: a warp per row, else a CTA.
 template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP, bool ONE>
 __global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdArgs<T, W> a, int warps, int depth) {
@@ -679,8 +679,10 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
     if (leader)
         for (int i = 0; i < depth; ++i) fill(i, r0 + i * step);
     // Up to two segments a thread the row's g and x-hat are held from the sums to
-    // the output, past that they are computed again from the slot (registers).
-    constexpr bool HOLD = NCH <= 2;
+    // the output, past that they are computed again from the slot (registers); so
+    // too at 320 threads, where that fits two CTAs (8192 x 5120 bf16 with dropout
+    // 89 us; held, in one CTA, 99 us; float32 is the other way, 89 us and 82 us).
+    constexpr bool HOLD = NCH <= 2 && MAXT != 320;
     // four segments: their sums fill the registers, the weights are read again too
     constexpr bool WREG = NCH <= 2;
     Raw8<W> wv[WREG ? NCH : 1];
@@ -938,7 +940,7 @@ static Shape shape_of(int64_t cols, int esize, bool drop, bool bwd, bool vec) {
     }
     const int inputs = (bwd ? 2 : 1) + (drop ? 1 : 0);
     const int64_t slot = (int64_t)row_pitch(cols, esize, vec) * inputs * s.rows_per_cta;
-    s.per_sm = bwd ? bwd_ctas(s.threads) : fwd_ctas(s.nch, s.threads) * (s.threads <= 128 ? 2 : 1);
+    s.per_sm = bwd ? (esize == 4 && s.threads > 256 ? 1 : bwd_ctas(s.threads)) : fwd_ctas(s.nch, s.threads) * (s.threads <= 128 ? 2 : 1);
     const int64_t room = SLOT_ROOM / s.per_sm;
     s.depth = (int)(room / slot < MAX_DEPTH ? room / slot : MAX_DEPTH);
     if (s.depth < 2) {  // the longest rows: one CTA per SM
@@ -1038,6 +1040,7 @@ static int bwd_launch(BwdArgs<T, W> a, W *dw, W *db, void *ws, cudaStream_t st) 
              : s.nch == 4         ? bwd_main<T, W, 4, 512, VEC, DROP, false>(a, s, parts, st)
              : multi              ? bwd_main<T, W, 2, 256, VEC, DROP, true>(a, s, parts, st)
              : s.threads <= 256   ? bwd_main<T, W, 2, 256, VEC, DROP, false>(a, s, parts, st)
+             : s.per_sm == 2      ? bwd_main<T, W, 2, 320, VEC, DROP, false>(a, s, parts, st)
                                   : bwd_main<T, W, 2, 512, VEC, DROP, false>(a, s, parts, st);
     }
     if (rc || !a.part) return rc;
