@@ -28,7 +28,6 @@ import torch
 from . import _lib
 
 _host = _lib.host()
-BLOCK = 32
 
 
 @dataclass

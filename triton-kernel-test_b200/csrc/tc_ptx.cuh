@@ -4,8 +4,7 @@
 // and the shared-memory / instruction descriptors of tcgen05.mma.
 //
 // Descriptor bit layouts follow the PTX ISA (tcgen05 "shared memory
-// descriptor" and "instruction descriptor" tables), as also spelled out in
-// CUTLASS cute/arch/mma_sm100_desc.hpp.
+// descriptor" and "instruction descriptor" tables).
 #pragma once
 
 #include <cuda.h>
