@@ -49,6 +49,20 @@ static inline bool aligned(const void *p, size_t a) { return (reinterpret_cast<u
 
 int num_sms();  // cached per device
 
+// Before a launch of `k` with `dynamic` bytes of dynamic shared memory: a block
+// past 48 KB needs the kernel's limit raised, and the kernel's static arrays
+// count towards those 48 KB (1 KB is left for them: STATIC_ROOM bounds what a
+// caller of this declares).  The limit goes to `most`, the largest that any
+// launch of `k` takes, never to this call's size: host threads share it, and one
+// that lowered it between another's two calls would have that launch refused.
+constexpr size_t STATIC_ROOM = 1024;
+template <typename K>
+static inline int allow_smem(K k, size_t dynamic, size_t most) {
+    if (dynamic + STATIC_ROOM > 48 * 1024)
+        ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    return ACT_OK;
+}
+
 // ---------------------------------------------------------------- bf16 bits
 __device__ __forceinline__ float bf2f(uint16_t h) { return __uint_as_float(((uint32_t)h) << 16); }
 __device__ __forceinline__ uint16_t f2bf(float f) {

@@ -25,6 +25,10 @@ namespace mx4 {
 constexpr int MAX_TOKENS = ACTCOMP_MX4_LINEAR_TOKENS;
 constexpr int MAX_X_BYTES = ACTCOMP_MX4_LINEAR_BYTES;  // shared memory for x
 constexpr int DEPTH = 2, STAGE = 5 * 512;  // a warp's stages: four rows' pieces of 512 bytes and the scale words
+constexpr int MAX_SMEM = MAX_X_BYTES + 8 * DEPTH * STAGE;
+static_assert(MAX_X_BYTES % 16 == 0 && 8 * 4 * MAX_TOKENS * sizeof(float) <= STATIC_ROOM &&
+                  MAX_SMEM + STATIC_ROOM <= 227 * 1024,
+              "shared memory");
 
 struct LinArgs {
     const void *x;
@@ -235,8 +239,7 @@ extern "C" int actcomp_mx4_linear(const void *x, int64_t tokens, int64_t cols, i
     return by_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
         auto go = [&](auto kern) -> int {
-            if (smem > 48 * 1024)
-                ACT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            if (int rc = allow_smem(kern, (size_t)smem, MAX_SMEM)) return rc;
             kern<<<grid, 256, (int)smem, st>>>(a);
             return launch_status();
         };
