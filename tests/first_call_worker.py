@@ -35,9 +35,23 @@ def linear():
                 yield f"linear {tokens} x {k} {dtype}", call
 
 
+def norm():
+    """Row lengths whose ring is just under 48 KB."""
+    import test_norm_ops as T
+
+    for dtype in T.DTYPES:
+        for cols in ((3050,) if dtype == torch.float32 else (6104, 6100)):
+            yield f"forward {cols} {dtype}", lambda: T.test_layer_norm_forward(dtype, 3, cols)
+        if dtype == torch.float32:
+            continue
+        for cols in (3048, 3045):
+            yield f"branch forward {cols} {dtype}", lambda: T.test_branch_forward(dtype, 3, cols)
+            yield f"backward {cols} {dtype}", lambda: T.check_backward(dtype, 5, cols, wide=False, fused=False)
+
+
 def main(group):
     failed = 0
-    for name, call in {"linear": linear}[group]():
+    for name, call in {"linear": linear, "norm": norm}[group]():
         try:
             call()
         except Exception as e:

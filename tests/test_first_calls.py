@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-@pytest.mark.parametrize("group", ["linear"])
+@pytest.mark.parametrize("group", ["linear", "norm"])
 def test_first_call_of_each_kernel(group):
     r = subprocess.run([sys.executable, os.path.join(HERE, "first_call_worker.py"), group], capture_output=True,
                        text=True, timeout=600)

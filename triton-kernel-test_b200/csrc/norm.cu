@@ -316,6 +316,8 @@ __host__ __device__ constexpr int fwd_ctas(int nch, int maxt) { return maxt > 25
 __host__ __device__ constexpr int bwd_ctas(int maxt) { return maxt > 320 ? 1 : 2; }
 constexpr int MAX_DEPTH = 4;
 constexpr int RING_HEAD = 8 * MAX_DEPTH * 8 + 16;  // barriers of up to eight warps' rings, the abort word
+constexpr int MAX_SMEM = RING_HEAD + SLOT_ROOM;
+static_assert(MAX_SMEM + STATIC_ROOM <= 227 * 1024, "shared memory");  // the reductions' arrays: 256 bytes at most
 // Bytes of a row in a slot.
 __host__ __device__ __forceinline__ uint32_t row_pitch(int64_t cols, int esize, bool vec) {
     return (uint32_t)(vec ? cols * esize : (cols * esize + 15) / 16 * 16);
@@ -996,8 +998,7 @@ static int fwd_launch(const FwdArgs<T, W> &a, cudaStream_t st) {
     const Shape s = shape_of(a.cols, sizeof(T), DROP, false, VEC);
     const int grid = grid_of(s, a.rows);
     auto go = [&](auto k) -> int {
-        if (s.smem > 48 * 1024)
-            ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem));
+        if (int rc = allow_smem(k, s.smem, MAX_SMEM)) return rc;
         k<<<grid, s.threads, s.smem, st>>>(a, s.wpr, s.depth);
         return launch_status();
     };
@@ -1015,7 +1016,7 @@ static int fwd_launch(const FwdArgs<T, W> &a, cudaStream_t st) {
 template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP, bool MULTI>
 static int bwd_main(const BwdArgs<T, W> &a, const Shape &s, int grid, cudaStream_t st) {
     auto k = ln_bwd_kernel<T, W, NCH, MAXT, VEC, DROP, MULTI>;
-    if (s.smem > 48 * 1024) ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem));
+    if (int rc = allow_smem(k, s.smem, MAX_SMEM)) return rc;
     k<<<grid, s.threads, s.smem, st>>>(a, s.wpr, s.depth);
     return launch_status();
 }
