@@ -915,9 +915,10 @@ __global__ void __launch_bounds__(256) ln_bwd_finish_kernel(const float *part, i
 }
 
 // ---------------------------------------------------------------- launches
-// Segments per thread, warps per row, ring slots and the kernel's shared memory.
+// Segments per thread, warps per row, the template's thread bound (backward), ring
+// slots, the kernel's shared memory and the resident CTAs that its template allows.
 struct Shape {
-    int nch, wpr, threads, rows_per_cta, depth, smem, per_sm;
+    int nch, wpr, threads, maxt, rows_per_cta, depth, smem, per_sm;
 };
 static Shape shape_of(int64_t cols, int esize, bool drop, bool bwd, bool vec) {
     const int segs = (int)((cols + SEG - 1) / SEG);
@@ -928,8 +929,9 @@ static Shape shape_of(int64_t cols, int esize, bool drop, bool bwd, bool vec) {
         s.wpr = (segs + s.nch - 1) / s.nch;
         s.rows_per_cta = s.wpr <= 4 ? 8 / s.wpr : 1;  // two or more
         s.threads = 32 * s.wpr * s.rows_per_cta;
+        s.maxt = s.nch == 4 ? 512 : s.threads <= 256 ? 256 : s.threads <= 320 && esize == 2 ? 320 : 512;
     } else if (segs <= 4) {
-        s = {segs <= 1 ? 1 : (segs <= 2 ? 2 : 4), 1, 256, 8, 0, 0, 0};
+        s = {segs <= 1 ? 1 : (segs <= 2 ? 2 : 4), 1, 256, 0, 8, 0, 0, 0};
     } else {
         // Fewer, fuller warps spend less on a row's reductions: 16384 x 4096 bf16
         // in 52 us with four segments a thread, 56 with two, 86 with one; the
@@ -942,12 +944,20 @@ static Shape shape_of(int64_t cols, int esize, bool drop, bool bwd, bool vec) {
     }
     const int inputs = (bwd ? 2 : 1) + (drop ? 1 : 0);
     const int64_t slot = (int64_t)row_pitch(cols, esize, vec) * inputs * s.rows_per_cta;
-    s.per_sm = bwd ? (esize == 4 && s.threads > 256 ? 1 : bwd_ctas(s.threads)) : fwd_ctas(s.nch, s.threads) * (s.threads <= 128 ? 2 : 1);
+    s.per_sm = bwd ? bwd_ctas(s.maxt) : fwd_ctas(s.nch, s.threads) * (s.threads <= 128 ? 2 : 1);
     const int64_t room = SLOT_ROOM / s.per_sm;
     s.depth = (int)(room / slot < MAX_DEPTH ? room / slot : MAX_DEPTH);
     if (s.depth < 2) {  // the longest rows: one CTA per SM
         s.per_sm = 1;
         s.depth = (int)(SLOT_ROOM / slot < MAX_DEPTH ? SLOT_ROOM / slot : MAX_DEPTH);
+    }
+    // Four segments a thread read the weights again from L1, and the slots take L1's
+    // room: 8192 rows, us with four (what fits) | three | two slots: bf16 9216 137 |
+    // 133 | 140, with dropout 245 | 221 | 219; float32 9216 228 (three fit) | 228 |
+    // 188; bf16 ragged 8705 326 | 327 | 315.
+    if (bwd && s.nch == 4) {
+        const int most = vec && esize == 2 && !drop ? 3 : 2;
+        if (s.depth > most) s.depth = most;
     }
     s.smem = RING_HEAD + (int)(s.depth * slot);
     if (bwd && s.rows_per_cta > 1) {
@@ -1040,8 +1050,8 @@ static int bwd_launch(BwdArgs<T, W> a, W *dw, W *db, void *ws, cudaStream_t st) 
         rc = s.nch == 1           ? bwd_main<T, W, 1, 256, VEC, DROP, true>(a, s, parts, st)
              : s.nch == 4         ? bwd_main<T, W, 4, 512, VEC, DROP, false>(a, s, parts, st)
              : multi              ? bwd_main<T, W, 2, 256, VEC, DROP, true>(a, s, parts, st)
-             : s.threads <= 256   ? bwd_main<T, W, 2, 256, VEC, DROP, false>(a, s, parts, st)
-             : s.per_sm == 2      ? bwd_main<T, W, 2, 320, VEC, DROP, false>(a, s, parts, st)
+             : s.maxt == 256      ? bwd_main<T, W, 2, 256, VEC, DROP, false>(a, s, parts, st)
+             : s.maxt == 320      ? bwd_main<T, W, 2, 320, VEC, DROP, false>(a, s, parts, st)
                                   : bwd_main<T, W, 2, 512, VEC, DROP, false>(a, s, parts, st);
     }
     if (rc || !a.part) return rc;
