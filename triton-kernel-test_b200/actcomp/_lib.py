@@ -164,6 +164,10 @@ SIGNATURES = {
     "actcomp_mx4_gemm": (ctypes.c_int, [ctypes.POINTER(Mx4Desc), ctypes.POINTER(Mx4Desc), c_vp, c_i64, c_i32, c_vp]),
 }
 
+#: entry points behind :class:`Host`, bound on its first use: another build of the
+#: library may lack them, the rest of the package does not need them
+_HOST_API = ("actcomp_dropout", "actcomp_layer_norm", "actcomp_mx4_")
+
 _lock = threading.Lock()
 _lib = None
 
@@ -184,6 +188,8 @@ def load() -> ctypes.CDLL:
                     "(nvcc, sm_100a). actcomp has no CPU fallback.")
         lib = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in SIGNATURES.items():
+            if name.startswith(_HOST_API) and not hasattr(lib, name):
+                continue
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
@@ -205,18 +211,43 @@ def check(fn: str, status: int) -> None:
         raise ActcompError(fn, status)
 
 
-def host():
+class Host:
     """The extension module that runs the host side of :mod:`actcomp.norm` and
-    :mod:`actcomp.mx4` (csrc/host.cpp), bound to the loaded library."""
-    lib = load()
-    path = os.path.join(_HERE, "_host.so")
-    if not os.path.exists(path):
-        raise ImportError(f"{path} is missing: build it with `python triton-kernel-test_b200/actcomp/build.py`")
-    from . import _host
+    :mod:`actcomp.mx4` (csrc/host.cpp), loaded and bound to the library by the
+    first call of one of its functions: nothing else of the package needs it."""
 
-    _host.bind({name: ctypes.cast(getattr(lib, name), c_vp).value for name in SIGNATURES
-                if name.startswith(("actcomp_dropout", "actcomp_layer_norm", "actcomp_mx4_"))})
-    return _host
+    _guard = threading.Lock()
+
+    def __getattr__(self, name):  # reached until _load has put the functions here
+        with Host._guard:
+            if "bind" not in self.__dict__:
+                self._load()
+        return object.__getattribute__(self, name)
+
+    def _load(self) -> None:
+        from importlib import util
+
+        from . import build
+
+        lib = load()
+        path = build.host_path()
+        if not os.path.exists(path):
+            if os.environ.get("ACTCOMP_AUTOBUILD") != "1":
+                raise ImportError(f"{path} is missing: build it with `python triton-kernel-test_b200/actcomp/build.py` "
+                                  "(a module for another torch or Python does not serve)")
+            build.build_host()
+        names = [n for n in SIGNATURES if n.startswith(_HOST_API)]
+        missing = [n for n in names if not hasattr(lib, n)]
+        if missing:
+            raise ImportError(f"{LIB_PATH} lacks {', '.join(missing)}")
+        spec = util.spec_from_file_location(__package__ + "._host", path)
+        module = util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind({n: ctypes.cast(getattr(lib, n), c_vp).value for n in names})
+        self.__dict__.update({k: v for k, v in vars(module).items() if not k.startswith("__")})
+
+
+host = Host()
 
 
 def call(name: str, *args) -> None:

@@ -23,8 +23,6 @@ LIB = os.path.join(PKG, "libactcomp.so")
 # the bounds-checked build (-DACT_BOUNDS_CHECK): device-side index checks that
 # record a bit in the device error word instead of trapping; tests only
 LIB_BC = os.path.join(PKG, "libactcomp_bc.so")
-# the host side of actcomp.norm and actcomp.mx4 (csrc/host.cpp), a Python extension module
-HOST = os.path.join(PKG, "_host.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -60,28 +58,39 @@ def stale(lib: str = LIB) -> bool:
     return any(os.path.getmtime(p) > t for p in _deps())
 
 
-def build_host(force: bool = False) -> str:
-    """Compile (if stale) csrc/host.cpp against torch's headers and return the
-    path of _host.so."""
+def host_path() -> str:
+    """The extension module of the host side of actcomp.norm and actcomp.mx4
+    (csrc/host.cpp).  It is compiled against one torch and one Python and named
+    after both, so that one built for others is never loaded or taken as up to date."""
     import sysconfig
 
-    src = os.path.join(CSRC, "host.cpp")
+    import torch
+
+    return os.path.join(PKG, f"_host-torch{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
+def build_host(force: bool = False) -> str:
+    """Compile (if stale) csrc/host.cpp against torch's headers and return the
+    module's path."""
+    import sysconfig
+
+    src, out = os.path.join(CSRC, "host.cpp"), host_path()
     deps = [src, os.path.join(os.path.dirname(ROOT), "include", "actcomp.h")]
-    if not force and os.path.exists(HOST) and all(os.path.getmtime(p) <= os.path.getmtime(HOST) for p in deps):
-        return HOST
+    if not force and os.path.exists(out) and all(os.path.getmtime(p) <= os.path.getmtime(out) for p in deps):
+        return out
     import torch
 
     base = os.path.dirname(torch.__file__)
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
     inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], cuda]
-    tmp = HOST + ".tmp"
+    tmp = out + ".tmp"
     subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", src, "-o", tmp,
                     *[f"-I{i}" for i in inc], f"-L{os.path.join(base, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
                     "-ltorch", "-ltorch_python", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"],
                    check=True)
-    os.replace(tmp, HOST)
-    return HOST
+    os.replace(tmp, out)
+    return out
 
 
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None, bounds_check: bool = False) -> str:

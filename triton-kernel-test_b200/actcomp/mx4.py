@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 
-_host = _lib.host()
+_host = _lib.host
 
 
 @dataclass

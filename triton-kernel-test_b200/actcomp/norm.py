@@ -28,7 +28,7 @@ import torch
 
 from . import _lib
 
-_host = _lib.host()
+_host = _lib.host
 Seed = Union[int, torch.Tensor]
 
 

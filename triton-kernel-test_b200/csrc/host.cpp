@@ -1,9 +1,9 @@
 // host.cpp -- the host side of actcomp.norm and actcomp.mx4: argument checks,
 // output allocation and the call of the C ABI, as a Python extension module
-// (actcomp/_host.so).  It computes nothing.  A call's host time is what a user
-// waits for at small sizes: layer norm of 8 x 4096 is 3 us on the device, and its
-// Python path (three tensors, a dozen attribute reads, ctypes) took 13 us where
-// this takes 8.
+// (built and named by actcomp/build.py).  It computes nothing.  A call's host time
+// is what a user waits for at small sizes: layer norm of 8 x 4096 is 3 us on the
+// device, and its Python path (three tensors, a dozen attribute reads, ctypes) took
+// 13 us where this takes 8.
 //
 // The entry points' addresses come from the library that the package has loaded
 // (bind), so another build of it serves here as well.
