@@ -378,7 +378,9 @@ int actcomp_dropout(const actcomp_drop_args *a, void *stream);
 /* Layer norm of each row: y = (h - mean) * rstd * weight + bias, mean and rstd =
  * 1 / sqrt(var + eps) in float32 (rows each).  res == NULL: h = x.  Otherwise
  * h = res + dropout(x), written to h, and y normalises the unrounded float32 sum.
- * weight / bias may be NULL (1 / 0). */
+ * weight / bias may be NULL (1 / 0).  A device-side wait that gives up (here and in
+ * the backward pass; actcomp_last_device_error) leaves NaN in the rows of its CTA and
+ * in the weight gradients. */
 typedef struct actcomp_ln_args {
     int64_t rows, cols;
     const void *x;
@@ -431,6 +433,12 @@ typedef struct actcomp_ln_bwd_args {
 } actcomp_ln_bwd_args;
 size_t actcomp_layer_norm_bwd_workspace(int64_t rows, int64_t cols);
 int actcomp_layer_norm_bwd(const actcomp_ln_bwd_args *a, void *workspace, size_t workspace_bytes, void *stream);
+/* Failure-detection self-test of the row copies that both layer norm kernels wait
+ * for: one CTA sums each of `rows` (1..1024) rows of 128 floats of x (16-byte
+ * aligned) into out, but brings only the first `brought` of them, with waits cut to
+ * `polls` (1..2^24) polls.  If a row never comes, all the sums of that CTA are NaN
+ * and the device error word records the timeout. */
+int actcomp_selftest_row_waits(const float *x, int32_t rows, int32_t brought, uint32_t polls, float *out, void *stream);
 
 /* ========================================================= microscaled 4-bit
  * A rows x cols matrix in 4-bit floating point with one power-of-two scale per
@@ -463,7 +471,8 @@ int actcomp_mx4_quantize(const void *x, int64_t rows, int64_t cols, int64_t ldx,
 /* The values of q as rows x cols of `dtype` (row stride ldo). */
 int actcomp_mx4_dequantize(const actcomp_mx4 *q, void *out, int64_t ldo, int32_t dtype, void *stream);
 /* c = a . b^T (a->rows x b->rows, row stride ldc), a->cols == b->cols, float32
- * accumulation on the tensor cores; c_dtype 0 = float32, 1 = bf16, 2 = fp16. */
+ * accumulation on the tensor cores; c_dtype 0 = float32, 1 = bf16, 2 = fp16.  Where a
+ * device-side wait gives up (actcomp_last_device_error) parts of c stay unwritten. */
 int actcomp_mx4_gemm(const actcomp_mx4 *a, const actcomp_mx4 *b, void *c, int64_t ldc, int32_t c_dtype, void *stream);
 
 /* c = x . w^T (tokens x w->rows) for up to ACTCOMP_MX4_LINEAR_TOKENS tokens in one

@@ -154,6 +154,7 @@ SIGNATURES = {
     "actcomp_layer_norm": (ctypes.c_int, [ctypes.POINTER(LnArgs), c_vp]),
     "actcomp_layer_norm_bwd_workspace": (ctypes.c_size_t, [c_i64, c_i64]),
     "actcomp_layer_norm_bwd": (ctypes.c_int, [ctypes.POINTER(LnBwdArgs), c_vp, ctypes.c_size_t, c_vp]),
+    "actcomp_selftest_row_waits": (ctypes.c_int, [c_vp, c_i32, c_i32, ctypes.c_uint32, c_vp, c_vp]),
     "actcomp_mx4_code_bytes": (ctypes.c_size_t, [c_i64, c_i64]),
     "actcomp_mx4_scale_bytes": (ctypes.c_size_t, [c_i64, c_i64]),
     "actcomp_mx4_quantize": (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_i32, ctypes.POINTER(Mx4Desc),
@@ -164,9 +165,10 @@ SIGNATURES = {
     "actcomp_mx4_gemm": (ctypes.c_int, [ctypes.POINTER(Mx4Desc), ctypes.POINTER(Mx4Desc), c_vp, c_i64, c_i32, c_vp]),
 }
 
-#: entry points behind :class:`Host`, bound on its first use: another build of the
-#: library may lack them, the rest of the package does not need them
+#: entry points behind :class:`Host`, bound on its first use
 _HOST_API = ("actcomp_dropout", "actcomp_layer_norm", "actcomp_mx4_")
+#: what another build of the library may lack: the rest of the package does not need them
+_OPTIONAL = _HOST_API + ("actcomp_selftest_row_waits",)
 
 _lock = threading.Lock()
 _lib = None
@@ -188,7 +190,7 @@ def load() -> ctypes.CDLL:
                     "(nvcc, sm_100a). actcomp has no CPU fallback.")
         lib = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in SIGNATURES.items():
-            if name.startswith(_HOST_API) and not hasattr(lib, name):
+            if name.startswith(_OPTIONAL) and not hasattr(lib, name):
                 continue
             fn = getattr(lib, name)
             fn.restype = res

@@ -17,6 +17,10 @@ low_rank_system_profile_backward.py:14-18, forward and both gradients):
 A product contracts over the dimension its operands are blocked along, so a
 gradient needs the other direction's blocks: wt is the quantised transpose, and
 the weight gradient contracts dy and x over tokens, both quantised by columns.
+
+Waits inside the product are bounded.  One that gives up leaves parts of the
+result unwritten and is recorded in the device error word, which
+``_lib.load().actcomp_last_device_error`` reads (ACT_E_TIMEOUT).
 """
 from __future__ import annotations
 

@@ -19,7 +19,12 @@ row, column) alone: a rank that holds rows from ``row_offset`` on draws its part
 of the whole batch's mask.  ``seed`` is an int in [0, 2^64) or a one-element
 int64 CUDA tensor that the kernel reads (so that a captured graph can draw new
 masks); ``p`` is held to 16 bits (``round(p * 65536) / 65536``) and the scale
-uses the held value."""
+uses the held value.
+
+Waits inside the layer norm kernels are bounded.  One that gives up leaves NaN in
+the rows that its part of the device had and in the weight gradients, and is
+recorded in the device error word, which
+``_lib.load().actcomp_last_device_error`` reads (ACT_E_TIMEOUT)."""
 from __future__ import annotations
 
 from typing import Optional, Union

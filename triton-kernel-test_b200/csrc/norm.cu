@@ -318,6 +318,15 @@ constexpr int MAX_DEPTH = 4;
 constexpr int RING_HEAD = 8 * MAX_DEPTH * 8 + 16;  // barriers of up to eight warps' rings, the abort word
 constexpr int MAX_SMEM = RING_HEAD + SLOT_ROOM;
 static_assert(MAX_SMEM + STATIC_ROOM <= 227 * 1024, "shared memory");  // the reductions' arrays: 256 bytes at most
+// NaN in rows r0, r0 + step, ... of p, by the `nt` threads of which this is `t`.
+template <typename T>
+__device__ __forceinline__ void nan_rows(T *p, int64_t ld, int64_t r0, int64_t step, int64_t rows, int64_t cols, int t,
+                                         int nt) {
+#pragma unroll 1
+    for (int64_t r = r0; r < rows; r += step)
+#pragma unroll 1
+        for (int64_t c = t; c < cols; c += nt) p[r * ld + c] = from_f<T>(__uint_as_float(0x7fc00000u));
+}
 // Bytes of a row in a slot.
 __host__ __device__ __forceinline__ uint32_t row_pitch(int64_t cols, int esize, bool vec) {
     return (uint32_t)(vec ? cols * esize : (cols * esize + 15) / 16 * 16);
@@ -337,6 +346,11 @@ struct RowView {
 // passed the barrier that follows its last read.  A bulk copy takes whole
 // 16-byte pieces: of a row that is not aligned so (VEC false) the pieces inside
 // it, which leaves up to seven 16-bit values at either end to plain loads.
+// Waits are bounded.  One that gives up sets the device error word and the CTA's
+// abort word: no slot is filled again, and after its last row a CTA that sees the
+// word writes NaN over all its results (fwd_nan, bwd_nan: calls at the kernels' ends,
+// so that the rows' own registers stay as they were; a test of each wait's outcome in
+// the rows' code cost up to 17 %, this 0 to 3, on some ragged forms up to 6).
 template <typename T, int INPUTS, bool VEC>
 struct RowRing {
     uint8_t *slots;
@@ -391,9 +405,19 @@ struct RowRing {
         }
     }
     // `ahead` (0 or 1): the row after the current one
-    __device__ __forceinline__ void wait(uint8_t *dyn, int ahead = 0) {
+    __device__ __forceinline__ bool wait(uint8_t *dyn, int ahead = 0, uint32_t polls = 1u << 24) {
         const bool wrap = slot + ahead >= depth;
-        tc::mbar_wait(&bars[wrap ? 0 : slot + ahead], phase ^ (wrap ? 1u : 0u), abort_word(dyn));
+        return tc::mbar_wait(&bars[wrap ? 0 : slot + ahead], phase ^ (wrap ? 1u : 0u), abort_word(dyn), polls);
+    }
+    // After the last row, past a barrier of the warps that share it: whether a wait
+    // has given up.  Copies still under way are then waited for, again with a limit
+    // (a barrier's older phase reads as complete, so both parities are asked for).
+    __device__ __forceinline__ bool gave_up(uint8_t *dyn) const {
+        if (!*abort_word(dyn)) return false;
+        for (int i = 0; i < 2 * depth; ++i)
+            for (uint32_t k = 0; k < (1u << 12) && !tc::mbar_try_wait(&bars[i >> 1], i & 1); ++k) {
+            }
+        return true;
     }
     __device__ __forceinline__ RowView<T> view(int k, const T *row, int ahead = 0) const {
         const int s = slot + ahead >= depth ? 0 : slot + ahead;
@@ -406,6 +430,22 @@ struct RowRing {
     }
     __device__ __forceinline__ void next() {
         if (++slot == depth) slot = 0, phase ^= 1;
+    }
+};
+
+// A group's rows and this thread's place in it, found again from the launch (opaque
+// to the compiler: carried along the row loop they cost its registers).
+struct Place {
+    int64_t r0, step;
+    int t, nt;
+    __device__ __forceinline__ explicit Place(int wpr) {
+        int tid, cta;
+        asm volatile("mov.u32 %0, %%tid.x;\n mov.u32 %1, %%ctaid.x;" : "=r"(tid), "=r"(cta));
+        nt = 32 * wpr;
+        const int groups = (int)blockDim.x / nt, mine = tid / nt;
+        t = tid - mine * nt;
+        r0 = (int64_t)cta * groups + mine;
+        step = (int64_t)gridDim.x * groups;
     }
 };
 
@@ -432,10 +472,21 @@ __device__ __forceinline__ Raw8<T> load8(const RowView<T> &row, int seg0, int co
     }
 }
 
+// NaN over a forward CTA's results (see RowRing).
+template <typename T, typename W>
+__device__ __noinline__ void fwd_nan(const FwdArgs<T, W> &a, int wpr) {
+    const Place p(wpr);
+    nan_rows(a.y, a.ldy, p.r0, p.step, a.rows, a.cols, p.t, p.nt);
+    if (a.res) nan_rows(a.h, a.ldh, p.r0, p.step, a.rows, a.cols, p.t, p.nt);
+    nan_rows(a.mean, 1, p.r0, p.step, a.rows, 1, p.t, p.nt);
+    nan_rows(a.rstd, 1, p.r0, p.step, a.rows, 1, p.t, p.nt);
+}
+
 // MAXT: the launch's thread count rounded up to 256, 320 or 512.
 // ONE: a warp per row, else a CTA.
 template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP, bool ONE>
-__global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdArgs<T, W> a, int warps, int depth) {
+__global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT))
+    ln_fwd_kernel(const __grid_constant__ FwdArgs<T, W> a, int warps, int depth) {
     const int wpr = ONE ? 1 : warps;  // warps per row
     extern __shared__ __align__(128) uint8_t dyn[];
     constexpr int NW = MAXT / 32;
@@ -499,12 +550,13 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdAr
             }
             s[k] = t.x + t.y;
         }
+        const bool go = leader && !*ring.abort_word(dyn);  // no wait has given up
         row_sums<NW, R, ONE>(s, red[0], warp, lane);
         // every reader of the slots is past its reads
         if (ONE) __syncwarp();
 #pragma unroll
         for (int k = 0; k < R; ++k) {
-            if (leader) fill(ring.slot, r + (depth + k) * step);
+            if (go) fill(ring.slot, r + (depth + k) * step);
             ring.next();
         }
         float mean[R], q[R];
@@ -550,6 +602,7 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(NCH, MAXT)) ln_fwd_kernel(FwdAr
             }
         }
     }
+    if (ring.gave_up(dyn)) fwd_nan<T, W>(a, ONE ? 1 : blockDim.x >> 5);
 }
 
 // Rows longer than MAX_SEGS segments: one CTA per row, three passes over it
@@ -651,9 +704,20 @@ __device__ __forceinline__ float2 row_sum2(float u, float v, float2 *red, int wp
     return s;
 }
 
+// NaN over a backward CTA's results, its part of the weight gradients' sums among them.
+template <typename T, typename W>
+__device__ __noinline__ void bwd_nan(const BwdArgs<T, W> &a, int wpr) {
+    const Place p(wpr);
+    nan_rows(a.dx, a.lddx, p.r0, p.step, a.rows, a.cols, p.t, p.nt);
+    if (a.dr) nan_rows(a.dr, a.lddr, p.r0, p.step, a.rows, a.cols, p.t, p.nt);
+    if (a.part)
+        nan_rows(a.part, 2 * a.cols, blockIdx.x, gridDim.x, gridDim.x, 2 * a.cols, threadIdx.x, blockDim.x);
+}
+
 // MULTI: a CTA has several rows in hand, each a group of `wpr` warps; else one.
 template <typename T, typename W, int NCH, int MAXT, bool VEC, bool DROP, bool MULTI>
-__global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T, W> a, int wpr, int depth) {
+__global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT))
+    ln_bwd_kernel(const __grid_constant__ BwdArgs<T, W> a, int wpr, int depth) {
     constexpr int NW = MAXT / 32;
     __shared__ __align__(16) float2 red[2][NW];
     if (threadIdx.x < 2 * NW) red[0][threadIdx.x] = make_float2(0.f, 0.f);
@@ -666,7 +730,7 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
     const uint64_t key = DROP ? drop_seed(a.d) : 0;
     constexpr int IN = DROP ? 3 : 2;
     RowRing<T, IN, VEC> ring;
-    const bool leader = w0 == 0 && lane == 0;
+    bool leader = w0 == 0 && lane == 0;
     const int64_t r0 = (int64_t)blockIdx.x * rpc + mine, step = (int64_t)gridDim.x * rpc;
     auto fill = [&](int s, int64_t row) {
         if (row >= a.rows) return;
@@ -697,16 +761,20 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
 #pragma unroll
         for (int j = 0; j < 4; ++j) dw[i].p[j] = db[i].p[j] = make_float2(0.f, 0.f);
     }
+    // How the leader knows that a slot must not be filled again: by its own waits or by
+    // the abort word.  8192 rows bf16, us: 9216 values 132 and 147, 5120 61 and 58.
+    constexpr bool OWN_WAIT = NCH == 4 && VEC;
     int turn = 0;
     float mean = r0 < a.rows ? a.mean[r0] : 0.f, rstd = r0 < a.rows ? a.rstd[r0] : 0.f;
     for (int64_t r = r0; r < a.rows; r += step, ++turn) {
+        const bool go = leader && turn > 0 && (OWN_WAIT || !*ring.abort_word(dyn));
         const float2 mean2 = make_float2(mean, mean), rstd2 = make_float2(rstd, rstd);
         const float rs = rstd;
         if (r + step < a.rows) mean = a.mean[r + step], rstd = a.rstd[r + step];
         const RowView<T> yr = ring.view(0, a.dy + r * a.lddy), xr = ring.view(1, a.x + r * a.ldx);
         float2 s1 = make_float2(0.f, 0.f), s2 = s1;
         F8 gh[HOLD ? NCH : 1], xh[HOLD ? NCH : 1];
-        ring.wait(dyn);
+        if (!ring.wait(dyn) && OWN_WAIT) leader = false;
         auto weights = [&](int i) {
             if constexpr (WREG) {
                 stay_packed(wv[i]);
@@ -740,7 +808,8 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
         const float2 s = row_sum2<NW, MULTI>(s1.x + s1.y, s2.x + s2.y, red[turn & 1], wpr, mine, w0, lane);
         // the row before this one has been read by all
         if (MULTI && wpr == 1) __syncwarp();
-        if (leader && turn > 0) fill(ring.slot == 0 ? depth - 1 : ring.slot - 1, r + (depth - 1) * step);
+        if (OWN_WAIT ? leader && turn > 0 : go)
+            fill(ring.slot == 0 ? depth - 1 : ring.slot - 1, r + (depth - 1) * step);
         // dx = rstd g - rstd mean(g) - x-hat rstd mean(g x-hat)
         const float c1 = -rs * (s.x * inv_n), c2 = -rs * (s.y * inv_n);
         const float2 c1_2 = make_float2(c1, c1), c2_2 = make_float2(c2, c2);
@@ -772,31 +841,35 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) ln_bwd_kernel(BwdArgs<T,
         }
         ring.next();
     }
-    if (!a.part) return;
-    float *part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
-    if constexpr (MULTI) {
-        // the groups' sums, over the rings' space once every warp is done with it
-        __syncthreads();
-        float *acc = reinterpret_cast<float *>(dyn + RING_HEAD), *own = acc + (int64_t)mine * 2 * a.cols;
+    if (a.part) {
+        float *part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
+        if constexpr (MULTI) {
+            // the groups' sums, over the rings' space once every warp is done with it
+            __syncthreads();
+            float *acc = reinterpret_cast<float *>(dyn + RING_HEAD), *own = acc + (int64_t)mine * 2 * a.cols;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            store8<float, VEC>(own, (w0 + i * wpr) * SEG, n[i], lane, dw[i]);
-            store8<float, VEC>(own + a.cols, (w0 + i * wpr) * SEG, n[i], lane, db[i]);
-        }
-        __syncthreads();
-        for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) {
-            float s = 0.f;
-            for (int i = 0; i < rpc; ++i) s += acc[(int64_t)i * 2 * a.cols + c];
-            part[c] = s;
-        }
-        return;
-    }
+            for (int i = 0; i < NCH; ++i) {
+                store8<float, VEC>(own, (w0 + i * wpr) * SEG, n[i], lane, dw[i]);
+                store8<float, VEC>(own + a.cols, (w0 + i * wpr) * SEG, n[i], lane, db[i]);
+            }
+            __syncthreads();
+            for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) {
+                float s = 0.f;
+                for (int i = 0; i < rpc; ++i) s += acc[(int64_t)i * 2 * a.cols + c];
+                part[c] = s;
+            }
+        } else {
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-        const int seg0 = (w0 + i * wpr) * SEG;
-        store8<float, VEC>(part, seg0, n[i], lane, dw[i]);
-        store8<float, VEC>(part + a.cols, seg0, n[i], lane, db[i]);
+            for (int i = 0; i < NCH; ++i) {
+                const int seg0 = (w0 + i * wpr) * SEG;
+                store8<float, VEC>(part, seg0, n[i], lane, dw[i]);
+                store8<float, VEC>(part + a.cols, seg0, n[i], lane, db[i]);
+            }
+        }
     }
+    __syncthreads();
+    // the same for all: every wait of the CTA lies before this barrier
+    if (ring.gave_up(dyn)) bwd_nan<T, W>(a, MULTI ? wpr : blockDim.x >> 5);
 }
 
 // Rows longer than MAX_SEGS segments, first kernel: the row's two sums.
@@ -912,6 +985,38 @@ __global__ void __launch_bounds__(256) ln_bwd_finish_kernel(const float *part, i
             db[c - cols] = from_f<W>(s);
         }
     }
+}
+
+// Self-test of the ring's waits: a warp takes `rows` rows of 4 * 32 values of which
+// only the first `brought` are copied, with waits cut to `polls` polls, and writes
+// their sums as the kernels above write their results.
+__global__ void __launch_bounds__(32) selftest_ring_kernel(const float *x, int rows, int brought, uint32_t polls,
+                                                           float *out) {
+    __shared__ __align__(128) uint8_t dyn[RING_HEAD + 2 * 128 * 4];
+    RowRing<float, 1, true> ring;
+    const int lane = threadIdx.x & 31;
+    auto fill = [&](int s, int row) {
+        if (row >= brought || *ring.abort_word(dyn)) return;
+        const float *src[1] = {x + row * 128};
+        ring.fill(s, src);
+    };
+    ring.init(dyn, 0, 128, 2, lane == 0);
+    if (lane == 0)
+        for (int i = 0; i < 2; ++i) fill(i, i);
+    for (int r = 0; r < rows; ++r) {
+        ring.wait(dyn, 0, polls);
+        const float4 v = reinterpret_cast<const float4 *>(ring.view(0, x + r * 128).s)[lane];
+        const float s = warp_sum(v.x + v.y + v.z + v.w);
+        __syncwarp();
+        if (lane == 0) {
+            out[r] = s;
+            fill(ring.slot, r + 2);
+        }
+        ring.next();
+    }
+    __syncwarp();
+    if (ring.gave_up(dyn))
+        for (int r = lane; r < rows; r += 32) out[r] = __uint_as_float(0x7fc00000u);
 }
 
 // ---------------------------------------------------------------- launches
@@ -1214,4 +1319,15 @@ extern "C" int actcomp_layer_norm_bwd(const actcomp_ln_bwd_args *g, void *worksp
         return vec ? bwd_launch<T, W, true, false>(a, dw, db, workspace, st)
                    : bwd_launch<T, W, false, false>(a, dw, db, workspace, st);
     });
+}
+
+extern "C" int actcomp_selftest_row_waits(const float *x, int32_t rows, int32_t brought, uint32_t polls, float *out,
+                                          void *stream) {
+    using namespace act;
+    using namespace act::norm;
+    ACT_CHECK(x && out && rows >= 1 && rows <= 1024 && brought >= 0 && brought <= rows, ACT_E_INVALID);
+    ACT_CHECK(polls >= 1 && polls <= (1u << 24), ACT_E_INVALID);
+    ACT_CHECK(aligned(x, 16) && aligned(out, 4), ACT_E_ALIGN);
+    selftest_ring_kernel<<<1, 32, 0, as_stream(stream)>>>(x, rows, brought, polls, out);
+    return launch_status();
 }
