@@ -67,16 +67,20 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Opti
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
-                        rstd: torch.Tensor, bias_grad: bool = True):
+                        rstd: torch.Tensor, bias_grad: bool = True, bias_dtype: Optional[torch.dtype] = None):
     """(dx, dweight, dbias) of :func:`layer_norm` (dweight None without a
-    weight, dbias None with bias_grad=False).  The sums over rows run in a fixed
-    order: the same inputs give the same bits."""
-    return _host.layer_norm_backward(dy, x, weight, mean, rstd, bias_grad)
+    weight, dbias None with bias_grad=False), the two sums in the weight's dtype;
+    without a weight dbias is in ``bias_dtype`` (the bias's: the activation's, which
+    is the default, or float32).  They run over the rows in a fixed order: the same
+    inputs give the same bits."""
+    return _host.layer_norm_backward(dy, x, weight, mean, rstd, bias_grad, bias_dtype)
 
 
 def dropout_add_layer_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: Optional[torch.Tensor],
                                     mean: torch.Tensor, rstd: torch.Tensor, p: float, seed: Seed,
-                                    row_offset: int = 0, dh: Optional[torch.Tensor] = None, bias_grad: bool = True):
+                                    row_offset: int = 0, dh: Optional[torch.Tensor] = None, bias_grad: bool = True,
+                                    bias_dtype: Optional[torch.dtype] = None):
     """(dx, dresidual, dweight, dbias) of :func:`dropout_add_layer_norm` from
-    the gradient of y and, if h is used further on, dh, the gradient h gets there."""
-    return _host.branch_backward(dy, h, weight, mean, rstd, p, seed, row_offset, dh, bias_grad)
+    the gradient of y and, if h is used further on, dh, the gradient h gets there.
+    ``bias_grad`` and ``bias_dtype`` as in :func:`layer_norm_backward`."""
+    return _host.branch_backward(dy, h, weight, mean, rstd, p, seed, row_offset, dh, bias_grad, bias_dtype)

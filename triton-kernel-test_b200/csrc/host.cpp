@@ -222,17 +222,25 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> branch(const Tensor &x, const Tensor 
 
 std::tuple<Tensor, OptTensor, OptTensor, OptTensor> backward(const Tensor &dy, const Tensor &x, const OptTensor &weight,
                                                              const Tensor &mean, const Tensor &rstd, const OptTensor &dh,
-                                                             bool fused, bool bias_grad, const Draw &d) {
+                                                             bool fused, bool bias_grad,
+                                                             std::optional<at::ScalarType> bias_dtype, const Draw &d) {
     const int dt = dtype_of(x.scalar_type());
     const Geometry g = geometry(x);
-    const int wdt = affine(x, g.cols, weight, {});
+    // what the weight gradients are in: the weight's dtype, without one the bias's
+    const at::ScalarType wtype = weight ? weight->scalar_type() : bias_dtype.value_or(x.scalar_type());
+    affine(x, g.cols, weight, {});
+    if (wtype != x.scalar_type() && wtype != at::kFloat)
+        bad_type(std::string("bias_dtype must be ") + at::toString(x.scalar_type()) + " or float32, got " +
+                 at::toString(wtype));
+    if (bias_dtype && *bias_dtype != wtype) bad_type("weight and bias must have one dtype");
+    const int wdt = dtype_of(wtype);
     if (g.cols == 0) bad_value("layer norm over an empty last dimension");
     const Tensor m = stats(mean, g.rows, x, "mean"), s = stats(rstd, g.rows, x, "rstd");
     const Rows ry = rows_of(dy, g.cols), rx = rows_of(x, g.cols), rh = dh ? rows_of(*dh, g.cols) : Rows{};
     const OptTensor w = packed(weight);
     const Tensor dx = fresh(x);
     const OptTensor dr = fused ? OptTensor(fresh(x)) : OptTensor();
-    const auto wopt = weight ? weight->options() : x.options();
+    const auto wopt = x.options().dtype(wtype);
     const OptTensor dw = weight ? OptTensor(at::empty({g.cols}, wopt)) : OptTensor();
     const OptTensor db = bias_grad ? OptTensor(at::empty({g.cols}, wopt)) : OptTensor();
     const c10::cuda::CUDAGuard guard(x.device());
@@ -247,10 +255,11 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> backward(const Tensor &dy, c
 }
 
 std::tuple<Tensor, OptTensor, OptTensor> layer_norm_backward(const Tensor &dy, const Tensor &x, const OptTensor &weight,
-                                                             const Tensor &mean, const Tensor &rstd, bool bias_grad) {
+                                                             const Tensor &mean, const Tensor &rstd, bool bias_grad,
+                                                             std::optional<at::ScalarType> bias_dtype) {
     need_cuda(x);
     same(x, dy, "dy");
-    auto [dx, dr, dw, db] = backward(dy, x, weight, mean, rstd, {}, false, bias_grad, Draw{});
+    auto [dx, dr, dw, db] = backward(dy, x, weight, mean, rstd, {}, false, bias_grad, bias_dtype, Draw{});
     return {dx, dw, db};
 }
 
@@ -258,11 +267,13 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> branch_backward(const Tensor &d
                                                                  const OptTensor &weight, const Tensor &mean,
                                                                  const Tensor &rstd, double p, const py::object &seed,
                                                                  const py::object &row_offset, const OptTensor &dh,
-                                                                 bool bias_grad) {
+                                                                 bool bias_grad,
+                                                                 std::optional<at::ScalarType> bias_dtype) {
     need_cuda(h);
     same(h, dy, "dy");
     if (dh) same(h, *dh, "dh");
-    auto [dx, dr, dw, db] = backward(dy, h, weight, mean, rstd, dh, true, bias_grad, draw(h, p, seed, row_offset));
+    auto [dx, dr, dw, db] = backward(dy, h, weight, mean, rstd, dh, true, bias_grad, bias_dtype,
+                                     draw(h, p, seed, row_offset));
     return {dx, *dr, dw, db};
 }
 
