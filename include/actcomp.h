@@ -372,7 +372,8 @@ typedef struct actcomp_drop_args {
     const uint64_t *seed_ptr;
     uint64_t row_offset;
 } actcomp_drop_args;
-/* y = dropout(x); also the backward pass, on the gradient.  y may be x. */
+/* y = dropout(x); also the backward pass, on the gradient.  y may be x with the same
+ * row stride, and may not overlap it otherwise. */
 int actcomp_dropout(const actcomp_drop_args *a, void *stream);
 
 /* Layer norm of each row: y = (h - mean) * rstd * weight + bias, mean and rstd =

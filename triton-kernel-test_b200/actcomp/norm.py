@@ -40,7 +40,8 @@ Seed = Union[int, torch.Tensor]
 def dropout(x: torch.Tensor, p: float, seed: Seed, row_offset: int = 0,
             out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Each value kept with probability 1 - p and scaled by 1 / (1 - p), else 0.
-    ``out`` (contiguous, like x; may be x itself) receives the result."""
+    ``out`` (contiguous, like x; may be x itself) receives the result; where it lies
+    over other parts of x, x is copied first."""
     return _host.dropout(x, p, seed, row_offset, out)
 
 

@@ -175,7 +175,14 @@ Tensor dropout(const Tensor &x, double p, const py::object &seed, const py::obje
         if (!out->is_contiguous()) bad_value("out must be contiguous");
     }
     const Tensor y = out ? *out : fresh(x);
-    const Rows r = rows_of(x, g.cols);
+    Rows r = rows_of(x, g.cols);
+    // out lies over part of x, elsewhere than x's own values: rows would be
+    // overwritten before they are read
+    if (out && x.numel() > 0 && (ptr(r.t) != ptr(y) || r.ld != g.cols)) {
+        const auto xa = reinterpret_cast<uintptr_t>(ptr(r.t)), ya = reinterpret_cast<uintptr_t>(ptr(y));
+        const size_t es = x.element_size(), xn = ((g.rows - 1) * r.ld + g.cols) * es, yn = x.numel() * es;
+        if (xa < ya + yn && ya < xa + xn) r = {x.clone(at::MemoryFormat::Contiguous), g.cols};
+    }
     const actcomp_drop_args a{g.rows, g.cols, ptr(r.t), r.ld, ptr(y), g.cols, dt, 0, d.p, d.seed, d.seed_ptr, d.row_offset};
     const c10::cuda::CUDAGuard guard(x.device());
     check("actcomp_dropout", api.dropout(&a, stream_of(x)));
