@@ -223,7 +223,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (p.tma_out) {
                     tc::fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) {
+                    if (lane == 0 && ACT_DCHECK(row0 < p.M && col < p.N)) {
                         tc::tma_store_3d(&tmC, dst, col, row0, 0);
                         tc::bulk_commit();
                     }
@@ -233,7 +233,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     constexpr int PER = 16 / ES;
                     const int rows = p.M - row0 < 32 ? p.M - row0 : 32;
                     TOut *d = static_cast<TOut *>(p.C) + (int64_t)row0 * p.ldc + col + lane;
-                    if (col + lane < p.N)
+                    if (col + lane < p.N && ACT_DCHECK(col + lane < p.ldc && row0 + rows <= p.M))
                         for (int i = 0; i < rows; ++i, d += p.ldc)
                             *d = *reinterpret_cast<const TOut *>(dst + kmajor_swz<32 * ES>(i, lane / PER) +
                                                                  lane % PER * ES);

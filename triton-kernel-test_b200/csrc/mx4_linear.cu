@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(256, M == 1 ? 4 : (M == 2 ? 3 : 2)) linear_ker
         if (b < nb && row < a.n) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (row + 32 * j < a.n) cp_async16(d + 512 * j, cw + 32 * j * rb + 16 * (int64_t)b);
+                if (row + 32 * j < a.n && ACT_DCHECK(16 * (int64_t)b + 16 <= rb)) cp_async16(d + 512 * j, cw + 32 * j * rb + 16 * (int64_t)b);
             cp_async16(d + 2048, sw + (int64_t)(b >> 2) * ATOM_BYTES);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256, M == 1 ? 4 : (M == 2 ? 3 : 2)) linear_ker
         float t = 0.f;
         for (int i = 0; i < ks; ++i) t += red[warp + i][lane];
         const int j = lane / M, m = lane - j * M, r = row + 32 * j;
-        if (r < a.n) static_cast<TOut *>(a.c)[m * a.ldc + r] = from_f<TOut>(t);
+        if (r < a.n && ACT_DCHECK(r < a.ldc)) static_cast<TOut *>(a.c)[m * a.ldc + r] = from_f<TOut>(t);
     }
 }
 

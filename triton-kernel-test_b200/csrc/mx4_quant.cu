@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256)
             m = max_of<T>(m, __shfl_xor_sync(0xffffffffu, m, 2));
             const uint32_t sc = scale_code(amax_bits<T>(m));
             sc4 |= sc << (8 * j);
-            if (code && r0 + 32 * j < rows) {
+            if (code && r0 + 32 * j < rows && ACT_DCHECK(c / 2 + 4 <= rb)) {
                 const float inv = inv_scale(sc);
                 float v[8];
                 raw[j].floats(v);
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(256)
         // four blocks x four rows of scale bytes (lanes 0 and 16)
         const uint32_t b1 = __shfl_down_sync(0xffffffffu, sc4, 4), b2 = __shfl_down_sync(0xffffffffu, sc4, 8),
                        b3 = __shfl_down_sync(0xffffffffu, sc4, 12);
-        if (word)
+        if (word && ACT_DCHECK(g < groups && ka < nka))
             *reinterpret_cast<uint4 *>(scales + ((int64_t)(g >> 5) * nka + ka) * ATOM_BYTES + (g & 31) * 16) =
                 transpose_bytes(sc4, b1, b2, b3);
     }
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(256, 4)
                 m = max_of<T>(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = max_of<T>(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 const uint32_t sc = scale_code(amax_bits<T>(m));
-                if (r < rows && c < blocks_of(cols) * BLOCK) {
+                if (r < rows && c < blocks_of(cols) * BLOCK && ACT_DCHECK(c / 2 + 4 <= rb)) {
                     const float inv = inv_scale(sc);
                     float v[8];
                     raw[i].floats(v);
@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(256, 4)
                 uint32_t w = sc;
                 w |= __shfl_down_sync(0xffffffffu, w, 4) << 8;
                 w |= __shfl_down_sync(0xffffffffu, w, 8) << 16;
-                if ((lane & 15) == 0) *reinterpret_cast<uint32_t *>(scales + scale_word(r, kc, nka)) = w;
+                if ((lane & 15) == 0 && ACT_DCHECK(kc < nka && r < (rows + 127) / 128 * 128))
+                    *reinterpret_cast<uint32_t *>(scales + scale_word(r, kc, nka)) = w;
             }
         }
     }
@@ -206,11 +207,11 @@ __global__ void __launch_bounds__(256, 4)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int col = 64 * i + (tid >> 2), q = tid & 3;
-        if (c0 + col < cols && r0 + 32 * q < rows)
+        if (c0 + col < cols && r0 + 32 * q < rows && ACT_DCHECK(r0 / 2 + 16 * q + 16 <= rb_t))
             *reinterpret_cast<uint4 *>(codes_t + (c0 + col) * rb_t + r0 / 2 + 16 * q) =
                 *reinterpret_cast<const uint4 *>(out + col * 80 + 16 * q);
     }
-    if (tid < 128)
+    if (tid < 128 && ACT_DCHECK(kr < nka_t && c0 + tid < (cols + 127) / 128 * 128))
         *reinterpret_cast<uint32_t *>(scales_t + scale_word(c0 + tid, kr, nka_t)) = words[tid];
 }
 
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(256)
                 }
             }
             T *row = out + (r0 + 32 * j) * ldo + c0;
-            if (VEC && n == 8) {
+            if (VEC && n == 8 && ACT_DCHECK(c + 8 <= cols && r0 + 32 * j < rows)) {
 #pragma unroll
                 for (int k = 0; k < (int)sizeof(T) / 2; ++k)
                     reinterpret_cast<uint4 *>(row + 8 * lane)[k] =
@@ -287,7 +288,8 @@ __global__ void __launch_bounds__(256)
                 const T *v = reinterpret_cast<const T *>(turn[warp]);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    if (32 * k + lane < left) row[32 * k + lane] = v[32 * k + lane];
+                    if (32 * k + lane < left && ACT_DCHECK(c0 + 32 * k + lane < cols && r0 + 32 * j < rows))
+                        row[32 * k + lane] = v[32 * k + lane];
                 __syncwarp();
             }
         }

@@ -139,8 +139,8 @@ __device__ __forceinline__ void stay_packed(Raw8<T> &r) {
 template <bool VEC>
 __device__ __forceinline__ int count_of(int64_t seg0, int64_t n, int lane) {
     const int64_t left = n - seg0 - (VEC ? 8 * lane : lane);
-    if (VEC) return left > 0 ? 8 : 0;
-    return left <= 0 ? 0 : (left > 224 ? 8 : (int)((left + 31) >> 5));
+    const int count = VEC ? (left > 0 ? 8 : 0) : left <= 0 ? 0 : (left > 224 ? 8 : (int)((left + 31) >> 5));
+    return ACT_DCHECK(count == 0 || (VEC ? 8 : 32 * (count - 1) + 1) <= left) ? count : 0;
 }
 
 // Values outside the row read as `fill`.
