@@ -153,15 +153,25 @@ def _(x, weight, bias, eps):
     return _empty(x.shape, x.dtype, x), _empty(x.shape[:-1], _F32, x), _empty(x.shape[:-1], _F32, x)
 
 
+def _weight_grads(x, weight, bias_dtype):
+    """Fake dweight and dbias; dweight is empty without a weight (a custom op returns no None)."""
+    dt = weight.dtype if weight is not None else bias_dtype or x.dtype
+    return _empty(x.shape[-1:] if weight is not None else (0,), dt, x), _empty(x.shape[-1:], dt, x)
+
+
 @torch.library.custom_op("actcomp::layer_norm_backward", mutates_args=())
-def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor,
-                        rstd: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return norm.layer_norm_backward(dy, x, weight, mean, rstd)
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
+                        rstd: torch.Tensor, bias_dtype: Optional[torch.dtype] = None) -> tuple[torch.Tensor,
+                                                                                               torch.Tensor,
+                                                                                               torch.Tensor]:
+    """norm.layer_norm_backward; without a weight its gradient is an empty tensor."""
+    dx, dw, db = norm.layer_norm_backward(dy, x, weight, mean, rstd, True, bias_dtype)
+    return dx, db.new_empty(0) if dw is None else dw, db
 
 
 @layer_norm_backward.register_fake
-def _(dy, x, weight, mean, rstd):
-    return _empty(x.shape, x.dtype, x), _empty(weight.shape, weight.dtype, x), _empty(weight.shape, weight.dtype, x)
+def _(dy, x, weight, mean, rstd, bias_dtype=None):
+    return (_empty(x.shape, x.dtype, x),) + _weight_grads(x, weight, bias_dtype)
 
 
 @torch.library.custom_op("actcomp::dropout_add_layer_norm", mutates_args=())
@@ -178,17 +188,20 @@ def _(x, residual, weight, bias, p, seed, row_offset, eps):
 
 
 @torch.library.custom_op("actcomp::dropout_add_layer_norm_backward", mutates_args=())
-def dropout_add_layer_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor,
-                                    rstd: torch.Tensor, p: float, seed: torch.Tensor, row_offset: int,
-                                    dh: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor,
-                                                                         torch.Tensor]:
-    return norm.dropout_add_layer_norm_backward(dy, h, weight, mean, rstd, p, seed, row_offset, dh)
+def dropout_add_layer_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: Optional[torch.Tensor],
+                                    mean: torch.Tensor, rstd: torch.Tensor, p: float, seed: torch.Tensor,
+                                    row_offset: int, dh: Optional[torch.Tensor],
+                                    bias_dtype: Optional[torch.dtype] = None) -> tuple[torch.Tensor, torch.Tensor,
+                                                                                       torch.Tensor, torch.Tensor]:
+    """norm.dropout_add_layer_norm_backward; without a weight its gradient is an empty tensor."""
+    dx, dr, dw, db = norm.dropout_add_layer_norm_backward(dy, h, weight, mean, rstd, p, seed, row_offset, dh, True,
+                                                          bias_dtype)
+    return dx, dr, db.new_empty(0) if dw is None else dw, db
 
 
 @dropout_add_layer_norm_backward.register_fake
-def _(dy, h, weight, mean, rstd, p, seed, row_offset, dh):
-    return (_empty(h.shape, h.dtype, h), _empty(h.shape, h.dtype, h), _empty(weight.shape, weight.dtype, h),
-            _empty(weight.shape, weight.dtype, h))
+def _(dy, h, weight, mean, rstd, p, seed, row_offset, dh, bias_dtype=None):
+    return (_empty(h.shape, h.dtype, h), _empty(h.shape, h.dtype, h)) + _weight_grads(h, weight, bias_dtype)
 
 
 # ---------------------------------------------------------------- microscaled 4-bit
