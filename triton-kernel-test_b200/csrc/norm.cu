@@ -1121,7 +1121,9 @@ static int fwd_launch(const FwdArgs<T, W> &a, cudaStream_t st) {
         if (s.nch == 1) return go(ln_fwd_kernel<T, W, 1, 256, VEC, DROP, true>);
         return s.nch == 2 ? go(ln_fwd_kernel<T, W, 2, 256, VEC, DROP, true>) : go(ln_fwd_kernel<T, W, 4, 256, VEC, DROP, true>);
     }
-    if (s.nch == 1) return go(ln_fwd_kernel<T, W, 1, 256, VEC, DROP, false>);
+    if constexpr (DROP || sizeof(T) == 4) {  // see shape_of: the others take two segments
+        if (s.nch == 1) return go(ln_fwd_kernel<T, W, 1, 256, VEC, DROP, false>);
+    }
     if (s.nch == 2) return go(ln_fwd_kernel<T, W, 2, 256, VEC, DROP, false>);
     if (s.nch == 3) return go(ln_fwd_kernel<T, W, 3, 256, VEC, DROP, false>);
     return s.threads <= 256 ? go(ln_fwd_kernel<T, W, 4, 256, VEC, DROP, false>)
@@ -1152,11 +1154,12 @@ static int bwd_launch(BwdArgs<T, W> a, W *dw, W *db, void *ws, cudaStream_t st) 
         const Shape s = shape_of(a.cols, sizeof(T), DROP, true, VEC);
         parts = grid_of(s, a.rows);
         const bool multi = s.rows_per_cta > 1;
+        constexpr int MID = sizeof(T) == 2 ? 320 : 512;  // float32 has no form of 320 threads (shape_of)
         rc = s.nch == 1           ? bwd_main<T, W, 1, 256, VEC, DROP, true>(a, s, parts, st)
              : s.nch == 4         ? bwd_main<T, W, 4, 512, VEC, DROP, false>(a, s, parts, st)
              : multi              ? bwd_main<T, W, 2, 256, VEC, DROP, true>(a, s, parts, st)
              : s.maxt == 256      ? bwd_main<T, W, 2, 256, VEC, DROP, false>(a, s, parts, st)
-             : s.maxt == 320      ? bwd_main<T, W, 2, 320, VEC, DROP, false>(a, s, parts, st)
+             : s.maxt == MID      ? bwd_main<T, W, 2, MID, VEC, DROP, false>(a, s, parts, st)
                                   : bwd_main<T, W, 2, 512, VEC, DROP, false>(a, s, parts, st);
     }
     if (rc || !a.part) return rc;
