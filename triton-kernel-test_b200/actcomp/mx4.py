@@ -88,8 +88,9 @@ def matmul(a: Mx4, b: Mx4, out_dtype: Optional[torch.dtype] = None) -> torch.Ten
 
 def linear(x: torch.Tensor, w: Mx4, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x . w^T for x (..., K) and w (N, K) in 4 bits: x is quantised by rows on
-    the way; (..., N) of ``out_dtype`` (default: x's).  Up to four tokens take one
-    kernel that reads the weight at memory speed, more the tensor cores."""
+    the way; (..., N) of ``out_dtype`` (default: x's).  One token, and up to four on
+    a weight that is not large, take one kernel, the others quantisation and the
+    tensor cores."""
     return _host.linear(x, w.rows, w.cols, w.codes, w.scales, out_dtype)
 
 
@@ -98,7 +99,7 @@ def linear_forward(x: torch.Tensor, w: Mx4, out_dtype: Optional[torch.dtype] = N
     weight gradient needs of it."""
     if x.shape[-1] != w.cols:
         raise ValueError(f"x has {x.shape[-1]} columns, the weight {w.cols}")
-    if x.numel() <= _lib.MX4_LINEAR_TOKENS * w.cols:
+    if _host.one_kernel(x.numel() // w.cols, w.rows, w.cols):
         return linear(x, w, out_dtype), quantize(x, transpose=True)
     q, saved = quantize_pair(x)
     return matmul(q, w, out_dtype).view(x.shape[:-1] + (w.rows,)), saved

@@ -354,7 +354,22 @@ Tensor matmul(int64_t m, int64_t n, int64_t k, const Tensor &a_codes, const Tens
     return product(desc_of(m, k, a_codes, a_scales), desc_of(n, k, b_codes, b_scales), a_codes, {m, n}, dtype);
 }
 
-// x . w^T; `few`: the tokens and columns that the one-kernel form takes
+// Whether x . w^T goes through the one-kernel form (actcomp_mx4_linear) or through
+// quantisation and product.  The one kernel decodes the weight again for every token,
+// the product does not (a weight in memory, us, one kernel / two):
+//   n x k           1 token      2            3            4
+//   4096 x 4096     6.2 / 14.4   8.4 / 14.4   10.8 / 14.4  13.0 / 14.3
+//   11008 x 4096    9.9 / 17.4   12.6 / 17.2  16.0 / 15.4  19.0 / 15.4
+//   4096 x 11008    12.1 / 23.3  18.1 / 23.4  23.7 / 23.2  29.3 / 23.1
+//   8192 x 8192     13.3 / 22.9  18.4 / 20.2  23.6 / 23.8  28.6 / 20.2
+//   16384 x 16384   38.8 / 42.2  53.8 / 43.4  66.3 / 40.2  81.0 / 40.0
+// They cross near 2^27 multiplications; one token stays below at every size.
+bool one_kernel(int64_t tokens, int64_t n, int64_t k) {
+    return tokens <= ACTCOMP_MX4_LINEAR_TOKENS && tokens * ((k + 31) / 32) * 36 <= ACTCOMP_MX4_LINEAR_BYTES &&
+           (tokens == 1 || (double)tokens * (double)n * (double)k <= (double)(1 << 27));
+}
+
+// x . w^T
 Tensor linear(const Tensor &x, int64_t n, int64_t k, const Tensor &codes, const Tensor &scales,
               std::optional<at::ScalarType> out_dtype) {
     need_cuda(x);
@@ -369,8 +384,7 @@ Tensor linear(const Tensor &x, int64_t n, int64_t k, const Tensor &codes, const 
     const int64_t tokens = x.numel() / k;
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
     shape.back() = n;
-    if (tokens <= ACTCOMP_MX4_LINEAR_TOKENS && (odt == dt || odt == 0) &&
-        tokens * ((k + 31) / 32) * 36 <= ACTCOMP_MX4_LINEAR_BYTES) {
+    if (one_kernel(tokens, n, k) && (odt == dt || odt == 0)) {
         const Tensor out = at::empty(shape, x.options().dtype(dtype));
         const c10::cuda::CUDAGuard guard(x.device());
         check("actcomp_mx4_linear",
@@ -399,4 +413,5 @@ PYBIND11_MODULE(_host, m) {
     m.def("dequantize", &dequantize);
     m.def("matmul", &matmul);
     m.def("linear", &linear);
+    m.def("one_kernel", &one_kernel);
 }
