@@ -4,7 +4,8 @@
 // and the shared-memory / instruction descriptors of tcgen05.mma.
 //
 // Descriptor bit layouts follow the PTX ISA (tcgen05 "shared memory
-// descriptor" and "instruction descriptor" tables).
+// descriptor" and "instruction descriptor" tables), as also spelled out in
+// CUTLASS cute/arch/mma_sm100_desc.hpp.
 #pragma once
 
 #include <cuda.h>
