@@ -20,7 +20,8 @@ the weight gradient contracts dy and x over tokens, both quantised by columns.
 
 Waits inside the product are bounded.  One that gives up leaves parts of the
 result unwritten and is recorded in the device error word, which
-``_lib.load().actcomp_last_device_error`` reads (ACT_E_TIMEOUT).
+``_lib.load().actcomp_last_device_error`` reads (ACT_E_TIMEOUT).  All functions
+compute outside autograd: results carry no graph, whatever the inputs require.
 """
 from __future__ import annotations
 

@@ -24,7 +24,10 @@ uses the held value.
 Waits inside the layer norm kernels are bounded.  One that gives up leaves NaN in
 the rows that its part of the device had and in the weight gradients, and is
 recorded in the device error word, which
-``_lib.load().actcomp_last_device_error`` reads (ACT_E_TIMEOUT)."""
+``_lib.load().actcomp_last_device_error`` reads (ACT_E_TIMEOUT).
+
+All functions compute outside autograd: results carry no graph, whatever the inputs
+require."""
 from __future__ import annotations
 
 from typing import Optional, Union

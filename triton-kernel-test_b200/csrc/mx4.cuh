@@ -42,8 +42,9 @@ __device__ __forceinline__ float scale_value(uint32_t code) {
 }
 
 // Eight scaled values to eight e2m1 codes, value j in nibble j (nearest, ties
-// to even, saturating).  Each byte leaves its asm block by itself: four of them
-// packed inside one block came out as zeros in some kernels (nvcc 12.9).
+// to even, saturating).  Each byte leaves its asm block by itself: with four of
+// them packed inside one block some kernels wrote zeros.  The cause is not known
+// (no reduced case was kept); the tests compare every code with a plain restatement.
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint16_t r;
     asm("{\n .reg .b8 t;\n cvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n mov.b16 %0, {t, 0};\n}" : "=h"(r) : "f"(lo), "f"(hi));
@@ -57,8 +58,8 @@ __device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
 // Codes j and j + 4 of a word as a pair of fp16 times 2^-14 (exact): the sign to
 // bit 15, exponent and mantissa to bits 11..9.  With fp16's bias of 15 against
 // e2m1's 1 that is the value times 2^-14, and e2m1's subnormal (exponent 0) is an
-// fp16 subnormal.  (The conversion instruction from e2m1 pairs takes the wrong
-// byte of the word in some kernels when nvcc 12.9 folds the shift into it.)
+// fp16 subnormal.  (With the conversion instruction from e2m1 pairs, on bytes
+// shifted out of the word, some kernels gave wrong values; the cause is not known.)
 template <int J>
 __device__ __forceinline__ uint32_t tiny_pair(uint32_t codes) {
     const uint32_t m = J < 3 ? codes << (J < 3 ? 9 - 4 * J : 0) : codes >> 3;

@@ -3,9 +3,10 @@
 //
 // It cannot do without the weight's 17/32 byte a value, read once, and one launch;
 // the tensor cores' 128-row tiles would be nearly empty and the quantisation a
-// launch of its own (16.0 us for both at 1 x 4096 x 11008, 8.9 us here).  Every CTA quantises all of x (it is
-// small) into shared memory as 8-bit integers (twice the e2m1 value: 0, 1, 2, 3,
-// 4, 6, 8, 12 and their negatives), one scale per block.
+// launch of its own (1 x 4096 x 11008, weight in L2: 16.0 us for both, 8.9 us here; in
+// memory 17.4 and 9.9).  Every CTA quantises all of x (it is small) into shared
+// memory as 8-bit integers (twice the e2m1 value: 0, 1, 2, 3, 4, 6, 8, 12 and their
+// negatives), one scale per block.
 //   warp  the four rows r0, r0 + 32, r0 + 64, r0 + 96 of a scale atom, whose
 //         scale words lie in one 16-byte piece; its pieces arrive by cp.async;
 //   lane  whole blocks of 32 values (16 bytes), every 32nd; a block's dot product
@@ -14,8 +15,11 @@
 // one of eight table bytes, the fourth (the sign) replaces it by its sign bit,
 // 0; the codes with their signs flipped give the negative ones' magnitudes.
 // Few rows: a CTA's warps share rows and split their blocks (KS).
-// Decoding and __dp4a bound it, not the weight's bytes (24 MB, 3.7 us): each
-// further token adds 3.2 us.  fp16 pairs and HFMA2 instead took 10.8 us.
+// Not the weight's bytes (24 MB, 3.7 us) but the work per code holds it: each
+// further token adds 3 us, so that three tokens or four on a large weight are
+// better off with the product (host.cpp has the rule and both sides' figures).  No
+// pipe is saturated (integer 55 %, issue slots 61 % at one token): the rest is
+// latency.  fp16 pairs and HFMA2 instead took 10.8 us.
 #include "mx4.cuh"
 
 namespace act {

@@ -1,9 +1,12 @@
 // mx4_quant.cu -- microscaled 4-bit quantisation (by rows, by columns, or both)
 // and its inverse; the format is stated in include/actcomp.h.
 //
-// HBM-bound: 2 bytes in and 17/32 out per bf16 value and direction; the integer
-// pipe is close behind (65 to 70 % busy).  16384 x 11008 bf16 on a B200: rows 85 us
-// (456 MB, 5.3 TB/s), columns 95 us, both 146 us (552 MB), inverse 91 us.
+// Its floor is HBM: 2 bytes in and 17/32 out per bf16 value and direction; instruction
+// issue and the integer pipe (65 to 72 % busy) hold it.  16384 x 11008 on a B200, us
+// and share of the copy rate:
+//             rows       columns    both       inverse
+//   bf16      86  82 %   93  76 %   144  59 %  90  78 %
+//   float32   132 96 %   206 61 %   259 55 %   190 66 %   (tile forms spill 60 to 88 bytes)
 //   rows   a lane takes eight consecutive values, four lanes a block of 32: loads
 //          and code stores are contiguous over the warp, the block's largest
 //          magnitude takes two shuffles; four rows of a scale atom together, so

@@ -26,17 +26,25 @@
 // by bulk copies into shared memory (RowRing).  Persistent CTAs: weights and the
 // weight-gradient sums stay in registers from row to row.  Short rows take a warp
 // or a group of warps each, rows of up to 16384 values a CTA; longer ones go
-// through kernels that re-read the row.
+// through kernels that re-read the row, and so do float32 rows of the backward pass
+// that leave no two ring slots in shared memory: past 13952 values, with dropout
+// (three inputs) past 9300.
 //
 // Measured on a B200, 16384 x 4096 bf16 (share of the copy rate, 6.47 TB/s):
-//   dropout                 60 us  4.5 TB/s  70 %  (the generator's multiplies; float32 87 us, 95 %)
+//   dropout                 60 us  4.5 TB/s  70 %  (float32 87 us, 95 %)
 //   forward                 47 us  5.7 TB/s  88 %
 //   backward                70 us  5.7 TB/s  89 %
-//   branch forward          98 us  5.5 TB/s  85 %
-//   branch backward        121 us  5.5 TB/s  86 %
+//   branch forward          97 us  5.5 TB/s  86 %
+//   branch backward        122 us  5.5 TB/s  85 %
+// The bf16 dropout saturates no pipe (issue slots 58 %, FMA 67 %); ten generator
+// rounds instead of one are 10 of its 60 us.  p = 0 draws its masks all the same.
 // Before the ring (loads in the row's own time) forward took 123 us and backward
 // 245; value by value instead of in pairs 90 and 112.  Ragged rows (16384 x 4097)
-// take 91 and 198 us: two-byte accesses, four times the instructions.
+// take 92 and 212 us, with dropout 224 and 346: two-byte accesses, four times the
+// instructions, and spilled registers (59 of the ragged forms, up to 260 bytes).
+// Longer rows at 8192 rows bf16 (floor; backward and branch backward): 6144 values 64
+// (47) and 104 (78) us, 8192 76 (62) and 123 (104), 9216 134 (70) and 217 (117), 11008
+// 141 (84) and 221 (139), 16384 182 (125) and 288 (208): one CTA per SM there.
 #include <cuda_fp16.h>
 #include <string.h>
 
@@ -747,7 +755,9 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT))
     // Up to two segments a thread the row's g and x-hat are held from the sums to
     // the output, past that they are computed again from the slot (registers); so
     // too at 320 threads, where that fits two CTAs (8192 x 5120 bf16 with dropout
-    // 89 us; held, in one CTA, 99 us; float32 is the other way, 89 us and 82 us).
+    // 89 us; held, in one CTA, 99 us).  Past 320 threads two CTAs do not fit, and
+    // float32 holds in one CTA from there on (8192 x 5120 without dropout 82 us,
+    // computed again in two CTAs 89 us).
     constexpr bool HOLD = NCH <= 2 && MAXT != 320;
     // four segments: their sums fill the registers, the weights are read again too
     constexpr bool WREG = NCH <= 2;
@@ -952,8 +962,10 @@ __global__ void __launch_bounds__(128) ln_bwd_cols_kernel(BwdArgs<T, W> a, const
 
 // dw / db from the `parts` partial sums, in a fixed order: a column's sum does
 // not depend on timing.  A warp takes 32 columns, the CTA's eight warps every
-// eighth partial, eight loads in flight.  Launched under the kernel before it
-// (programmatic dependence): it waits for that kernel's end before it reads.
+// eighth partial, eight loads in flight.  Launched with programmatic dependence on
+// the kernel before it, which gives no signal of its own: the CTAs start as that
+// kernel's last ones leave, which hides the launch, and wait for its end (and its
+// writes) before they read.
 template <typename W>
 __global__ void __launch_bounds__(256) ln_bwd_finish_kernel(const float *part, int parts, int64_t cols, W *dw, W *db) {
     __shared__ float red[8][33];

@@ -8,7 +8,7 @@
 //   the four output words are eight 16-bit halves, half column & 7 decides:
 //   kept iff half >= threshold, threshold = round(p * 2^16) in 0 .. 2^16.
 // Sixteen bits a value: one generator call serves eight values, one 16-byte load
-// of a 16-bit type.  The 20 wide products of a call are then a fifth of a bf16
+// of a 16-bit type.  The 20 wide products of a call are then a sixth of a bf16
 // dropout's time (16384 x 4096: 60 us, with one round instead of ten 50 us); at 32
 // bits a value there would be twice as many.  The scale uses the held probability
 // threshold / 2^16, so the expectation is exact.  Rows count from row_offset: a
