@@ -358,7 +358,7 @@ struct RowView {
 // abort word: no slot is filled again, and after its last row a CTA that sees the
 // word writes NaN over all its results (fwd_nan, bwd_nan: calls at the kernels' ends,
 // so that the rows' own registers stay as they were; a test of each wait's outcome in
-// the rows' code cost up to 17 %, this 0 to 3, on some ragged forms up to 6).
+// the rows' code cost up to 17 %, this 0 to 5, on one ragged form 6).
 template <typename T, int INPUTS, bool VEC>
 struct RowRing {
     uint8_t *slots;
