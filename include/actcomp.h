@@ -441,6 +441,59 @@ int actcomp_layer_norm_bwd(const actcomp_ln_bwd_args *a, void *workspace, size_t
  * and the device error word records the timeout. */
 int actcomp_selftest_row_waits(const float *x, int32_t rows, int32_t brought, uint32_t polls, float *out, void *stream);
 
+/* ========================================================= root-mean-square norm
+ * y = h * rstd * weight with h = x, or h = x + res written to h (y normalises the
+ * unrounded float32 sum), rstd = 1 / sqrt(mean of h^2 + eps) in float32 (rows).
+ * Types, strides and alignment as for layer norm; weight may be NULL (1); rows may be
+ * 0.  codes != NULL (then y == NULL): the output in 8 bits instead, e4m3 with one
+ * scale per 128 values of a row, rounded from the float32 result; codes rows x ldc
+ * bytes (16-byte aligned, ldc a multiple of 16) and scales as an actcomp_fp8 of rows x
+ * cols in blocks of ACTCOMP_FP8_ROWS.  A device-side wait that gives up (here and in
+ * the backward pass; actcomp_last_device_error) leaves NaN in the rows of its CTA and
+ * in the weight gradient. */
+typedef struct actcomp_rms_args {
+    int64_t rows, cols;
+    const void *x;
+    int64_t ldx;
+    const void *res;
+    int64_t ldr;
+    const void *weight;
+    void *y;
+    int64_t ldy;
+    void *h;
+    int64_t ldh;
+    uint8_t *codes;
+    int64_t ldc;
+    uint8_t *scales;
+    float *rstd;
+    int32_t dtype, wdtype;
+    float eps;
+    int32_t reserved;
+} actcomp_rms_args;
+int actcomp_rms_norm(const actcomp_rms_args *a, void *stream);
+/* Backward from dy, the normalised input x (h with a residual) and rstd: dx is the
+ * gradient of h (+ dh, the gradient that h receives from elsewhere, if not NULL), which
+ * is that of x and of the residual both.  dweight may be NULL; its sum over rows runs
+ * in a fixed order.  workspace: actcomp_rms_norm_bwd_workspace() bytes, 16-byte
+ * aligned, uninitialised. */
+typedef struct actcomp_rms_bwd_args {
+    int64_t rows, cols;
+    const void *dy;
+    int64_t lddy;
+    const void *x;
+    int64_t ldx;
+    const void *dh;
+    int64_t lddh;
+    const void *weight;
+    const float *rstd;
+    void *dx;
+    int64_t lddx;
+    void *dweight;
+    int32_t dtype, wdtype;
+} actcomp_rms_bwd_args;
+size_t actcomp_rms_norm_bwd_workspace(int64_t rows, int64_t cols);
+int actcomp_rms_norm_bwd(const actcomp_rms_bwd_args *a, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ========================================================= microscaled 4-bit
  * A rows x cols matrix in 4-bit floating point with one power-of-two scale per
  * 32 consecutive values of a row (OCP Microscaling, MXFP4).  No reference
@@ -485,6 +538,95 @@ int actcomp_mx4_gemm(const actcomp_mx4 *a, const actcomp_mx4 *b, void *c, int64_
 #define ACTCOMP_MX4_LINEAR_BYTES (160 * 1024)
 int actcomp_mx4_linear(const void *x, int64_t tokens, int64_t cols, int64_t ldx, int32_t dtype, const actcomp_mx4 *w,
                        void *c, int64_t ldc, int32_t c_dtype, void *stream);
+
+/* ========================================================= 8-bit floating point
+ * A rows x cols matrix in 8-bit floating point with one power-of-two scale per block
+ * of 128 values.  No reference counterpart.
+ *   codes   rows x ld bytes, row-major (columns past cols are unspecified): e4m3
+ *           (ACTCOMP_FP8_E4M3, largest value 448) or e5m2 (ACTCOMP_FP8_E5M2, 57344)
+ *   scales  one byte e a block, value 2^(e - 127), 255 = NaN.  Blocks:
+ *           ACTCOMP_FP8_ROWS   1 x 128, along the rows;
+ *           ACTCOMP_FP8_COLS   128 x 1, down the columns;
+ *           ACTCOMP_FP8_TILES  128 x 128, byte of (row block i, column block j) at
+ *                              i * ceil(cols / 128) + j.
+ *           ROWS: byte of (row r, column block b) at (b * ceil(rows / 128) + r / 128) *
+ *           128 + (r % 32) * 4 + (r % 128) / 32; COLS: the same with column and row
+ *           block.  Bytes of rows or columns past the end are unspecified.
+ * A value is its code times its block's scale.  Quantisation: the scale's exponent is
+ * the smallest (at least -127) under which the block's largest magnitude is at most the
+ * format's largest value, code = value / scale to the nearest, ties to even; a block that
+ * holds a NaN or an infinity gets scale 255 (all its values read as NaN).
+ * transposed: the operand of a product is the transpose of what is stored.  A product
+ * contracts along its operands' blocks: ROWS takes transposed = 0, COLS 1, TILES
+ * either.  codes and scales are 16-byte aligned, ld is a multiple of 16; rows and cols
+ * are at least 1. */
+#define ACTCOMP_FP8_E4M3 0
+#define ACTCOMP_FP8_E5M2 1
+#define ACTCOMP_FP8_ROWS 0
+#define ACTCOMP_FP8_COLS 1
+#define ACTCOMP_FP8_TILES 2
+typedef struct actcomp_fp8 {
+    int64_t rows, cols, ld;
+    uint8_t *codes;
+    uint8_t *scales;
+    int32_t format, block, transposed, reserved;
+} actcomp_fp8;
+size_t actcomp_fp8_scale_bytes(int64_t rows, int64_t cols, int32_t block);
+/* Quantise x (rows x cols, dtype 0 = float32, 1 = bf16, 2 = fp16, row stride ldx) into q
+ * (blocks ROWS or TILES), qt (COLS), or, with q in ROWS, both of one format from one
+ * read; each may be NULL. */
+int actcomp_fp8_quantize(const void *x, int64_t rows, int64_t cols, int64_t ldx, int32_t dtype, const actcomp_fp8 *q,
+                         const actcomp_fp8 *qt, void *stream);
+/* The values of q as stored (whatever transposed says), rows x cols of `dtype` (row
+ * stride ldo). */
+int actcomp_fp8_dequantize(const actcomp_fp8 *q, void *out, int64_t ldo, int32_t dtype, void *stream);
+/* c = a . b^T (row stride ldc) for operands of one contraction length, float32
+ * accumulation on the tensor cores; c_dtype 0 = float32, 1 = bf16, 2 = fp16.  Where a
+ * device-side wait gives up (actcomp_last_device_error) parts of c stay unwritten. */
+int actcomp_fp8_gemm(const actcomp_fp8 *a, const actcomp_fp8 *b, void *c, int64_t ldc, int32_t c_dtype, void *stream);
+
+/* ========================================================= cross entropy of a linear layer
+ * loss and lse = log sum_v exp z_v of z = x . weight^T (tokens x vocab), which is never
+ * in memory: loss = lse - z[target], 0 where target == ignore_index, NaN where it lies
+ * outside the vocabulary otherwise.  x (tokens x channels, row stride ldx) and weight
+ * (vocab x channels, row stride ldw) in bf16 (dtype 1) or fp16 (2), 16-byte aligned rows;
+ * loss and lse float32, tokens each.  tokens may be 0.  The products are accumulated
+ * in float32 on the tensor cores.  A device-side wait that gives up
+ * (actcomp_last_device_error) leaves NaN in loss and lse of the tokens it had; in the
+ * backward pass parts of the gradients may stay unwritten.  workspaces are
+ * uninitialised; the forward's is 16-byte, the backward's 256-byte aligned. */
+typedef struct actcomp_xent_args {
+    int64_t tokens, channels, vocab;
+    const void *x;
+    int64_t ldx;
+    const void *weight;
+    int64_t ldw;
+    const int64_t *target;
+    int64_t ignore_index;
+    float *loss; /* not used by the backward pass */
+    float *lse;  /* the backward pass reads it */
+    int32_t dtype, reserved;
+} actcomp_xent_args;
+size_t actcomp_xent_workspace(int64_t tokens, int64_t vocab);
+int actcomp_xent(const actcomp_xent_args *a, void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients from dloss (tokens, not read where the target is ignored) and dlse (tokens,
+ * or NULL): dz = exp(z - lse) (dloss + dlse) - [target] dloss, dx = dz . weight, dweight =
+ * dz^T . x, in x's type; either may be NULL.  dz is rounded to x's type, scaled so that
+ * fp16 holds it.  A token without a gradient (ignored or dloss 0, and no dlse) adds
+ * nothing, whatever its row of x holds; one whose target lies outside the vocabulary
+ * makes its row of dx and all of dweight NaN.  The vocabulary is taken in pieces of `piece`
+ * columns (rounded to whole tiles of 256; 0: what keeps a piece's dz in 1 GiB); the
+ * workspace is actcomp_xent_bwd_workspace() bytes of the same piece. */
+typedef struct actcomp_xent_grads {
+    const float *dloss, *dlse;
+    void *dx;
+    int64_t lddx;
+    void *dweight;
+    int64_t lddw;
+} actcomp_xent_grads;
+size_t actcomp_xent_bwd_workspace(int64_t tokens, int64_t channels, int64_t vocab, int64_t piece);
+int actcomp_xent_bwd(const actcomp_xent_args *a, const actcomp_xent_grads *g, int64_t piece, void *workspace,
+                     size_t workspace_bytes, void *stream);
 
 /* Error statistics of a reconstruction against its original (n bf16 values):
  * out[0] += sum (a-b)^2, out[1] += sum b^2, out[2] = max(out[2], max|a-b|),

@@ -116,6 +116,40 @@ class Mx4Desc(ctypes.Structure):
     _fields_ = [("rows", c_i64), ("cols", c_i64), ("codes", c_vp), ("scales", c_vp)]
 
 
+class RmsArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("cols", c_i64), ("x", c_vp), ("ldx", c_i64), ("res", c_vp), ("ldr", c_i64),
+        ("weight", c_vp), ("y", c_vp), ("ldy", c_i64), ("h", c_vp), ("ldh", c_i64), ("codes", c_vp), ("ldc", c_i64),
+        ("scales", c_vp), ("rstd", c_vp), ("dtype", c_i32), ("wdtype", c_i32), ("eps", ctypes.c_float),
+        ("reserved", c_i32),
+    ]
+
+
+class RmsBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("cols", c_i64), ("dy", c_vp), ("lddy", c_i64), ("x", c_vp), ("ldx", c_i64), ("dh", c_vp),
+        ("lddh", c_i64), ("weight", c_vp), ("rstd", c_vp), ("dx", c_vp), ("lddx", c_i64), ("dweight", c_vp),
+        ("dtype", c_i32), ("wdtype", c_i32),
+    ]
+
+
+class Fp8Desc(ctypes.Structure):
+    _fields_ = [("rows", c_i64), ("cols", c_i64), ("ld", c_i64), ("codes", c_vp), ("scales", c_vp),
+                ("format", c_i32), ("block", c_i32), ("transposed", c_i32), ("reserved", c_i32)]
+
+
+class XentArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", c_i64), ("channels", c_i64), ("vocab", c_i64), ("x", c_vp), ("ldx", c_i64), ("weight", c_vp),
+        ("ldw", c_i64), ("target", c_vp), ("ignore_index", c_i64), ("loss", c_vp), ("lse", c_vp), ("dtype", c_i32),
+        ("reserved", c_i32),
+    ]
+
+
+class XentGrads(ctypes.Structure):
+    _fields_ = [("dloss", c_vp), ("dlse", c_vp), ("dx", c_vp), ("lddx", c_i64), ("dweight", c_vp), ("lddw", c_i64)]
+
+
 #: entry point -> (restype, argtypes); mirrors include/actcomp.h
 SIGNATURES = {
     "actcomp_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -163,12 +197,27 @@ SIGNATURES = {
     "actcomp_mx4_linear": (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_i32, ctypes.POINTER(Mx4Desc), c_vp, c_i64,
                                           c_i32, c_vp]),
     "actcomp_mx4_gemm": (ctypes.c_int, [ctypes.POINTER(Mx4Desc), ctypes.POINTER(Mx4Desc), c_vp, c_i64, c_i32, c_vp]),
+    "actcomp_rms_norm": (ctypes.c_int, [ctypes.POINTER(RmsArgs), c_vp]),
+    "actcomp_rms_norm_bwd_workspace": (ctypes.c_size_t, [c_i64, c_i64]),
+    "actcomp_rms_norm_bwd": (ctypes.c_int, [ctypes.POINTER(RmsBwdArgs), c_vp, ctypes.c_size_t, c_vp]),
+    "actcomp_fp8_scale_bytes": (ctypes.c_size_t, [c_i64, c_i64, c_i32]),
+    "actcomp_fp8_quantize": (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_i32, ctypes.POINTER(Fp8Desc),
+                                            ctypes.POINTER(Fp8Desc), c_vp]),
+    "actcomp_fp8_dequantize": (ctypes.c_int, [ctypes.POINTER(Fp8Desc), c_vp, c_i64, c_i32, c_vp]),
+    "actcomp_fp8_gemm": (ctypes.c_int, [ctypes.POINTER(Fp8Desc), ctypes.POINTER(Fp8Desc), c_vp, c_i64, c_i32, c_vp]),
+    "actcomp_xent_workspace": (ctypes.c_size_t, [c_i64, c_i64]),
+    "actcomp_xent": (ctypes.c_int, [ctypes.POINTER(XentArgs), c_vp, ctypes.c_size_t, c_vp]),
+    "actcomp_xent_bwd_workspace": (ctypes.c_size_t, [c_i64, c_i64, c_i64, c_i64]),
+    "actcomp_xent_bwd": (ctypes.c_int, [ctypes.POINTER(XentArgs), ctypes.POINTER(XentGrads), c_i64, c_vp,
+                                        ctypes.c_size_t, c_vp]),
 }
 
 #: entry points behind :class:`Host`, bound on its first use
 _HOST_API = ("actcomp_dropout", "actcomp_layer_norm", "actcomp_mx4_")
+#: entry points behind it that it binds where the library has them (their callers ask)
+_HOST_LATER = ("actcomp_rms_norm", "actcomp_fp8_", "actcomp_xent")
 #: what another build of the library may lack: the rest of the package does not need them
-_OPTIONAL = _HOST_API + ("actcomp_selftest_row_waits",)
+_OPTIONAL = _HOST_API + _HOST_LATER + ("actcomp_selftest_row_waits",)
 
 _lock = threading.Lock()
 _lib = None
@@ -214,9 +263,10 @@ def check(fn: str, status: int) -> None:
 
 
 class Host:
-    """The extension module that runs the host side of :mod:`actcomp.norm` and
-    :mod:`actcomp.mx4` (csrc/host.cpp), loaded and bound to the library by the
-    first call of one of its functions: nothing else of the package needs it."""
+    """The extension module that runs the host side of :mod:`actcomp.norm`,
+    :mod:`actcomp.mx4`, :mod:`actcomp.fp8` and :mod:`actcomp.loss` (csrc/host.cpp),
+    loaded and bound to the library by the first call of one of its functions:
+    nothing else of the package needs it."""
 
     _guard = threading.Lock()
 
@@ -245,6 +295,7 @@ class Host:
         spec = util.spec_from_file_location(__package__ + "._host", path)
         module = util.module_from_spec(spec)
         spec.loader.exec_module(module)
+        names += [n for n in SIGNATURES if n.startswith(_HOST_LATER) and hasattr(lib, n)]
         module.bind({n: ctypes.cast(getattr(lib, n), c_vp).value for n in names})
         self.__dict__.update({k: v for k, v in vars(module).items() if not k.startswith("__")})
 

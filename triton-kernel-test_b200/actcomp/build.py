@@ -59,7 +59,7 @@ def stale(lib: str = LIB) -> bool:
 
 
 def host_path() -> str:
-    """The extension module of the host side of actcomp.norm and actcomp.mx4
+    """The extension module of the host side of actcomp.norm, mx4, fp8 and loss
     (csrc/host.cpp).  It is compiled against one torch and one Python and named
     after both, so that one built for others is never loaded or taken as up to date."""
     import sysconfig

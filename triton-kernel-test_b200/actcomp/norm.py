@@ -1,5 +1,5 @@
-"""Dropout without a stored mask, layer norm with its backward pass, and both
-across a residual branch.
+"""Dropout without a stored mask, layer norm with its backward pass, both across a
+residual branch, and root-mean-square norm.
 
 The reference's step (low_rank_system_profile_backward.py) has only the linear
 layers; these are what a training step runs between them.  What they save for
@@ -11,6 +11,11 @@ the backward pass is a seed and two float32 per row:
   dx, dw, db           = layer_norm_backward(dy, x, weight, mean, rstd)
   y, h, mean, rstd     = dropout_add_layer_norm(x, residual, weight, bias, p, seed)
   dx, dresidual, dw, db = dropout_add_layer_norm_backward(dy, h, weight, mean, rstd, p, seed, dh=dh)
+  y, rstd              = rms_norm(x, weight)
+  y, h, rstd           = add_rms_norm(x, residual, weight)
+  dx, dw               = rms_norm_backward(dy, x or h, weight, rstd, dh=dh)
+
+(:func:`actcomp.fp8.rms_norm` and :func:`actcomp.fp8.add_rms_norm` give y in 8 bits.)
 
 Activations are float32, bfloat16 or float16 of any leading shape, normalised
 over the last dimension; weight and bias have their dtype or float32.  A row is
@@ -21,7 +26,7 @@ int64 CUDA tensor that the kernel reads (so that a captured graph can draw new
 masks); ``p`` is held to 16 bits (``round(p * 65536) / 65536``) and the scale
 uses the held value.
 
-Waits inside the layer norm kernels are bounded.  One that gives up leaves NaN in
+Waits inside the norms' kernels are bounded.  One that gives up leaves NaN in
 the rows that its part of the device had and in the weight gradients, and is
 recorded in the device error word, which
 ``_lib.load().actcomp_last_device_error`` reads (ACT_E_TIMEOUT).
@@ -88,3 +93,27 @@ def dropout_add_layer_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: O
     the gradient of y and, if h is used further on, dh, the gradient h gets there.
     ``bias_grad`` and ``bias_dtype`` as in :func:`layer_norm_backward`."""
     return _host.branch_backward(dy, h, weight, mean, rstd, p, seed, row_offset, dh, bias_grad, bias_dtype)
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+             eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor]:
+    """(y, rstd): each row of the last dimension over the root of its mean square, times
+    weight; rstd = 1 / sqrt(mean of squares + eps) (float32, the leading shape) is what
+    the backward pass needs beside x."""
+    return _host.rms_norm(x, weight, eps)
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                 eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, h, rstd) with h = x + residual and y = rms_norm(h), in one pass; y normalises
+    the float32 sum, h is its rounding to the dtype."""
+    return _host.add_rms_norm(x, residual, weight, eps)
+
+
+def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], rstd: torch.Tensor,
+                      dh: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(dx, dweight) of :func:`rms_norm`, or with x = h of :func:`add_rms_norm`, whose x
+    and residual both have the gradient dx; dh is the gradient that h gets where it is
+    used further on.  dweight (None without a weight) has the weight's dtype; its sum
+    runs over the rows in a fixed order: the same inputs give the same bits."""
+    return _host.rms_norm_backward(dy, x, weight, rstd, dh)

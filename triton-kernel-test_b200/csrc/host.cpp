@@ -1,4 +1,4 @@
-// host.cpp -- the host side of actcomp.norm and actcomp.mx4: argument checks,
+// host.cpp -- the host side of actcomp.norm, mx4, fp8 and loss: argument checks,
 // output allocation and the call of the C ABI, as a Python extension module
 // (built and named by actcomp/build.py).  It computes nothing.  A call's host time
 // is what a user waits for at small sizes: layer norm of 8 x 4096 is 3 us on the
@@ -33,11 +33,34 @@ struct Api {
     decltype(&actcomp_mx4_dequantize) mx4_dequantize;
     decltype(&actcomp_mx4_gemm) mx4_gemm;
     decltype(&actcomp_mx4_linear) mx4_linear;
+    decltype(&actcomp_rms_norm) rms_norm;
+    decltype(&actcomp_rms_norm_bwd) rms_norm_bwd;
+    decltype(&actcomp_rms_norm_bwd_workspace) rms_norm_bwd_workspace;
+    decltype(&actcomp_fp8_quantize) fp8_quantize;
+    decltype(&actcomp_fp8_dequantize) fp8_dequantize;
+    decltype(&actcomp_fp8_gemm) fp8_gemm;
+    decltype(&actcomp_xent_workspace) xent_workspace;
+    decltype(&actcomp_xent) xent;
+    decltype(&actcomp_xent_bwd_workspace) xent_bwd_workspace;
+    decltype(&actcomp_xent_bwd) xent_bwd;
 } api{};
 
 template <typename F>
 void bind_one(const py::dict &addresses, const char *name, F &f) {
     f = reinterpret_cast<F>(addresses[name].cast<uintptr_t>());
+}
+// An entry point that an earlier build of the library lacks stays null; its callers ask need().
+template <typename F>
+void bind_later(const py::dict &addresses, const char *name, F &f) {
+    if (addresses.contains(name)) bind_one(addresses, name, f);
+}
+template <typename F>
+F need(F f, const char *name) {
+    if (!f) {
+        PyErr_SetString(PyExc_ImportError, (std::string("the loaded library lacks ") + name).c_str());
+        throw py::error_already_set();
+    }
+    return f;
 }
 void bind(const py::dict &d) {
     bind_one(d, "actcomp_dropout", api.dropout);
@@ -48,6 +71,16 @@ void bind(const py::dict &d) {
     bind_one(d, "actcomp_mx4_dequantize", api.mx4_dequantize);
     bind_one(d, "actcomp_mx4_gemm", api.mx4_gemm);
     bind_one(d, "actcomp_mx4_linear", api.mx4_linear);
+    bind_later(d, "actcomp_rms_norm", api.rms_norm);
+    bind_later(d, "actcomp_rms_norm_bwd", api.rms_norm_bwd);
+    bind_later(d, "actcomp_rms_norm_bwd_workspace", api.rms_norm_bwd_workspace);
+    bind_later(d, "actcomp_fp8_quantize", api.fp8_quantize);
+    bind_later(d, "actcomp_fp8_dequantize", api.fp8_dequantize);
+    bind_later(d, "actcomp_fp8_gemm", api.fp8_gemm);
+    bind_later(d, "actcomp_xent_workspace", api.xent_workspace);
+    bind_later(d, "actcomp_xent", api.xent);
+    bind_later(d, "actcomp_xent_bwd_workspace", api.xent_bwd_workspace);
+    bind_later(d, "actcomp_xent_bwd", api.xent_bwd);
 }
 
 // Raises the package's ActcompError for a non-zero status.
@@ -400,6 +433,261 @@ Tensor linear(const Tensor &x, int64_t n, int64_t k, const Tensor &codes, const 
     return product(q.desc, w, x, shape, dtype);
 }
 
+// ---------------------------------------------------------------- root-mean-square norm
+// (y or codes, scales, h, rstd)
+struct RmsOut {
+    Tensor y, scales, rstd;
+    OptTensor h;
+};
+RmsOut rms_forward(const Tensor &x, const OptTensor &residual, const OptTensor &weight, double eps, bool codes) {
+    need_cuda(x);
+    const auto fn = need(api.rms_norm, "actcomp_rms_norm");
+    const int dt = dtype_of(x.scalar_type());
+    const Geometry g = geometry(x);
+    if (residual) same(x, *residual, "residual");
+    const int wdt = affine(x, g.cols, weight, {});
+    if (g.cols == 0) bad_value("norm over an empty last dimension");
+    if (codes && g.rows == 0) bad_value("a non-empty tensor is expected, got shape " + str(x));
+    if (!(eps >= 0.0)) bad_value("eps must not be negative");
+    const Rows r = rows_of(x, g.cols), rr = residual ? rows_of(*residual, g.cols) : Rows{};
+    const OptTensor w = packed(weight);
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    RmsOut o;
+    const int64_t ldc = (g.cols + 15) / 16 * 16;
+    if (codes) {
+        o.y = at::empty({g.rows, ldc}, x.options().dtype(at::kByte));
+        o.scales = at::empty({(g.cols + 127) / 128 * ((g.rows + 127) / 128) * 128}, o.y.options());
+    } else {
+        o.y = fresh(x);
+    }
+    if (residual) o.h = fresh(x);
+    o.rstd = at::empty(lead, x.options().dtype(at::kFloat));
+    const actcomp_rms_args a{g.rows, g.cols, ptr(r.t), r.ld, residual ? ptr(rr.t) : nullptr, residual ? rr.ld : 0, ptr(w),
+                             codes ? nullptr : ptr(o.y), g.cols, ptr(o.h), g.cols,
+                             codes ? static_cast<uint8_t *>(ptr(o.y)) : nullptr, ldc,
+                             codes ? static_cast<uint8_t *>(ptr(o.scales)) : nullptr,
+                             static_cast<float *>(ptr(o.rstd)), dt, wdt, (float)eps, 0};
+    const c10::cuda::CUDAGuard guard(x.device());
+    check("actcomp_rms_norm", fn(&a, stream_of(x)));
+    return o;
+}
+std::tuple<Tensor, Tensor> rms_norm(const Tensor &x, const OptTensor &weight, double eps) {
+    const RmsOut o = rms_forward(x, {}, weight, eps, false);
+    return {o.y, o.rstd};
+}
+std::tuple<Tensor, Tensor, Tensor> add_rms_norm(const Tensor &x, const Tensor &residual, const OptTensor &weight,
+                                                double eps) {
+    const RmsOut o = rms_forward(x, residual, weight, eps, false);
+    return {o.y, *o.h, o.rstd};
+}
+std::tuple<int64_t, int64_t, Tensor, Tensor, OptTensor, Tensor> rms_norm_fp8(const Tensor &x, const OptTensor &residual,
+                                                                            const OptTensor &weight, double eps) {
+    const RmsOut o = rms_forward(x, residual, weight, eps, true);
+    return {o.y.size(0), x.size(-1), o.y, o.scales, o.h, o.rstd};
+}
+
+std::tuple<Tensor, OptTensor> rms_norm_backward(const Tensor &dy, const Tensor &x, const OptTensor &weight,
+                                                const Tensor &rstd, const OptTensor &dh) {
+    need_cuda(x);
+    const auto fn = need(api.rms_norm_bwd, "actcomp_rms_norm_bwd");
+    const int dt = dtype_of(x.scalar_type());
+    const Geometry g = geometry(x);
+    same(x, dy, "dy");
+    if (dh) same(x, *dh, "dh");
+    const int wdt = affine(x, g.cols, weight, {});
+    if (g.cols == 0) bad_value("norm over an empty last dimension");
+    const Tensor s = stats(rstd, g.rows, x, "rstd");
+    const Rows ry = rows_of(dy, g.cols), rx = rows_of(x, g.cols), rh = dh ? rows_of(*dh, g.cols) : Rows{};
+    const OptTensor w = packed(weight);
+    const Tensor dx = fresh(x);
+    const OptTensor dw = weight ? OptTensor(at::empty({g.cols}, weight->options())) : OptTensor();
+    const c10::cuda::CUDAGuard guard(x.device());
+    const size_t bytes = need(api.rms_norm_bwd_workspace, "actcomp_rms_norm_bwd_workspace")(g.rows, g.cols);
+    const Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 1)}, x.options().dtype(at::kByte));
+    const actcomp_rms_bwd_args a{g.rows, g.cols, ptr(ry.t), ry.ld, ptr(rx.t), rx.ld, dh ? ptr(rh.t) : nullptr,
+                                 dh ? rh.ld : 0, ptr(w), static_cast<const float *>(ptr(s)), ptr(dx), g.cols, ptr(dw),
+                                 dt, wdt};
+    check("actcomp_rms_norm_bwd", fn(&a, ptr(ws), bytes, stream_of(x)));
+    return {dx, dw};
+}
+
+// ---------------------------------------------------------------- 8-bit floating point
+// The stored matrix of a descriptor (rows, cols as stored).
+actcomp_fp8 fp8_desc(int64_t rows, int64_t cols, const Tensor &codes, const Tensor &scales, int format, int block,
+                     bool transposed) {
+    need_cuda(codes);
+    if (format < 0 || format > 1 || block < 0 || block > 2) bad_value("unknown 8-bit format or block form");
+    const int64_t b = ((rows + 127) / 128) * ((cols + 127) / 128) * (block == ACTCOMP_FP8_TILES ? 1 : 128);
+    if (rows < 1 || cols < 1 || codes.dim() != 2 || codes.size(0) != rows || codes.size(1) != (cols + 15) / 16 * 16 ||
+        scales.numel() != b || !codes.is_contiguous() || !scales.is_contiguous() || codes.scalar_type() != at::kByte ||
+        scales.scalar_type() != at::kByte || scales.device() != codes.device())
+        bad_value("codes and scales do not belong to a matrix of " + std::to_string(rows) + " x " + std::to_string(cols));
+    return {rows, cols, codes.size(1), static_cast<uint8_t *>(ptr(codes)), static_cast<uint8_t *>(ptr(scales)), format,
+            block, transposed, 0};
+}
+struct Fp8Buffers {
+    Tensor codes, scales;
+    actcomp_fp8 desc;
+};
+Fp8Buffers empty_fp8(const Tensor &x, int64_t rows, int64_t cols, int format, int block) {
+    const auto opt = x.options().dtype(at::kByte);
+    const int64_t blocks = ((rows + 127) / 128) * ((cols + 127) / 128);
+    Fp8Buffers q{at::empty({rows, (cols + 15) / 16 * 16}, opt),
+                 at::empty({block == ACTCOMP_FP8_TILES ? blocks : blocks * 128}, opt), {}};
+    q.desc = fp8_desc(rows, cols, q.codes, q.scales, format, block, block == ACTCOMP_FP8_COLS);
+    return q;
+}
+
+// (rows, cols, codes and scales by rows or tiles, codes and scales by columns) of the
+// joined matrix; what is not asked for is None
+std::tuple<int64_t, int64_t, OptTensor, OptTensor, OptTensor, OptTensor> fp8_quantize(const Tensor &x, bool by_rows,
+                                                                                     bool by_cols, bool tiles,
+                                                                                     int format) {
+    need_cuda(x);
+    const auto fn = need(api.fp8_quantize, "actcomp_fp8_quantize");
+    const int dt = dtype_of(x.scalar_type());
+    const Rows r = matrix(x);
+    const int64_t cols = x.size(-1), rows = x.numel() / cols;
+    std::optional<Fp8Buffers> q, qt;
+    if (by_rows || tiles) q = empty_fp8(x, rows, cols, format, tiles ? ACTCOMP_FP8_TILES : ACTCOMP_FP8_ROWS);
+    if (by_cols) qt = empty_fp8(x, rows, cols, format, ACTCOMP_FP8_COLS);
+    const c10::cuda::CUDAGuard guard(x.device());
+    check("actcomp_fp8_quantize", fn(ptr(r.t), rows, cols, r.ld, dt, q ? &q->desc : nullptr, qt ? &qt->desc : nullptr,
+                                     stream_of(x)));
+    const auto c = [](const std::optional<Fp8Buffers> &v) { return v ? OptTensor(v->codes) : OptTensor(); };
+    const auto s = [](const std::optional<Fp8Buffers> &v) { return v ? OptTensor(v->scales) : OptTensor(); };
+    return {rows, cols, c(q), s(q), c(qt), s(qt)};
+}
+
+Tensor fp8_dequantize(int64_t rows, int64_t cols, const Tensor &codes, const Tensor &scales, int format, int block,
+                      at::ScalarType dtype) {
+    const auto fn = need(api.fp8_dequantize, "actcomp_fp8_dequantize");
+    const int dt = dtype_of(dtype);
+    const actcomp_fp8 d = fp8_desc(rows, cols, codes, scales, format, block, block == ACTCOMP_FP8_COLS);
+    const Tensor out = at::empty({rows, cols}, codes.options().dtype(dtype));
+    const c10::cuda::CUDAGuard guard(codes.device());
+    check("actcomp_fp8_dequantize", fn(&d, ptr(out), cols, dt, stream_of(codes)));
+    return out;
+}
+
+// An operand as Python holds it: stored rows and columns, codes, scales, format, block, transposed.
+using Fp8Operand = std::tuple<int64_t, int64_t, Tensor, Tensor, int, int, bool>;
+actcomp_fp8 fp8_desc(const Fp8Operand &q) {
+    return fp8_desc(std::get<0>(q), std::get<1>(q), std::get<2>(q), std::get<3>(q), std::get<4>(q), std::get<5>(q),
+                    std::get<6>(q));
+}
+Tensor fp8_product(const actcomp_fp8 &a, const actcomp_fp8 &b, const Tensor &like, at::IntArrayRef shape,
+                   at::ScalarType dtype) {
+    const auto fn = need(api.fp8_gemm, "actcomp_fp8_gemm");
+    const int dt = dtype_of(dtype);
+    const Tensor out = at::empty(shape, like.options().dtype(dtype));
+    const c10::cuda::CUDAGuard guard(like.device());
+    check("actcomp_fp8_gemm", fn(&a, &b, ptr(out), b.transposed ? b.cols : b.rows, dt, stream_of(like)));
+    return out;
+}
+Tensor fp8_matmul(const Fp8Operand &a, const Fp8Operand &b, at::ScalarType dtype) {
+    const actcomp_fp8 da = fp8_desc(a), db = fp8_desc(b);
+    const Tensor &like = std::get<2>(a);
+    if (like.device() != std::get<2>(b).device()) bad_value("operands on different devices");
+    return fp8_product(da, db, like, {da.transposed ? da.cols : da.rows, db.transposed ? db.cols : db.rows}, dtype);
+}
+// x . w^T with x quantised by rows on the way
+Tensor fp8_linear(const Tensor &x, const Fp8Operand &w, std::optional<at::ScalarType> out_dtype) {
+    need_cuda(x);
+    const auto fn = need(api.fp8_quantize, "actcomp_fp8_quantize");
+    const int dt = dtype_of(x.scalar_type());
+    const actcomp_fp8 dw = fp8_desc(w);
+    const int64_t k = dw.transposed ? dw.rows : dw.cols, n = dw.transposed ? dw.cols : dw.rows;
+    if (x.dim() < 1 || x.size(-1) != k)
+        bad_value("x is " + str(x) + ", the weight has " + std::to_string(k) + " columns");
+    if (x.device() != std::get<2>(w).device()) bad_value("operands on different devices");
+    const Rows r = matrix(x);
+    const int64_t tokens = x.numel() / k;
+    const at::ScalarType dtype = out_dtype.value_or(x.scalar_type());
+    dtype_of(dtype);
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = n;
+    const Fp8Buffers q = empty_fp8(x, tokens, k, ACTCOMP_FP8_E4M3, ACTCOMP_FP8_ROWS);
+    {
+        const c10::cuda::CUDAGuard guard(x.device());
+        check("actcomp_fp8_quantize", fn(ptr(r.t), tokens, k, r.ld, dt, &q.desc, nullptr, stream_of(x)));
+    }
+    return fp8_product(q.desc, dw, x, shape, dtype);
+}
+
+// ---------------------------------------------------------------- cross entropy of a linear layer
+// x as rows that the copies to shared memory can take: 16-byte aligned, with a stride of
+// whole 16 bytes; copied where they are not.
+Rows rows16(const Tensor &x, int64_t cols) {
+    Rows r = rows_of(x, cols);
+    if (reinterpret_cast<uintptr_t>(ptr(r.t)) % 16 == 0 && r.ld % 8 == 0) return r;
+    const int64_t rows = x.numel() / cols, ld = (cols + 7) / 8 * 8;
+    const Tensor t = at::empty({rows, ld}, x.options());
+    t.narrow(1, 0, cols).copy_(r.t.reshape({rows, cols}));
+    return {t, ld};
+}
+struct XentIn {
+    Rows x, w;
+    Tensor target;
+    actcomp_xent_args a;
+    std::vector<int64_t> lead;
+};
+XentIn xent_in(const Tensor &x, const Tensor &weight, const Tensor &target, int64_t ignore_index) {
+    need_cuda(x);
+    if (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kHalf)
+        bad_type(std::string("bfloat16 or float16 expected, got ") + at::toString(x.scalar_type()));
+    if (x.dim() < 1 || x.size(-1) == 0) bad_value("x over an empty last dimension: " + str(x));
+    const int64_t cols = x.size(-1), tokens = x.numel() / cols;
+    if (weight.dim() != 2 || weight.size(1) != cols || weight.size(0) == 0 || weight.scalar_type() != x.scalar_type() ||
+        weight.device() != x.device())
+        bad_value("weight must be (vocabulary, " + std::to_string(cols) + ") with the dtype and device of x (" + str(x) +
+                  "), got " + str(weight));
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    if (target.sizes() != lead || target.scalar_type() != at::kLong || target.device() != x.device())
+        bad_value("target must hold one int64 for each row of x (" + str(x) + "), got " + str(target));
+    const c10::cuda::CUDAGuard guard(x.device());
+    XentIn in{tokens ? rows16(x, cols) : Rows{x, cols}, rows16(weight, cols), target.contiguous(), {},
+              std::vector<int64_t>(lead.begin(), lead.end())};
+    in.a = {tokens, cols, weight.size(0), ptr(in.x.t), in.x.ld, ptr(in.w.t), in.w.ld,
+            static_cast<const int64_t *>(ptr(in.target)), ignore_index, nullptr, nullptr, dtype_of(x.scalar_type()), 0};
+    return in;
+}
+
+std::tuple<Tensor, Tensor> xent(const Tensor &x, const Tensor &weight, const Tensor &target, int64_t ignore_index) {
+    const auto fn = need(api.xent, "actcomp_xent");
+    XentIn in = xent_in(x, weight, target, ignore_index);
+    const Tensor loss = at::empty(in.lead, x.options().dtype(at::kFloat)), lse = at::empty(in.lead, loss.options());
+    const c10::cuda::CUDAGuard guard(x.device());
+    const size_t bytes = need(api.xent_workspace, "actcomp_xent_workspace")(in.a.tokens, in.a.vocab);
+    const Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 1)}, x.options().dtype(at::kByte));
+    in.a.loss = static_cast<float *>(ptr(loss));
+    in.a.lse = static_cast<float *>(ptr(lse));
+    check("actcomp_xent", fn(&in.a, ptr(ws), bytes, stream_of(x)));
+    return {loss, lse};
+}
+
+std::tuple<OptTensor, OptTensor> xent_backward(const Tensor &dloss, const Tensor &x, const Tensor &weight,
+                                               const Tensor &target, const Tensor &lse, const OptTensor &dlse,
+                                               int64_t ignore_index, bool x_grad, bool weight_grad, int64_t piece) {
+    const auto fn = need(api.xent_bwd, "actcomp_xent_bwd");
+    if (!x_grad && !weight_grad) bad_value("no gradient is asked for");
+    if (piece < 0) bad_value("vocab_piece must not be negative");
+    XentIn in = xent_in(x, weight, target, ignore_index);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor d = stats(dloss, in.a.tokens, x, "dloss"), l = stats(lse, in.a.tokens, x, "lse");
+    const OptTensor dl = dlse ? OptTensor(stats(*dlse, in.a.tokens, x, "dlse")) : OptTensor();
+    const OptTensor dx = x_grad ? OptTensor(fresh(x)) : OptTensor();
+    const OptTensor dw = weight_grad ? OptTensor(fresh(weight)) : OptTensor();
+    const size_t bytes = need(api.xent_bwd_workspace, "actcomp_xent_bwd_workspace")(in.a.tokens, in.a.channels,
+                                                                                   in.a.vocab, piece);
+    const Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 1)}, x.options().dtype(at::kByte));
+    in.a.lse = static_cast<float *>(ptr(l));
+    const actcomp_xent_grads g{static_cast<const float *>(ptr(d)), static_cast<const float *>(ptr(dl)), ptr(dx),
+                               in.a.channels, ptr(dw), in.a.channels};
+    check("actcomp_xent_bwd", fn(&in.a, &g, piece, ptr(ws), bytes, stream_of(x)));
+    return {dx, dw};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -414,4 +702,14 @@ PYBIND11_MODULE(_host, m) {
     m.def("matmul", &matmul);
     m.def("linear", &linear);
     m.def("one_kernel", &one_kernel);
+    m.def("rms_norm", &rms_norm);
+    m.def("add_rms_norm", &add_rms_norm);
+    m.def("rms_norm_fp8", &rms_norm_fp8);
+    m.def("rms_norm_backward", &rms_norm_backward);
+    m.def("fp8_quantize", &fp8_quantize);
+    m.def("fp8_dequantize", &fp8_dequantize);
+    m.def("fp8_matmul", &fp8_matmul);
+    m.def("fp8_linear", &fp8_linear);
+    m.def("xent", &xent);
+    m.def("xent_backward", &xent_backward);
 }
