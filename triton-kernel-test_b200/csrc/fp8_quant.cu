@@ -49,12 +49,33 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
     const int n = c >= cols ? 0 : (cols - c < 8 ? (int)(cols - c) : 8);
     constexpr uint32_t TOP = FORMAT == E5M2 ? 15 : 8;
     Raw8<T> raw[NR];
+    if constexpr (!VEC) {  // neighbouring lanes neighbouring values, through shared memory
+        extern __shared__ __align__(16) uint8_t dyn[];
+        T *stage = reinterpret_cast<T *>(dyn);
+        const int left = cols - c0 < 128 ? (int)(cols - c0) : 128;
+        constexpr int PITCH = 128 + 16 / (int)sizeof(T);
+#pragma unroll 4
+        for (int i = warp; i < 128; i += 8) {
+            T v[4];
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-        const int64_t r = r0 + ty + 16 * i;
-        if (r < rows && n == 8 && VEC) raw[i].load_vec(x + r * ldx + c);
-        else if (r < rows && n > 0) raw[i].load(x + r * ldx + c, n);
-        else raw[i].zero();
+            for (int j = 0; j < 4; ++j) {
+                v[j] = T(0.f);
+                if (r0 + i < rows && 32 * j + lane < left) v[j] = x[(r0 + i) * ldx + c0 + 32 * j + lane];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) stage[i * PITCH + 32 * j + lane] = v[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NR; ++i) raw[i].load_vec(stage + (ty + 16 * i) * PITCH + cl);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const int64_t r = r0 + ty + 16 * i;
+            if (r < rows && n == 8) raw[i].load_vec(x + r * ldx + c);
+            else if (r < rows && n > 0) raw[i].load(x + r * ldx + c, n);
+            else raw[i].zero();
+        }
     }
     if constexpr ((MODE & BY_COLS) != 0) {
         constexpr int NW = sizeof(T) == 2 ? 4 : 8;  // words of eight columns' magnitudes
@@ -206,7 +227,14 @@ __global__ void __launch_bounds__(256)
             }
         }
         T *d = out + r * ldo + c;
-        if (VEC && n == 8 && ACT_DCHECK(c + 8 <= ldo)) {
+        if (!VEC) {
+            extern __shared__ __align__(16) uint8_t dyn[];
+            constexpr int PITCH = 128 + 16 / (int)sizeof(T);
+            T *st = reinterpret_cast<T *>(dyn) + lr * PITCH + cl;
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+                reinterpret_cast<uint4 *>(st)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        } else if (n == 8 && ACT_DCHECK(c + 8 <= ldo)) {
 #pragma unroll
             for (int k = 0; k < (int)sizeof(T) / 2; ++k)
                 reinterpret_cast<uint4 *>(d)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
@@ -219,6 +247,25 @@ __global__ void __launch_bounds__(256)
                 }
         }
     }
+    if constexpr (!VEC) {  // neighbouring lanes neighbouring values
+        extern __shared__ __align__(16) uint8_t dyn[];
+        constexpr int PITCH = 128 + 16 / (int)sizeof(T);
+        const T *st = reinterpret_cast<const T *>(dyn);
+        const int lane = tid & 31, left = cols - c0 < 128 ? (int)(cols - c0) : 128;
+        __syncthreads();
+#pragma unroll 4
+        for (int i = tid >> 5; i < 128 && r0 + i < rows; i += 8)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (32 * j + lane < left && ACT_DCHECK(c0 + 32 * j + lane < ldo))
+                    out[(r0 + i) * ldo + c0 + 32 * j + lane] = st[i * PITCH + 32 * j + lane];
+    }
+}
+
+// Shared memory of the forms that go through it.
+template <typename T>
+static constexpr int stage_bytes() {
+    return 128 * (128 * (int)sizeof(T) + 16);
 }
 
 template <typename F>
@@ -270,8 +317,10 @@ extern "C" int actcomp_fp8_quantize(const void *x, int64_t rows, int64_t cols, i
     cudaStream_t st = as_stream(stream);
     return with_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
+        const int smem = vec ? 0 : stage_bytes<T>();
         auto go = [&](auto k) -> int {
-            k<<<grid, 256, 0, st>>>(static_cast<const T *>(x), rows, cols, ldx, a, b);
+            if (int rc = allow_smem(k, smem + 6 * 1024, stage_bytes<T>())) return rc;
+            k<<<grid, 256, smem, st>>>(static_cast<const T *>(x), rows, cols, ldx, a, b);
             return launch_status();
         };
         auto pick = [&](auto fmt) -> int {
@@ -298,8 +347,10 @@ extern "C" int actcomp_fp8_dequantize(const actcomp_fp8 *q, void *out, int64_t l
     cudaStream_t st = as_stream(stream);
     return with_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
+        const int smem = vec ? 0 : stage_bytes<T>();
         auto go = [&](auto k) -> int {
-            k<<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols, q->ld, q->block, static_cast<T *>(out), ldo);
+            if (int rc = allow_smem(k, smem, stage_bytes<T>())) return rc;
+            k<<<grid, 256, smem, st>>>(q->codes, q->scales, q->rows, q->cols, q->ld, q->block, static_cast<T *>(out), ldo);
             return launch_status();
         };
         if (q->format == E4M3) return vec ? go(dequant_kernel<T, true, E4M3>) : go(dequant_kernel<T, false, E4M3>);

@@ -205,7 +205,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         *abort = 0;
         tc::fence_mbar_init();
     }
+    if (threadIdx.x == 32) {
+        tc::prefetch_tmap(&tmA);
+        tc::prefetch_tmap(&tmB);
+    }
     if (warp == 1) {
+        __syncwarp();
         tc::tmem_alloc_pair(tmem_slot, 512);
         tc::tmem_relinquish_pair();
     }
@@ -214,10 +219,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tc::cluster_sync();
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    // Launched with programmatic dependence: what is above runs beside the end of the
+    // kernel before, nothing in memory is touched before it has ended.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     if (warp == 0 && lane == 0) {
-        tc::prefetch_tmap(&tmA);
-        tc::prefetch_tmap(&tmB);
         constexpr int BK = KIND == FP8 ? 128 : 64;  // values of a stage
         int s = 0;
         uint32_t phase = 1;
@@ -353,44 +359,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         tc::bulk_wait<0>();
     } else if (KIND == FP8 && warp >= 6) {
         const uint32_t quad = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        int it = 0;
-        bool ok = true;
-        for (int t = cluster; t < tiles && ok; t += clusters) {
-            const Tile tl = tile_of(t, p);
+        constexpr int AHEAD = 4;  // stages whose words are on their way together
+        // the words of stages k0 .. of tile t, past its last one those of the last
+        auto fetch = [&](uint32_t (&w)[AHEAD][3], const Tile &tl, int k0) {
             const int ga = tl.m * 2 + (int)rank, gb = tl.n * 2;
-            constexpr int AHEAD = 4;  // stages whose words are on their way together
-            for (int kb0 = tl.k0; kb0 < tl.k1 && ok; kb0 += AHEAD) {
-                uint32_t w[AHEAD][3];
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const int kb = kb0 + i < tl.k1 ? kb0 + i : kb0;
-                    w[i][0] = scale_word(p.sa, kb, ga, lane);
-                    w[i][1] = scale_word(p.sb, kb, gb, lane);
-                    w[i][2] = scale_word(p.sb, kb, gb + 1, lane);
-                }
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    if (kb0 + i >= tl.k1 || !ok) break;
-                    // the set's earlier MMAs are done
-                    if (it >= SETS &&
-                        !(ok = tc::mbar_spin(&empty[(it - SETS) % STAGES], ((it - SETS) / STAGES) & 1, abort)))
-                        break;
-                    tc::tc_fence_after();
-                    uint32_t u[8];
-                    const uint32_t d = quad + L::SF0 + it % SETS * SF_STEP;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) u[j] = w[i][0] >> (8 * j), u[4 + j] = w[i][1] >> (8 * j);
-                    tc::tmem_st8(d, u);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) u[j] = w[i][2] >> (8 * j);
-                    tc::tmem_st4(d + 8, u);
-                    tc::tmem_st_wait();
-                    tc::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive_remote_tmem(tc::map_cluster(&full[it % STAGES], 0));
-                    ++it;
-                }
+            for (int i = 0; i < AHEAD; ++i) {
+                const int kb = k0 + i < tl.k1 ? k0 + i : tl.k1 - 1;
+                w[i][0] = scale_word(p.sa, kb, ga, lane);
+                w[i][1] = scale_word(p.sb, kb, gb, lane);
+                w[i][2] = scale_word(p.sb, kb, gb + 1, lane);
             }
+        };
+        int it = 0, t = cluster;
+        bool ok = t < tiles;
+        Tile tl = tile_of(ok ? t : 0, p);
+        int k0 = tl.k0;
+        uint32_t next[AHEAD][3];
+        if (ok) fetch(next, tl, k0);
+        while (ok) {
+            uint32_t w[AHEAD][3];
+            memcpy(w, next, sizeof(w));
+            const int n = tl.k1 - k0 < AHEAD ? tl.k1 - k0 : AHEAD;
+            // the words after these are asked for before these are needed
+            bool more = true;
+            if ((k0 += AHEAD) >= tl.k1) {
+                if ((more = (t += clusters) < tiles)) tl = tile_of(t, p), k0 = tl.k0;
+            }
+            if (more) fetch(next, tl, k0);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                if (i >= n) break;
+                // the set's earlier MMAs are done
+                if (it >= SETS &&
+                    !(ok = tc::mbar_spin(&empty[(it - SETS) % STAGES], ((it - SETS) / STAGES) & 1, abort)))
+                    break;
+                tc::tc_fence_after();
+                uint32_t u[8];
+                const uint32_t d = quad + L::SF0 + it % SETS * SF_STEP;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u[j] = w[i][0] >> (8 * j), u[4 + j] = w[i][1] >> (8 * j);
+                tc::tmem_st8(d, u);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u[j] = w[i][2] >> (8 * j);
+                tc::tmem_st4(d + 8, u);
+                tc::tmem_st_wait();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive_remote_tmem(tc::map_cluster(&full[it % STAGES], 0));
+                ++it;
+            }
+            if (!more) break;
         }
     }
     tc::tc_fence_before();
@@ -434,8 +453,18 @@ static int launch(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensor
     auto kern = pair_kernel<KIND, Epi>;
     ACT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     const int tiles = p.m_tiles * p.n_tiles * p.splits, pairs = max_pairs(kern);
-    kern<<<2 * (tiles < pairs ? tiles : pairs), THREADS, SMEM, st>>>(tmA, tmB, tmC, p, ep);
-    return launch_status();
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs)));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    ACT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmC, p, ep));
+    return ACT_OK;
 }
 
 }  // namespace pair
