@@ -565,7 +565,7 @@ int actcomp_mx4_linear(const void *x, int64_t tokens, int64_t cols, int64_t ldx,
 #define ACTCOMP_FP8_ROWS 0
 #define ACTCOMP_FP8_COLS 1
 #define ACTCOMP_FP8_TILES 2
-#define ACTCOMP_FP8_FEW_TOKENS 32 /* rows of a up to which a product takes the few-token kernel */
+#define ACTCOMP_FP8_FEW_TOKENS 128 /* rows of a up to which a product takes the few-token kernel */
 typedef struct actcomp_fp8 {
     int64_t rows, cols, ld;
     uint8_t *codes;

@@ -1,241 +1,316 @@
-// fp8_few.cu -- x . w^T for a few tokens in 8-bit floating point.
+// fp8_few.cu -- the product of two 8-bit matrices of which the first has few rows (a
+// batch of tokens being served against a weight): C = X . W^T with the weight's rows as
+// the tensor cores' M.
 //
-// It cannot do without the weight's byte a value, read once: 256-row tiles of the
-// tensor cores would be nearly empty and there are too few of them to keep all of
-// memory busy.  Here a warp takes 16 rows of the weight and a share of the contraction,
-// and multiplies on the warp's own matrix instruction (m16n8k32, float32 accumulation):
-// no code is decoded, and eight tokens cost what one does.
-//   A lane brings 16 consecutive codes of a row at a time (four lanes 64 bytes); the
-// order in which an instruction's steps take them is the same for both operands, and
-// of no consequence.  A block of 128 is four instructions from zero, whose sum is
-// scaled and added in float32.
-//   The warps of a CTA share rows and split their blocks (KS), so that all loads of a
-// warp are under way at once; their sums meet in shared memory in a fixed order.
+// It cannot do without the weight's byte a value, read once.  The tiles of 256 x 256
+// (fp8_gemm.cu) would be mostly empty and too few to keep memory busy: 200 x 4096 x
+// 11008 has 43.  Here a CTA takes 128 rows of the weight against all tokens (the MMA's N is
+// their number rounded to 16), and the contraction is cut over a cluster of up
+// to eight CTAs, so that the device has two to four CTAs per SM; their sums meet in
+// shared memory, each CTA adding some of the tokens' columns in the order of the ranks.  Per CTA:
+//   warp 0      TMA producer: 128 rows x 128 of W, N x 128 of X a stage;
+//   warp 1      TMEM allocation, MMA issue;
+//   warps 2..5  scales from memory to TMEM, every lane quadrant the same (as in
+//               pair_gemm.cuh), then the sums.
+// Tokens on the M side, decoded codes on the warps' own matrix instruction, took 22 us
+// for one token (4096 x 11008): the instruction is made of conversions and 16-bit steps.
 #include <algorithm>
 
-#include "fp8.cuh"
+#include "pair_gemm.cuh"
 
 namespace act {
 namespace fp8 {
 
-struct FewArgs {
-    const uint8_t *x, *w;
-    const uint8_t *xs, *ws;
+constexpr int FEW_THREADS = 192;
+constexpr int W_BYTES = 128 * 128;  // of a stage
+constexpr int FEW_SETS = 8, SET_COLS = 8;  // scale sets in TMEM: 128 rows of W, up to 128 tokens
+constexpr int MOST_N = ACTCOMP_FP8_FEW_TOKENS;
+// Accumulators that the steps take in turn, so that one waits less for the step before it.
+__host__ __device__ constexpr int accumulators(int n) { return n <= 48 ? 4 : n <= 96 ? 2 : 1; }
+__host__ __device__ constexpr int columns(int n) { return n * accumulators(n) + FEW_SETS * SET_COLS; }
+// TMEM is asked for by CTAs that others of their cluster wait for: it must never be what a resident CTA waits for
+// (two launches beside each other could wait for each other's).  So a CTA takes as large a part of the SM's shared
+// memory as of its TMEM: 228 KB over 512 columns.
+__host__ __device__ constexpr int few_smem(int tmem_cols) { return tmem_cols * (228 * 1024 / 512) - 1024; }
+
+static_assert(columns(16) <= 128 && columns(48) <= 256 && columns(96) <= 256 && columns(MOST_N) <= 256, "TMEM");
+static_assert((few_smem(128) - 1536) / (W_BYTES + 16 * 128) >= 3 && (few_smem(256) - 1536) / (W_BYTES + MOST_N * 128) >= 3,
+              "stages");
+
+struct FewParams {
+    int tokens, n;        // rows of X and of W
+    int kblocks, k_split;  // blocks of 128 of the contraction, and of a rank
+    int N, accs;           // the MMA's N, and accumulators
+    int w_mn;              // whether W lies with its rows contiguous
+    uint32_t idesc;
+    int stages, tmem_cols;
+    pair::Scales sw, sx;
     void *c;
-    int64_t ldx, ldw, ldc;
-    int tokens, n, k;
-    int x_groups;        // of 128 tokens' scales (ROWS)
-    int64_t ws_k;        // bytes from a block of the contraction to the next
-    int ws_g, ws_lines;  // from 128 rows to the next; whether a scale belongs to a row (else to 128)
-    int ks_log;          // log2 of the warps that share rows
+    int64_t ldc;
 };
 
-template <int FX, int FW>
-__device__ __forceinline__ void mma_k32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-#define ACT_FP8_MMA(A, B)                                                                                              \
-    asm("mma.sync.aligned.m16n8k32.row.col.f32." A "." B                                                               \
-        ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"                                         \
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                               \
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
-    if constexpr (FW == E4M3 && FX == E4M3) ACT_FP8_MMA("e4m3", "e4m3");
-    else if constexpr (FW == E4M3) ACT_FP8_MMA("e4m3", "e5m2");
-    else if constexpr (FX == E4M3) ACT_FP8_MMA("e5m2", "e4m3");
-    else ACT_FP8_MMA("e5m2", "e5m2");
-#undef ACT_FP8_MMA
-}
+template <typename TOut>
+__global__ void __launch_bounds__(FEW_THREADS)
+    few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+               const __grid_constant__ FewParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
+    const int stage_bytes = W_BYTES + p.N * 128, stages = p.stages;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + stages * stage_bytes);
+    uint64_t *empty = full + stages, *set_full = empty + stages, *set_free = set_full + FEW_SETS,
+             *acc_full = set_free + FEW_SETS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_full + 1);
+    volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    uint32_t ranks, rank;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;\n mov.u32 %1, %%cluster_ctarank;" : "=r"(ranks), "=r"(rank));
+    const int tile = blockIdx.x / (int)ranks;
+    const int k0 = (int)rank * p.k_split, k1 = min(k0 + p.k_split, p.kblocks), steps = k1 > k0 ? k1 - k0 : 0;
 
-// n of 16 codes at p (16-byte aligned, all there to read where n > 0), the others 0.
-__device__ __forceinline__ uint4 load16(const uint8_t *p, int n) {
-    if (n <= 0) return make_uint4(0, 0, 0, 0);
-    uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
-    if (n < 16) {
-        uint32_t *w = reinterpret_cast<uint32_t *>(&q);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int left = n - 4 * i;
-            w[i] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            tc::mbar_init(&full[s], 1);
+            tc::mbar_init(&empty[s], 1);
         }
+        // The scales have barriers of their own: there are more sets than stages, so that their warps may be further
+        // ahead than the producer, whose barriers they must not arrive on then.
+        for (int s = 0; s < FEW_SETS; ++s) {
+            tc::mbar_init(&set_full[s], 4);
+            tc::mbar_init(&set_free[s], 1);
+        }
+        tc::mbar_init(acc_full, 1);
+        *abort = 0;
+        tc::fence_mbar_init();
+        tc::prefetch_tmap(&tmW);
+        tc::prefetch_tmap(&tmX);
     }
-    return q;
-}
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-
-constexpr int FEW_WARPS = 8, THREADS = 32 * FEW_WARPS;
-constexpr int X_ROOM = 96 * 1024;  // shared memory for x: two CTAs per SM
-// A token's codes in shared memory: whole blocks, and 64 bytes, so that the eight lanes of a quarter warp
-// (two tokens, four pieces of 16 bytes) meet all banks.
-__host__ __device__ __forceinline__ int x_pitch(int k) { return (k + 127) / 128 * 128 + 64; }
-
-// NT: groups of eight tokens.
-template <typename TOut, int NT, int FX, int FW>
-__global__ void __launch_bounds__(THREADS, 2) few_kernel(const __grid_constant__ FewArgs a) {
-    extern __shared__ __align__(16) uint8_t xs[];  // tokens x pitch codes, then blocks x 8 NT scales
-    __shared__ float part[FEW_WARPS][NT][4][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int ks = 1 << a.ks_log, mine = warp & (ks - 1), per = FEW_WARPS >> a.ks_log;
-    const int g = lane >> 2, q = lane & 3;
-    const int blocks = (a.k + 127) / 128, pitch = x_pitch(a.k);
-    float *xf = reinterpret_cast<float *>(xs + a.tokens * pitch);
-    const int sets = (a.n + 15) / 16, turns = (sets + per - 1) / per;
+    if (warp == 1) {
+        tc::tmem_alloc(tmem_slot, p.tmem_cols);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    // launched with programmatic dependence (see pair_gemm.cuh)
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    constexpr int UNROLL = NT == 1 ? 4 : 2;  // blocks of a warp on their way together (registers)
-    uint4 w[UNROLL][4];  // row, half of the block
-    uint32_t sc[UNROLL][2];
-    auto fetch = [&](int turn, int b0) {
-        const int64_t r0 = ((int64_t)turn * per + (warp >> a.ks_log)) * 16, ra = r0 + g, rb = ra + 8;
-        const uint8_t *wa = a.w + ra * a.ldw + 16 * q, *wb = wa + 8 * a.ldw;
-        const uint8_t *sa = a.ws + (r0 >> 7) * a.ws_g, *sb = sa;
-        if (a.ws_lines) sa += (ra & 31) * 4 + ((ra >> 5) & 3), sb += (rb & 31) * 4 + ((rb >> 5) & 3);
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int b = b0 + u * ks;
-            if (b < blocks && 128 * b + 128 <= a.k && r0 + 16 <= a.n) {  // a whole block of whole rows
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    w[u][h] = __ldg(reinterpret_cast<const uint4 *>(wa + 128 * b + 64 * h));
-                    w[u][2 + h] = __ldg(reinterpret_cast<const uint4 *>(wb + 128 * b + 64 * h));
-                }
-                sc[u][0] = __ldg(sa + b * a.ws_k);
-                sc[u][1] = a.ws_lines ? __ldg(sb + b * a.ws_k) : sc[u][0];
-            } else {
-                const int left = b < blocks ? a.k - 128 * b - 16 * q : 0;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    w[u][h] = load16(wa + 128 * b + 64 * h, ra < a.n ? left - 64 * h : 0);
-                    w[u][2 + h] = load16(wb + 128 * b + 64 * h, rb < a.n ? left - 64 * h : 0);
-                }
-                sc[u][0] = b < blocks && ra < a.n ? __ldg(sa + b * a.ws_k) : 0u;
-                sc[u][1] = b < blocks && rb < a.n ? __ldg(sb + b * a.ws_k) : 0u;
+    const int sets = p.accs * p.N;  // TMEM column of the scale sets
+    bool ok = true;
+    if (warp == 0 && lane == 0) {
+        int s = 0;
+        uint32_t phase = 1;
+        for (int i = 0; i < steps; ++i) {
+            if (!(ok = tc::mbar_spin(&empty[s], phase, abort))) break;
+            uint8_t *w = smem + s * stage_bytes;
+            const int k = (k0 + i) * 128;
+            tc::mbar_arrive_expect_tx(&full[s], stage_bytes);
+            if (p.w_mn) tc::tma_load_3d(w, &tmW, &full[s], tile * 128, k, 0);
+            else tc::tma_load_3d(w, &tmW, &full[s], k, tile * 128, 0);
+            tc::tma_load_3d(w + W_BYTES, &tmX, &full[s], k, 0, 0);
+            if (++s == stages) s = 0, phase ^= 1;
+        }
+    } else if (warp == 1) {
+        // What this loop takes a block when nothing is waited for (300 cycles; with divisions for the stage and
+        // sleeping waits 750) is most of a short contraction's time.
+        const uint64_t desc_w = tc::smem_desc(smem, p.w_mn ? 8192 : 16, 1024, tc::SW_128B);
+        const uint64_t desc_x = tc::smem_desc(smem + W_BYTES, 16, 1024, tc::SW_128B);
+        const uint32_t step = p.w_mn ? 32 * 128 / 16 : 2, d1 = tmem + (p.accs > 1 ? p.N : 0),
+                       d2 = tmem + (p.accs > 2 ? 2 * p.N : 0), d3 = tmem + (p.accs - 1) * p.N;
+        int s = 0, set = 0;
+        uint32_t phase = 0, set_phase = 0;
+        for (int i = 0; i < steps; ++i) {
+            if (!(ok = tc::mbar_spin(&set_full[set], set_phase, abort))) break;
+            if (!(ok = tc::mbar_spin(&full[s], phase, abort))) break;
+            tc::tc_fence_after();
+            const uint64_t da = desc_w + (uint32_t)(s * (stage_bytes / 16)), db = desc_x + (uint32_t)(s * (stage_bytes / 16));
+            const uint32_t sf = tmem + sets + set * SET_COLS;
+            if (tc::elect_one()) {
+                // a step into each accumulator in turn: the first of each starts it
+                tc::mma_mxf8(tmem, da, db, p.idesc, sf, sf + 4, i > 0);
+                tc::mma_mxf8(d1, da + step, db + 2, p.idesc, sf, sf + 4, i > 0 || p.accs < 2);
+                tc::mma_mxf8(d2, da + 2 * step, db + 4, p.idesc, sf, sf + 4, i > 0 || p.accs < 4);
+                tc::mma_mxf8(d3, da + 3 * step, db + 6, p.idesc, sf, sf + 4, i > 0 || p.accs < 4);
+                if (i + stages < steps) tc::mma_commit(&empty[s]);
+                if (i + FEW_SETS < steps) tc::mma_commit(&set_free[set]);
             }
+            __syncwarp();
+            if (++s == stages) s = 0, phase ^= 1;
+            if (++set == FEW_SETS) set = 0, set_phase ^= 1;
+        }
+        if (tc::elect_one()) tc::mma_commit(acc_full);
+        __syncwarp();
+    } else if (warp >= 2) {
+        const uint32_t quad = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        constexpr int AHEAD = 4;  // blocks whose words are on their way, and written, together
+        uint32_t next[AHEAD][2];
+        auto fetch = [&](int i0) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int kb = min(k0 + i0 + i, p.kblocks - 1);
+                next[i][0] = pair::scale_word(p.sw, kb, tile, lane);
+                next[i][1] = pair::scale_word(p.sx, kb, 0, lane);
+            }
+        };
+        if (steps > 0) fetch(0);
+        for (int i0 = 0; i0 < steps && ok; i0 += AHEAD) {
+            uint32_t w[AHEAD][2];
+            memcpy(w, next, sizeof(w));
+            if (i0 + AHEAD < steps) fetch(i0 + AHEAD);
+            // several blocks' words at once: the stores' latency, not their number, is what a turn here takes
+            const int n = min(AHEAD, steps - i0);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int it = i0 + i;
+                if (i >= n) break;
+                // the set's earlier MMAs are done
+                if (it >= FEW_SETS &&
+                    !(ok = tc::mbar_spin(&set_free[it % FEW_SETS], (it / FEW_SETS - 1) & 1, abort)))
+                    break;
+                tc::tc_fence_after();
+                uint32_t u[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u[j] = w[i][0] >> (8 * j), u[4 + j] = w[i][1] >> (8 * j);
+                tc::tmem_st8(quad + sets + it % FEW_SETS * SET_COLS, u);
+            }
+            tc::tmem_st_wait();
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane < n && ok) tc::mbar_arrive(&set_full[(i0 + lane) % FEW_SETS]);
+            __syncwarp();
+        }
+        ok = ok && tc::mbar_spin(acc_full, 0, abort);
+        tc::tc_fence_after();
+    }
+
+    // a thread's row of the weight, sums of N tokens in TMEM
+    const int row = (warp & 3) * 32 + lane, out_row = tile * 128 + row;
+    TOut *c = static_cast<TOut *>(p.c) + out_row;
+    const uint32_t acc = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    auto sums16 = [&](uint32_t acc, int g, uint32_t (&r)[16]) {  // of tokens g .., over the accumulators
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[i] = 0u;
+        if (steps == 0) return;
+        tc::tmem_ld16(acc + g, r);
+        for (int k = 1; k < p.accs; ++k) {
+            uint32_t q[16];
+            tc::tmem_ld16(acc + k * p.N + g, q);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(q[i]));
         }
     };
-    int turn = blockIdx.x;
-    fetch(turn, mine);
-    // x while the first codes of w are on their way
-    for (int i = threadIdx.x; i < a.tokens * blocks * 8; i += THREADS) {
-        const int tok = i / (blocks * 8), c = i - tok * blocks * 8;
-        *reinterpret_cast<uint4 *>(xs + tok * pitch + 16 * c) = load16(a.x + tok * a.ldx + 16 * c, a.k - 16 * c);
-    }
-    for (int i = threadIdx.x; i < blocks * 8 * NT; i += THREADS) {
-        const int b = i / (8 * NT), tok = i - b * 8 * NT;
-        xf[i] = scale_value(tok < a.tokens ? __ldg(a.xs + (int64_t)b * a.x_groups * 128 + (tok & 31) * 4 + (tok >> 5)) : 0u);
-    }
-    __syncthreads();
-    for (; turn < turns; turn += gridDim.x) {
-        float sum[NT][4];
+    if (ranks == 1) {
+        if (warp >= 2 && ok) {
+#pragma unroll 1
+            for (int g = 0; g < p.N; g += 16) {
+                uint32_t r[16];
+                sums16(acc, g, r);
+                if (out_row < p.n) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[t][i] = 0.f;
-        for (int b0 = mine; b0 < blocks; b0 += UNROLL * ks) {
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                const int b = b0 + u * ks;
-                if (b >= blocks) break;
-                const float fa = scale_value(sc[u][0]), fb = scale_value(sc[u][1]);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const uint8_t *xp = xs + (8 * t + g) * pitch + 128 * b + 16 * q;
-                    float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint4 x = 8 * t + g < a.tokens ? *reinterpret_cast<const uint4 *>(xp + 64 * h)
-                                                             : make_uint4(0, 0, 0, 0);
-                        const uint4 &p = w[u][h], &r = w[u][2 + h];
-                        mma_k32<FX, FW>(d, p.x, r.x, p.y, r.y, x.x, x.y);
-                        mma_k32<FX, FW>(d, p.z, r.z, p.w, r.w, x.z, x.w);
-                    }
-                    // columns of the result: tokens 8 t + 2 q and the next
-                    const float2 f = *reinterpret_cast<const float2 *>(xf + (b * NT + t) * 8 + 2 * q);
-                    sum[t][0] = __fmaf_rn(d[0] * fa, f.x, sum[t][0]);
-                    sum[t][1] = __fmaf_rn(d[1] * fa, f.y, sum[t][1]);
-                    sum[t][2] = __fmaf_rn(d[2] * fb, f.x, sum[t][2]);
-                    sum[t][3] = __fmaf_rn(d[3] * fb, f.y, sum[t][3]);
+                    for (int i = 0; i < 16; ++i)
+                        if (g + i < p.tokens && ACT_DCHECK(out_row < p.ldc))
+                            c[(int64_t)(g + i) * p.ldc] = pair::cvt_out<TOut>(__uint_as_float(r[i]));
                 }
             }
-            if (b0 + UNROLL * ks < blocks) fetch(turn, b0 + UNROLL * ks);
         }
-        if (turn + (int)gridDim.x < turns) fetch(turn + gridDim.x, mine);
+    } else {
+        // Columns first .. first + each - 1 are this rank's to add.  The sums go to their ranks' shared memory, over
+        // the rings once every rank is done with its own: [rank][column][row].
+        const int each = p.N / (int)ranks;
+        __syncwarp();
+        tc::cluster_sync();
+        if (warp >= 2) {
+#pragma unroll 1
+            for (int g = 0; g < p.N; g += 16) {
+                uint32_t r[16];
+                sums16(acc, g, r);
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part[warp][t][i][lane] = sum[t][i];
-        __syncthreads();
-        // the CTA's rows x tokens, neighbouring threads neighbouring rows
-        const int rows = 16 * per;
-        const int64_t first = (int64_t)turn * rows;
-        for (int e = threadIdx.x; e < rows * a.tokens; e += THREADS) {
-            const int tok = e / rows, r = e - tok * rows, set = r >> 4, lr = r & 15;
-            if (first + r >= a.n) continue;
-            // the accumulator's place: row lr & 7 by lane / 4, the upper eight rows two registers on
-            const int i = (lr >> 3) * 2 + (tok & 1), l = (lr & 7) * 4 + ((tok & 7) >> 1);
-            float s = 0.f;
-            for (int j = 0; j < ks; ++j) s += part[(set << a.ks_log) + j][tok >> 3][i][l];
-            if (ACT_DCHECK(tok < a.tokens && first + r < a.ldc))
-                static_cast<TOut *>(a.c)[tok * a.ldc + first + r] = from_f<TOut>(s);
+                for (int i = 0; i < 16; ++i) {
+                    const int to = (g + i) / each, col = g + i - to * each;
+                    const float v = ok ? __uint_as_float(r[i]) : __uint_as_float(0x7fc00000u);
+                    tc::st_cluster_f32(tc::map_cluster(smem, to) + (uint32_t)((((int)rank * each + col) * 128 + row) * 4), v);
+                }
+            }
         }
-        __syncthreads();
+        __syncwarp();
+        tc::cluster_sync();
+        if (warp >= 2 && out_row < p.n) {
+            const float *in = reinterpret_cast<const float *>(smem) + row;
+            for (int col = 0; col < each; ++col) {
+                const int tok = (int)rank * each + col;
+                if (tok >= p.tokens) break;
+                float s = in[col * 128];
+                for (int k = 1; k < (int)ranks; ++k) s += in[(k * each + col) * 128];
+                if (ACT_DCHECK(out_row < p.ldc)) c[(int64_t)tok * p.ldc] = pair::cvt_out<TOut>(s);
+            }
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, p.tmem_cols);
     }
 }
 
-// Whether the product a . b^T goes through the kernel above: few tokens by rows that fit
-// shared memory, and a weight whose rows lie along the contraction.
-bool few_takes(const actcomp_fp8 *a, const actcomp_fp8 *b) {
-    return a->block == ROWS && !b->transposed && a->rows <= ACTCOMP_FP8_FEW_TOKENS && b->cols <= X_ROOM &&
-           a->rows * x_pitch((int)b->cols) <= X_ROOM;
-}
+// Whether the product a . b^T goes through the kernel above: a's rows are few and lie
+// along the contraction.
+bool few_takes(const actcomp_fp8 *a) { return !a->transposed && a->rows <= ACTCOMP_FP8_FEW_TOKENS; }
 
-int few_launch(const actcomp_fp8 *a, const actcomp_fp8 *b, void *c, int64_t ldc, int c_dtype, cudaStream_t st) {
-    FewArgs f{a->codes, b->codes, a->scales, b->scales, c, a->ld, b->ld, ldc, (int)a->rows, (int)b->rows, (int)b->cols,
-              (int)blocks_of(a->rows), 0, 0, 0, 0};
-    f.ws_lines = b->block == ROWS;
-    f.ws_k = f.ws_lines ? blocks_of(b->rows) * 128 : 1;
-    f.ws_g = f.ws_lines ? 128 : (int)blocks_of(b->cols);
-    // Enough warps for the device, as far as there are blocks to share.
-    const int64_t sets = (b->rows + 15) / 16, want = (int64_t)num_sms() * 2 * FEW_WARPS, blocks = blocks_of(b->cols);
-    while (f.ks_log < 3 && sets << f.ks_log < want && (2 << f.ks_log) <= blocks) ++f.ks_log;
-    const int64_t per = FEW_WARPS >> f.ks_log, turns = (sets + per - 1) / per;
-    const int nt = a->rows <= 8 ? 1 : a->rows <= 16 ? 2 : 4;
-    const int smem = (int)a->rows * x_pitch(f.k) + (int)blocks * nt * 8 * 4;
-    const int most = X_ROOM + (X_ROOM / 128 + 1) * 4 * 8 * 4;
-    const int64_t cap = (int64_t)num_sms() * 2;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
+int few_launch(const actcomp_fp8 *a, const actcomp_fp8 *b, const pair::Scales &sa, const pair::Scales &sb, void *c,
+               int64_t ldc, int c_dtype, cudaStream_t st) {
+    FewParams p{};
+    p.tokens = (int)a->rows;
+    p.n = (int)(b->transposed ? b->cols : b->rows);
+    p.kblocks = (int)blocks_of(a->cols);
+    p.N = (p.tokens + 15) / 16 * 16;
+    p.accs = accumulators(p.N);
+    p.w_mn = b->transposed;
+    p.idesc = tc::idesc_mxf8(128, p.N, b->format == E5M2, a->format == E5M2, p.w_mn, false);
+    p.sw = sb, p.sx = sa;
+    p.c = c, p.ldc = ldc;
+    p.tmem_cols = p.N == 16 ? 128 : 256;  // four or two CTAs per SM
+    const int stage = W_BYTES + p.N * 128, smem = few_smem(p.tmem_cols), sms = num_sms(), per_sm = 512 / p.tmem_cols;
+    p.stages = (smem - 1024 - 512) / stage;
+    // Ranks by an estimate in blocks of 0.35 us: an SM's share of the CTAs at a CTA's blocks each, and 20 for every
+    // wave's start, first loads and sums.  us (a weight in memory) at 1 | 2 | 4 | 8 ranks: 11008 x 4096, 1 token
+    // 21.3 | 18.5 | 16.4 | 20.5, 64 tokens 22.5 | 24.5 | 30.7 | 36.9; 4096 x 11008, 1 token 38.8 | 26.5 | 20.5 | 18.5.
+    const int64_t units = (p.n + 127) / 128;
+    int ranks = 1;
+    int64_t best = INT64_MAX;
+    for (int r = 1; r <= 8 && (r == 1 || p.kblocks >= 2 * r); r *= 2) {
+        const int64_t ctas = units * r, blocks = (p.kblocks + r - 1) / r;
+        const int64_t cost = (ctas + sms - 1) / sms * blocks + 20 * ((ctas + sms * per_sm - 1) / (sms * per_sm));
+        if (cost < best) best = cost, ranks = r;
+    }
+    p.k_split = (p.kblocks + ranks - 1) / ranks;
+    ACT_CHECK(units * ranks <= INT32_MAX, ACT_E_UNSUPPORTED);
+    CUtensorMap tmW, tmX;
+    if (int rc = make_map_3d(&tmW, b->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b->cols, b->rows, 1, b->ld, 0, 128, 128,
+                             CU_TENSOR_MAP_SWIZZLE_128B))
+        return rc;
+    if (int rc = make_map_3d(&tmX, a->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a->cols, a->rows, 1, a->ld, 0, 128, p.N,
+                             CU_TENSOR_MAP_SWIZZLE_128B))
+        return rc;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim = {(unsigned)ranks, 1, 1};
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(turns < cap ? turns : cap));
-    cfg.blockDim = dim3(THREADS);
+    cfg.gridDim = dim3((unsigned)(units * ranks));
+    cfg.blockDim = dim3(FEW_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    auto go = [&](auto out, auto n, auto fx, auto fw) -> int {
-        auto k = few_kernel<decltype(out), decltype(n)::value, decltype(fx)::value, decltype(fw)::value>;
-        ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-        ACT_CUDA_TRY(cudaLaunchKernelEx(&cfg, k, f));
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    auto go = [&](auto out) -> int {
+        auto k = few_kernel<decltype(out)>;
+        ACT_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem(256)));
+        ACT_CUDA_TRY(cudaLaunchKernelEx(&cfg, k, tmW, tmX, p));
         return ACT_OK;
     };
-    auto by_format = [&](auto out, auto n) -> int {
-        const std::integral_constant<int, E4M3> e4;
-        const std::integral_constant<int, E5M2> e5;
-        if (a->format == E4M3) return b->format == E4M3 ? go(out, n, e4, e4) : go(out, n, e4, e5);
-        return b->format == E4M3 ? go(out, n, e5, e4) : go(out, n, e5, e5);
-    };
-    auto by_tokens = [&](auto out) -> int {
-        if (nt == 1) return by_format(out, std::integral_constant<int, 1>{});
-        if (nt == 2) return by_format(out, std::integral_constant<int, 2>{});
-        return by_format(out, std::integral_constant<int, 4>{});
-    };
-    return c_dtype == 0 ? by_tokens(float{}) : c_dtype == 1 ? by_tokens(__nv_bfloat16{}) : by_tokens(__half{});
+    return c_dtype == 0 ? go(float{}) : c_dtype == 1 ? go(__nv_bfloat16{}) : go(__half{});
 }
 
 }  // namespace fp8

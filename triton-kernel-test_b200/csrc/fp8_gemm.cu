@@ -14,8 +14,9 @@ namespace act {
 namespace fp8 {
 
 int check(const actcomp_fp8 *q);  // fp8_quant.cu
-bool few_takes(const actcomp_fp8 *a, const actcomp_fp8 *b);  // fp8_few.cu
-int few_launch(const actcomp_fp8 *a, const actcomp_fp8 *b, void *c, int64_t ldc, int c_dtype, cudaStream_t st);
+bool few_takes(const actcomp_fp8 *a);  // fp8_few.cu
+int few_launch(const actcomp_fp8 *a, const actcomp_fp8 *b, const pair::Scales &sa, const pair::Scales &sb, void *c,
+               int64_t ldc, int c_dtype, cudaStream_t st);
 
 template <typename TOut>
 struct StoreEpi {
@@ -68,7 +69,7 @@ extern "C" int actcomp_fp8_gemm(const actcomp_fp8 *a, const actcomp_fp8 *b, void
     ACT_CHECK(va.k == vb.k && c && ldc >= vb.lines && c_dtype >= 0 && c_dtype <= 2, ACT_E_INVALID);
     const int es = c_dtype == 0 ? 4 : 2;
     ACT_CHECK(aligned(c, es), ACT_E_ALIGN);
-    if (few_takes(a, b)) return few_launch(a, b, c, ldc, c_dtype, as_stream(stream));
+    if (few_takes(a)) return few_launch(a, b, scales_of(a), scales_of(b), c, ldc, c_dtype, as_stream(stream));
     pair::Params p{};
     pair::set_tiles(p, (int)va.lines, (int)vb.lines, (int)blocks_of(va.k));
     ACT_CHECK((int64_t)p.m_tiles * p.n_tiles <= INT32_MAX, ACT_E_UNSUPPORTED);

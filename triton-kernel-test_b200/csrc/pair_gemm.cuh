@@ -11,7 +11,7 @@
 //   warps 2..5  epilogue, one accumulator row a thread (class Epi);
 //   warps 6..9  16-bit operands: epilogue too, the other 128 columns;
 //               8-bit operands: scales from memory to TMEM, every lane quadrant the
-//               same, five sets of 12 columns in turn; a set is written again only
+//               same, eight sets of 12 columns in turn; a set is written again only
 //               after the commit of the MMAs that read it.
 // TMEM (512 columns): two accumulators, so that a tile's epilogue runs beside the
 // next tile's MMAs.  With scales they lie at 0 and 160 and share columns 160 to 255,
@@ -30,14 +30,14 @@ namespace act {
 namespace pair {
 
 constexpr int BM = 256, BN = 256;  // of a pair
-constexpr int THREADS = 320, STAGES = 6, SETS = 5;
+constexpr int THREADS = 320, STAGES = 6, SETS = 8;
 constexpr int HALF_BYTES = 128 * 128;  // a CTA's half of A or of B: 128 rows x 128 bytes
 constexpr int STAGE = 2 * HALF_BYTES;
 constexpr int OUT_BYTES = 32 * 1024;  // staging of the output, over the epilogue warps
 constexpr int RING = STAGE * STAGES;
 constexpr int SMEM = 1024 + RING + OUT_BYTES + 512;
 constexpr int SF_STEP = 12;  // TMEM columns of a scale set: A 4 words, B 2 x 4
-static_assert(SMEM <= 232448 && SETS < STAGES, "placement");
+static_assert(SMEM <= 232448, "placement");
 
 enum Kind { F16 = 0, FP8 = 1 };
 template <int KIND>
@@ -185,7 +185,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     uint64_t *empty = full + STAGES;
     uint64_t *acc_full = empty + STAGES;  // [2]
     uint64_t *acc_free = acc_full + 2;    // [2], first CTA's
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_free + 2);
+    uint64_t *set_full = acc_free + 2;    // scale sets (first CTA's)
+    uint64_t *set_free = set_full + SETS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(set_free + SETS);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & 1;  // in the pair
@@ -194,9 +196,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            // the producer, and one arrival per scale warp of the pair
-            tc::mbar_init(&full[s], KIND == FP8 ? 9 : 1);
+            tc::mbar_init(&full[s], 1);
             tc::mbar_init(&empty[s], 1);
+        }
+        // The scales have barriers of their own: there are more sets than stages, so that their warps may be further
+        // ahead than the producer, whose barriers they must not arrive on then.
+        for (int i = 0; i < SETS; ++i) {
+            tc::mbar_init(&set_full[i], 8);  // the pair's scale warps
+            tc::mbar_init(&set_free[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&acc_full[i], 1);
@@ -263,7 +270,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                        : tc::smem_desc(smem + HALF_BYTES, 16, 1024, tc::SW_128B);
         const uint32_t ka = p.a_mn ? MN_STEP : 2, kb_ = p.b_mn ? MN_STEP : 2, idesc = p.idesc;
         int s = 0, set = 0, turn = 0;
-        uint32_t phase = 0;
+        uint32_t phase = 0, set_phase = 0;
         bool ok = true;
         for (int t = cluster; t < tiles && ok; t += clusters, ++turn) {
             const uint32_t acc = tmem + (turn & 1) * L::ACC1;
@@ -276,6 +283,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const Tile tl = tile_of(t, p);
             const int steps = tl.k1 - tl.k0;
             for (int kb = 0; kb < steps; ++kb) {
+                if constexpr (KIND == FP8)
+                    if (!(ok = tc::mbar_spin(&set_full[set], set_phase, abort))) break;
                 if (!(ok = tc::mbar_spin(&full[s], phase, abort))) break;
                 tc::tc_fence_after();
                 const uint64_t da = desc_a + (uint32_t)(s * (STAGE / 16)), db = desc_b + (uint32_t)(s * (STAGE / 16));
@@ -290,10 +299,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         }
                     }
                     tc::mma_commit_pair(&empty[s]);
+                    if constexpr (KIND == FP8) tc::mma_commit_pair(&set_free[set]);
                 }
                 __syncwarp();
                 if (++s == STAGES) s = 0, phase ^= 1;
-                if (++set == SETS) set = 0;
+                if (++set == SETS) set = 0, set_phase ^= 1;
             }
             if (tc::elect_one()) tc::mma_commit_pair(&acc_full[turn & 1]);
             __syncwarp();
@@ -359,7 +369,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         tc::bulk_wait<0>();
     } else if (KIND == FP8 && warp >= 6) {
         const uint32_t quad = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        constexpr int AHEAD = 4;  // stages whose words are on their way together
+        constexpr int AHEAD = 4;  // stages whose words are on their way, and written, together
         // the words of stages k0 .. of tile t, past its last one those of the last
         auto fetch = [&](uint32_t (&w)[AHEAD][3], const Tile &tl, int k0) {
             const int ga = tl.m * 2 + (int)rank, gb = tl.n * 2;
@@ -387,28 +397,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if ((more = (t += clusters) < tiles)) tl = tile_of(t, p), k0 = tl.k0;
             }
             if (more) fetch(next, tl, k0);
+            // several stages' words at once: the stores' latency, not their number, is what a turn here takes
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
                 if (i >= n) break;
                 // the set's earlier MMAs are done
-                if (it >= SETS &&
-                    !(ok = tc::mbar_spin(&empty[(it - SETS) % STAGES], ((it - SETS) / STAGES) & 1, abort)))
-                    break;
+                const int set = (it + i) % SETS;
+                if (it + i >= SETS && !(ok = tc::mbar_spin(&set_free[set], ((it + i) / SETS - 1) & 1, abort))) break;
                 tc::tc_fence_after();
                 uint32_t u[8];
-                const uint32_t d = quad + L::SF0 + it % SETS * SF_STEP;
+                const uint32_t d = quad + L::SF0 + set * SF_STEP;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) u[j] = w[i][0] >> (8 * j), u[4 + j] = w[i][1] >> (8 * j);
                 tc::tmem_st8(d, u);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) u[j] = w[i][2] >> (8 * j);
                 tc::tmem_st4(d + 8, u);
-                tc::tmem_st_wait();
-                tc::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive_remote_tmem(tc::map_cluster(&full[it % STAGES], 0));
-                ++it;
             }
+            tc::tmem_st_wait();
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane < n && ok) tc::mbar_arrive_remote_tmem(tc::map_cluster(&set_full[(it + lane) % SETS], 0));
+            __syncwarp();
+            it += n;
             if (!more) break;
         }
     }
