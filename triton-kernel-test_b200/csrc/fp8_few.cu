@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     // launched with programmatic dependence (see pair_gemm.cuh)
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    tc::dependence_wait();
 
     const int sets = p.accs * p.N;  // TMEM column of the scale sets
     bool ok = true;

@@ -11,6 +11,7 @@
 // transposition, and the scales of a block row or column are 128 bytes in one piece.
 #include "fp8.cuh"
 #include "mx4.cuh"
+#include "tc_ptx.cuh"
 
 namespace act {
 namespace fp8 {
@@ -24,8 +25,16 @@ struct Dst {
 };
 enum Mode { BY_ROWS = 1, BY_COLS = 2, BY_BOTH = 3, BY_TILES = 4 };
 
-// n of eight codes (two words) at p.
-__device__ __forceinline__ void store_codes8(uint8_t *p, uint32_t lo, uint32_t hi, int n) {
+// n of eight values times their factors (f(j): of the j-th pair) to codes at p.
+template <int FORMAT, typename F>
+__device__ __forceinline__ void store_scaled8(uint8_t *p, const float (&v)[8], F f, int n) {
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 t = mul2(make_float2(v[2 * j], v[2 * j + 1]), f(j));
+        h[j] = pack2<FORMAT>(t.x, t.y);
+    }
+    const uint32_t lo = __byte_perm(h[0], h[1], 0x5410), hi = __byte_perm(h[2], h[3], 0x5410);
     if (n == 8) {
         *reinterpret_cast<uint2 *>(p) = make_uint2(lo, hi);
     } else {
@@ -36,11 +45,12 @@ __device__ __forceinline__ void store_codes8(uint8_t *p, uint32_t lo, uint32_t h
 }
 
 template <typename T, bool VEC, int MODE, int FORMAT>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
     quant_kernel(const T *x, int64_t rows, int64_t cols, int64_t ldx, Dst a, Dst b) {
     __shared__ __align__(16) uint32_t colmax[8][128];  // of each warp
     __shared__ __align__(16) float colinv[128];
     __shared__ __align__(16) uint8_t line[2][128];  // scales of the rows, of the columns
+    tc::launch_dependents();  // the product that follows may set itself up
     const int ctiles = (int)blocks_of(cols), kr = blockIdx.x / ctiles, kc = blockIdx.x - kr * ctiles;
     const int64_t r0 = (int64_t)kr * 128, c0 = (int64_t)kc * 128;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -151,14 +161,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
                 if ((lane & 15) == 0) line[0][(lr & 31) * 4 + (lr >> 5)] = (uint8_t)sc;
             }
             if (live && ACT_DCHECK(c + n <= a.ld))
-                store_codes8(a.codes + r * a.ld + c, pack4<FORMAT>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-                             pack4<FORMAT>(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv), n);
+                store_scaled8<FORMAT>(a.codes + r * a.ld + c, v, [&](int) { return make_float2(inv, inv); }, n);
         }
         if constexpr ((MODE & BY_COLS) != 0) {
             if (live && ACT_DCHECK(c + n <= b.ld))
-                store_codes8(b.codes + r * b.ld + c,
-                             pack4<FORMAT>(v[0] * ci[0], v[1] * ci[1], v[2] * ci[2], v[3] * ci[3]),
-                             pack4<FORMAT>(v[4] * ci[4], v[5] * ci[5], v[6] * ci[6], v[7] * ci[7]), n);
+                store_scaled8<FORMAT>(b.codes + r * b.ld + c, v,
+                                      [&](int j) { return make_float2(ci[2 * j], ci[2 * j + 1]); }, n);
         }
     }
     if constexpr (MODE != BY_TILES) {

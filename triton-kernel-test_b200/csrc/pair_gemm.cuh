@@ -228,7 +228,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     const uint32_t tmem = *tmem_slot;
     // Launched with programmatic dependence: what is above runs beside the end of the
     // kernel before, nothing in memory is touched before it has ended.
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    tc::dependence_wait();
 
     if (warp == 0 && lane == 0) {
         constexpr int BK = KIND == FP8 ? 128 : 64;  // values of a stage

@@ -37,7 +37,7 @@ __host__ __device__ constexpr int rms_bwd_ctas(int maxt) { return maxt > 256 ? 1
 struct RmsShape {
     int nch, wpr, threads, rows_per_cta, depth, smem, per_sm;
 };
-static RmsShape rms_shape(int64_t cols, int esize, int inputs, bool bwd, bool vec) {
+static RmsShape rms_shape(int64_t cols, int esize, int inputs, bool bwd, bool vec, bool q8 = false) {
     const int segs = (int)((cols + SEG - 1) / SEG);
     RmsShape s{};
     if (bwd) {
@@ -50,7 +50,7 @@ static RmsShape rms_shape(int64_t cols, int esize, int inputs, bool bwd, bool ve
         s = {segs <= 1 ? 1 : (segs <= 2 ? 2 : 4), 1, 256, 8, 0, 0, 0};
     } else {
         // fewer, fuller warps spend less on a row's reductions
-        const bool full = inputs == 1 && esize == 2;
+        const bool full = inputs == 1 && esize == 2 && !q8;
         s.nch = segs <= 8 ? (full ? 2 : 1) : segs <= 16 ? (full ? 4 : 2) : segs <= 24 ? 3 : 4;
         s.wpr = (segs + s.nch - 1) / s.nch;
         s.threads = 32 * s.wpr;
@@ -103,44 +103,52 @@ struct RmsArgs {
     float eps;
 };
 
-// A segment's values of row r to codes, and its two blocks' scales.
+// The largest magnitude of a, b and m; NaN stays.
+__device__ __forceinline__ float absmax3(float m, float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+// A segment's values to codes (`codes`: the segment's first), and its two blocks' scales
+// (`scales`: the first block's, `step` bytes on the second's).
 template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t *codes, uint8_t *scales, int64_t ldc, int64_t r, int64_t groups,
-                                            int64_t seg0, int n, int lane, F8 v, int64_t cols) {
-    uint8_t *row = codes + r * ldc + seg0;
+__device__ __forceinline__ void store_codes(uint8_t *codes, uint8_t *scales, int64_t step, int n, int lane, const F8 &v,
+                                            int64_t left) {
     const float2 *p = v.p;
-    uint32_t m[2] = {0u, 0u};
     if constexpr (VEC) {
+        float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[0] = max(m[0], max(fp8::mag(p[j].x), fp8::mag(p[j].y)));
+        for (int j = 0; j < 4; ++j) m = absmax3(m, p[j].x, p[j].y);
+        uint32_t u = fp8::mag(m);
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], o));
-        const uint32_t sc = fp8::scale_code(m[0], fp8::top_of(fp8::E4M3));
+        for (int o = 8; o > 0; o >>= 1) u = max(u, __shfl_xor_sync(0xffffffffu, u, o));
+        const uint32_t sc = fp8::scale_code(u, 8);
         const float inv = fp8::inv_scale(sc);
         const float2 i2 = make_float2(inv, inv);
-        float2 q[4];
+        uint32_t h[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = mul2(p[j], i2);
-        if (n && ACT_DCHECK(seg0 + 8 * lane + 8 <= cols))
-            *reinterpret_cast<uint2 *>(row + 8 * lane) =
-                make_uint2(fp8::pack4<fp8::E4M3>(q[0].x, q[0].y, q[1].x, q[1].y),
-                           fp8::pack4<fp8::E4M3>(q[2].x, q[2].y, q[3].x, q[3].y));
-        if ((lane & 15) == 0 && n) scales[fp8::scale_at(r, (seg0 >> 7) + (lane >> 4), groups)] = (uint8_t)sc;
+        for (int j = 0; j < 4; ++j) {
+            const float2 t = mul2(p[j], i2);
+            h[j] = fp8::pack2<fp8::E4M3>(t.x, t.y);
+        }
+        if (n && ACT_DCHECK(8 * lane + 8 <= left)) {
+            *reinterpret_cast<uint2 *>(codes + 8 * lane) =
+                make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
+            if ((lane & 15) == 0) scales[lane ? step : 0] = (uint8_t)sc;
+        }
     } else {  // value 32 j + lane: block j / 4
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[j >> 1] = max(m[j >> 1], max(fp8::mag(p[j].x), fp8::mag(p[j].y)));
-#pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const uint32_t sc =
-                fp8::scale_code(__reduce_max_sync(0xffffffffu, m[k]), fp8::top_of(fp8::E4M3));
+            const float m = absmax3(absmax3(0.f, p[2 * k].x, p[2 * k].y), p[2 * k + 1].x, p[2 * k + 1].y);
+            const uint32_t sc = fp8::scale_code(__reduce_max_sync(0xffffffffu, fp8::mag(m)), 8);
             const float inv = fp8::inv_scale(sc);
 #pragma unroll
             for (int j = 2 * k; j < 2 * k + 2; ++j) {
                 const uint32_t c = fp8::pack2<fp8::E4M3>(p[j].x * inv, p[j].y * inv);
-                if (2 * j < n && ACT_DCHECK(seg0 + 64 * j + lane < cols)) row[64 * j + lane] = (uint8_t)c;
-                if (2 * j + 1 < n) row[64 * j + 32 + lane] = (uint8_t)(c >> 8);
+                if (2 * j < n && ACT_DCHECK(64 * j + lane < left)) codes[64 * j + lane] = (uint8_t)c;
+                if (2 * j + 1 < n) codes[64 * j + 32 + lane] = (uint8_t)(c >> 8);
             }
-            if (lane == 0 && 4 * k < n) scales[fp8::scale_at(r, (seg0 >> 7) + k, groups)] = (uint8_t)sc;
+            if (lane == 0 && 4 * k < n) scales[k ? step : 0] = (uint8_t)sc;
         }
     }
 }
@@ -165,6 +173,7 @@ __global__ void __launch_bounds__(MAXT, rms_ctas(NCH, MAXT))
     rms_fwd_kernel(const __grid_constant__ RmsArgs<T, W> a, int warps, int depth) {
     const int wpr = ONE ? 1 : warps;
     extern __shared__ __align__(128) uint8_t dyn[];
+    if constexpr (Q) tc::launch_dependents();  // the product that follows may set itself up
     constexpr int NW = MAXT / 32;
     // rows in hand at once: their reductions overlap and share their barriers
     constexpr int R = NCH <= 2 && sizeof(T) == 2 ? 2 : 1;
@@ -175,7 +184,7 @@ __global__ void __launch_bounds__(MAXT, rms_ctas(NCH, MAXT))
     const int rpc = ONE ? nwarps : 1;
     const int w0 = ONE ? 0 : warp, mine = ONE ? warp : 0;
     const float inv_n = 1.f / (float)a.cols;
-    const int64_t groups = fp8::blocks_of(a.rows);
+    const int64_t groups = fp8::blocks_of(a.rows), step8 = groups * fp8::BLOCK;  // from a block's scales to the next's
     constexpr int IN = RES ? 2 : 1;
     RowRing<T, IN, VEC> ring;
     const bool leader = ONE ? lane == 0 : threadIdx.x == 0;
@@ -249,7 +258,8 @@ __global__ void __launch_bounds__(MAXT, rms_ctas(NCH, MAXT))
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[k][i].p[j] = mul2(mul2(v[k][i].p[j], rstd2), w.p[j]);
                 if constexpr (Q)
-                    store_codes<VEC>(a.codes, a.scales, a.ldc, rk, groups, seg0, n[i], lane, v[k][i], a.cols);
+                    store_codes<VEC>(a.codes + rk * a.ldc + seg0, a.scales + fp8::scale_at(rk, 0, groups) + (seg0 >> 7) * step8,
+                                     step8, n[i], lane, v[k][i], a.cols - seg0);
                 else
                     store8<T, VEC>(a.y + rk * a.ldy, seg0, n[i], lane, v[k][i]);
             }
@@ -296,7 +306,10 @@ __global__ void __launch_bounds__(LONG_THREADS) rms_fwd_long_kernel(RmsArgs<T, W
             const F8 w = unpack<W>(load8_or<W, VEC>(a.w, 1.f, g * SEG, n, lane));
 #pragma unroll
             for (int j = 0; j < 4; ++j) v.p[j] = mul2(mul2(v.p[j], rstd2), w.p[j]);
-            if constexpr (Q) store_codes<VEC>(a.codes, a.scales, a.ldc, r, groups, g * SEG, n, lane, v, a.cols);
+            if constexpr (Q)
+                store_codes<VEC>(a.codes + r * a.ldc + g * SEG,
+                                              a.scales + fp8::scale_at(r, 2 * g, groups), groups * fp8::BLOCK, n, lane, v,
+                                              a.cols - g * SEG);
             else store8<T, VEC>(a.y + r * a.ldy, g * SEG, n, lane, v);
         }
     }
@@ -316,7 +329,7 @@ static int rms_fwd_launch(const RmsArgs<T, W> &a, cudaStream_t st) {
         rms_fwd_long_kernel<T, W, VEC, RES, Q><<<(int)(a.rows < cap ? a.rows : cap), LONG_THREADS, 0, st>>>(a);
         return launch_status();
     }
-    const RmsShape s = rms_shape(a.cols, sizeof(T), RES ? 2 : 1, false, VEC);
+    const RmsShape s = rms_shape(a.cols, sizeof(T), RES ? 2 : 1, false, VEC, Q);
     auto go = [&](auto k) -> int {
         if (int rc = allow_smem(k, s.smem, MAX_SMEM)) return rc;
         k<<<rms_grid(s, a.rows), s.threads, s.smem, st>>>(a, s.wpr, s.depth);
@@ -327,7 +340,7 @@ static int rms_fwd_launch(const RmsArgs<T, W> &a, cudaStream_t st) {
         return s.nch == 2 ? go(rms_fwd_kernel<T, W, 2, 256, VEC, RES, Q, true>)
                           : go(rms_fwd_kernel<T, W, 4, 256, VEC, RES, Q, true>);
     }
-    if constexpr (RES || sizeof(T) == 4) {  // see rms_shape: the others take two segments
+    if constexpr (RES || Q || sizeof(T) == 4) {  // see rms_shape: the others take two segments
         if (s.nch == 1) return go(rms_fwd_kernel<T, W, 1, 256, VEC, RES, Q, false>);
     }
     if (s.nch == 2) return go(rms_fwd_kernel<T, W, 2, 256, VEC, RES, Q, false>);

@@ -214,9 +214,9 @@ struct SumEpi {
 };
 
 // ---------------------------------------------------------------- small kernels
-// A token's partial maxima and sums joined: 32 tokens a CTA, a lane each, sixteen warps
-// over the partials.
-constexpr int JOIN_WARPS = 16;
+// A token's partial maxima and sums joined: 32 tokens a CTA, a lane each, 32 warps over
+// the partials, eight on their way at a time.
+constexpr int JOIN_WARPS = 32;
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
     join_kernel(const float2 *part, int parts, int tokens, int64_t vocab, const int64_t *target, int64_t ignore,
                 float *loss, float *lse) {
@@ -224,22 +224,46 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.x * 32 + lane;
     float m = -INFINITY, s = 0.f;
-    auto join = [&](float2 q) {
-        if (q.x > m) {
-            s = __fmaf_rn(s, exp2f(m - q.x), q.y);
-            m = q.x;
-        } else if (q.x > -INFINITY) {
-            s = __fmaf_rn(q.y, exp2f(q.x - m), s);
+    // N pairs into (m, s): one scale to the new maximum; without one (all -inf) the sums, 0 or the NaN of a tile
+    // that had nothing else, are added as they are
+    auto join = [&](auto &q) {
+        constexpr int N = sizeof(q) / sizeof(float2);
+        float now = m;
+#pragma unroll
+        for (int i = 0; i < N; ++i) now = fmaxf(now, q[i].x);
+        if (now > -INFINITY) {
+            s *= ex2(m - now);
+#pragma unroll
+            for (int i = 0; i < N; ++i) s = __fmaf_rn(q[i].y, ex2(q[i].x - now), s);
+            m = now;
         } else {
-            s += q.y;  // 0, or the NaN of a tile that had nothing else
+#pragma unroll
+            for (int i = 0; i < N; ++i) s += q[i].y;
         }
     };
-    if (row < tokens)
-        for (int i = warp; i < parts; i += JOIN_WARPS) join(part[(int64_t)i * tokens + row]);
+    tc::dependence_wait();
+    if (row < tokens) {
+        const float2 *p = part + row;
+        int i = warp;
+        for (; i + 7 * JOIN_WARPS < parts; i += 8 * JOIN_WARPS) {
+            float2 q[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) q[k] = p[(int64_t)(i + k * JOIN_WARPS) * tokens];
+            join(q);
+        }
+        float2 q[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            q[k] = i + k * JOIN_WARPS < parts ? p[(int64_t)(i + k * JOIN_WARPS) * tokens] : make_float2(-INFINITY, 0.f);
+        join(q);
+    }
     red[warp][lane] = make_float2(m, s);
     __syncthreads();
     if (warp != 0 || row >= tokens) return;
-    for (int i = 1; i < JOIN_WARPS; ++i) join(red[i][lane]);
+    for (int i = 1; i < JOIN_WARPS; ++i) {
+        float2 q[1] = {red[i][lane]};
+        join(q);
+    }
     const double l = (double)m * 0.69314718055994530942 + (double)logf(s);
     lse[row] = (float)l;
     const int64_t t = target[row];
@@ -265,8 +289,15 @@ __device__ __forceinline__ float pow2_below(float v) {
     const uint32_t e = __float_as_uint(v) & 0x7f800000u;
     return v == 0.f ? 1.f : __uint_as_float(e == 0x7f800000u ? 0x7f000000u : e == 0u ? 0x00800000u : e);
 }
-__global__ void __launch_bounds__(1024) largest_kernel(GradArgs g, float *scale) {
+// The tokens' factors, and x's rows scaled for dW (null: not wanted).  A warp a token;
+// every CTA finds the largest factor for itself (a pass over 12 bytes a token from L2,
+// on at most one CTA per SM, where a kernel of its own took 5 us).
+template <typename T>
+__global__ void __launch_bounds__(1024)
+    rows_kernel(GradArgs g, float *scale, Row *rows, const T *x, int64_t ldx, int64_t cols, T *xs, int64_t lds) {
     __shared__ float red[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    tc::dependence_wait();
     float m = 0.f;
     for (int64_t r = threadIdx.x; r < g.tokens; r += 1024) {
         float a, d;
@@ -274,20 +305,11 @@ __global__ void __launch_bounds__(1024) largest_kernel(GradArgs g, float *scale)
         m = fmaxf(m, fmaxf(fabsf(a), fabsf(d)));  // passes NaN over
     }
     m = warp_max(m);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    if (lane == 0) red[warp] = m;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        m = warp_max(red[threadIdx.x]);
-        if (threadIdx.x == 0) *scale = pow2_below(m);
-    }
-}
-// The tokens' factors, and x's rows scaled for dW (null: not wanted).  A warp a token.
-template <typename T>
-__global__ void __launch_bounds__(256)
-    rows_kernel(GradArgs g, const float *scale, Row *rows, const T *x, int64_t ldx, int64_t cols, T *xs, int64_t lds) {
-    const int lane = threadIdx.x & 31;
-    const float top = *scale;
-    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < g.tokens; r += (int64_t)gridDim.x * 8) {
+    const float top = pow2_below(warp_max(red[lane]));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *scale = top;
+    for (int64_t r = (int64_t)blockIdx.x * 32 + warp; r < g.tokens; r += (int64_t)gridDim.x * 32) {
         float a, d;
         factors(g, r, a, d);
         const bool live = !(a == 0.f && d == 0.f);
@@ -297,33 +319,64 @@ __global__ void __launch_bounds__(256)
         const float f = live ? s / top : 0.f;
         const T *src = x + r * ldx;
         T *dst = xs + r * lds;
-        const int64_t whole = (reinterpret_cast<uintptr_t>(src) & 15) ? 0 : cols & ~(int64_t)7;
-        for (int64_t c = 8 * lane; c < whole; c += 256) {
-            const uint4 q = *reinterpret_cast<const uint4 *>(src + c);
-            T v[8];
-            memcpy(v, &q, 16);
+        const int64_t whole = cols & ~(int64_t)7;  // rows are 16-byte aligned
+        auto scaled = [&](T v) { return live ? pair::cvt_out<T>((float)v * f) : pair::cvt_out<T>(0.f); };
+        for (int64_t c0 = 8 * lane; c0 < whole; c0 += 4 * 256) {
+            uint4 q[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = live ? pair::cvt_out<T>((float)v[j] * f) : pair::cvt_out<T>(0.f);
-            uint4 o;
-            memcpy(&o, v, 16);
-            *reinterpret_cast<uint4 *>(dst + c) = o;
+            for (int k = 0; k < 4; ++k)
+                if (c0 + 256 * k < whole) q[k] = *reinterpret_cast<const uint4 *>(src + c0 + 256 * k);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (c0 + 256 * k >= whole) break;
+                T v[8];
+                memcpy(v, &q[k], 16);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = scaled(v[j]);
+                memcpy(&q[k], v, 16);
+                *reinterpret_cast<uint4 *>(dst + c0 + 256 * k) = q[k];
+            }
         }
-        for (int64_t c = whole + lane; c < cols; c += 32)
-            dst[c] = live ? pair::cvt_out<T>((float)src[c] * f) : pair::cvt_out<T>(0.f);
+        for (int64_t c = whole + lane; c < cols; c += 32) dst[c] = scaled(src[c]);
     }
 }
-// dx from the splits' sums, in a fixed order.
+// dx from the splits' sums, in a fixed order: four values a thread, blockIdx.y over the
+// tokens.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    sum_kernel(const float *part, int splits, int64_t tokens, int64_t cols, int64_t ld, const Row *rows, T *dx,
-               int64_t lddx) {
-    const int64_t n = tokens * cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / cols, c = i - r * cols;
-        float s = 0.f;
-        for (int k = 0; k < splits; ++k) s += part[k * tokens * ld + r * ld + c];
-        dx[r * lddx + c] = pair::cvt_out<T>(s * rows[r].scale);
+    sum_kernel(const float *part, int splits, int tokens, int cols, int64_t ld, const Row *rows, T *dx, int64_t lddx) {
+    const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
+    tc::dependence_wait();
+    if (c >= cols) return;
+    for (int r = blockIdx.y; r < tokens; r += gridDim.y) {
+        const float *p = part + (int64_t)r * ld + c;
+        const int64_t step = (int64_t)tokens * ld;
+        float4 s = *reinterpret_cast<const float4 *>(p);  // ld is a multiple of 4: whole pieces are there
+        for (int k = 1; k < splits; ++k) {
+            const float4 q = *reinterpret_cast<const float4 *>(p + k * step);
+            s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
+        }
+        const float f = rows[r].scale, v[4] = {s.x * f, s.y * f, s.z * f, s.w * f};
+        T *d = dx + (int64_t)r * lddx + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < cols && ACT_DCHECK(c + i < lddx)) d[i] = pair::cvt_out<T>(v[i]);
     }
+}
+// A launch with programmatic dependence on the kernel before it.
+template <typename... P, typename... A>
+static int launch_after(void (*k)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    ACT_CUDA_TRY(cudaLaunchKernelEx(&cfg, k, P(args)...));
+    return ACT_OK;
 }
 
 // ---------------------------------------------------------------- host
@@ -417,11 +470,10 @@ static int backward(const actcomp_xent_args *g, const actcomp_xent_grads *o, con
     float *scale = reinterpret_cast<float *>(ws + q.scale), *part = reinterpret_cast<float *>(ws + q.part);
     T *gs = reinterpret_cast<T *>(ws + q.g), *xs = reinterpret_cast<T *>(ws + q.xs);
     const GradArgs ga{g->target, g->lse, o->dloss, o->dlse, g->ignore_index, g->vocab, g->tokens};
-    largest_kernel<<<1, 1024, 0, st>>>(ga, scale);
-    const int64_t cap = (int64_t)num_sms() * 8, need = (g->tokens + 7) / 8;
-    rows_kernel<T><<<(int)(need < cap ? need : cap), 256, 0, st>>>(ga, scale, rows, static_cast<const T *>(g->x), g->ldx,
-                                                                  g->channels, o->dweight ? xs : nullptr, q.ldx);
-    if (int rc = launch_status()) return rc;
+    const int64_t cap = num_sms(), need = (g->tokens + 31) / 32;
+    if (int rc = launch_after(rows_kernel<T>, dim3((unsigned)(need < cap ? need : cap)), 1024, st, ga, scale, rows,
+                              static_cast<const T *>(g->x), g->ldx, g->channels, o->dweight ? xs : nullptr, q.ldx))
+        return rc;
     const int k_first = (int)(((g->vocab < q.piece ? g->vocab : q.piece) + BK - 1) / BK);
     const int k_split = (k_first + q.splits - 1) / q.splits, splits = (k_first + k_split - 1) / k_split;
     for (int i = 0; i < q.pieces; ++i) {
@@ -468,10 +520,10 @@ static int backward(const actcomp_xent_args *g, const actcomp_xent_grads *o, con
             }
             if (rc) return rc;
             if (last && splits > 1) {
-                const int64_t ctas = ((int64_t)T_ * H + 255) / 256;
-                sum_kernel<T><<<(int)(ctas < 4 * cap ? ctas : 4 * cap), 256, 0, st>>>(
-                    part, splits, T_, H, q.ldd, rows, static_cast<T *>(o->dx), o->lddx);
-                if ((rc = launch_status())) return rc;
+                const dim3 grid((unsigned)((H + 1023) / 1024), (unsigned)(T_ < 65535 ? T_ : 65535));
+                if ((rc = launch_after(sum_kernel<T>, grid, 256, st, part, splits, T_, H, q.ldd, rows,
+                                       static_cast<T *>(o->dx), o->lddx)))
+                    return rc;
             }
         }
         if (o->dweight) {  // dW = g^T . x
@@ -518,9 +570,8 @@ extern "C" int actcomp_xent(const actcomp_xent_args *g, void *workspace, size_t 
     float2 *part = static_cast<float2 *>(workspace);
     cudaStream_t st = as_stream(stream);
     if (int rc = pair::launch<pair::F16, FwdEpi>(tmA, tmB, tmA, p, FwdP{part, g->loss, g->target}, st)) return rc;
-    join_kernel<<<(unsigned)((g->tokens + 31) / 32), 32 * JOIN_WARPS, 0, st>>>(part, 2 * p.n_tiles, (int)g->tokens, g->vocab,
-                                                                              g->target, g->ignore_index, g->loss, g->lse);
-    return launch_status();
+    return launch_after(join_kernel, dim3((unsigned)((g->tokens + 31) / 32)), 32 * JOIN_WARPS, st, part, 2 * p.n_tiles,
+                        (int)g->tokens, g->vocab, g->target, g->ignore_index, g->loss, g->lse);
 }
 
 extern "C" size_t actcomp_xent_bwd_workspace(int64_t tokens, int64_t channels, int64_t vocab, int64_t piece) {
