@@ -14,8 +14,8 @@
 //               columns) of its A rows and of all 256 B rows, counted on its own;
 //   warp 1      TMEM allocation; in the first CTA the MMA issuer;
 //   warps 2..5  epilogue: TMEM to registers, convert, swizzled shared memory,
-//               TMA store (rows or bases that are not 16-byte aligned: plain
-//               stores);
+//               TMA store (rows or bases that are not 16-byte aligned, or rows that
+//               do not end on 16 bytes: plain stores);
 //   warps 6..9  scales: shared memory to TMEM, every lane quadrant the same, four
 //               sets of 256 columns in turn; a set is written again only after
 //               the commit of the MMAs that read it.
@@ -365,7 +365,8 @@ extern "C" int actcomp_mx4_gemm(const actcomp_mx4 *a, const actcomp_mx4 *b, void
     p.n_tiles = (p.N + BN - 1) / BN;
     p.C = c;
     p.ldc = ldc;
-    p.tma_out = aligned(c, 16) && (ldc * es) % 16 == 0;
+    // rows of whole 16 bytes: a tile store that is clipped inside 16 bytes writes zeros to their end
+    p.tma_out = aligned(c, 16) && (ldc * es) % 16 == 0 && ((int64_t)p.N * es) % 16 == 0;
     ACT_CHECK((int64_t)p.m_tiles * p.n_tiles <= INT32_MAX, ACT_E_UNSUPPORTED);
     const int64_t rb = row_bytes(a->cols);
     CUtensorMap tmA, tmB, tmSA, tmSB, tmC;
