@@ -616,8 +616,8 @@ int actcomp_xent(const actcomp_xent_args *a, void *workspace, size_t workspace_b
  * fp16 holds it.  A token without a gradient (ignored or dloss 0, and no dlse) adds
  * nothing, whatever its row of x holds; one whose target lies outside the vocabulary
  * makes its row of dx and all of dweight NaN.  The vocabulary is taken in pieces of `piece`
- * columns (rounded to whole tiles of 256; 0: what keeps a piece's dz in 1 GiB); the
- * workspace is actcomp_xent_bwd_workspace() bytes of the same piece. */
+ * columns (rounded to whole tiles of 256; 0: what keeps a piece's dz in 1 GiB, 4096 at
+ * least); the workspace is actcomp_xent_bwd_workspace() bytes of the same piece. */
 typedef struct actcomp_xent_grads {
     const float *dloss, *dlse;
     void *dx;

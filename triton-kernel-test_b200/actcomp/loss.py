@@ -15,9 +15,10 @@ outside the vocabulary give NaN.
 
 The products run on bf16 or fp16 operands with float32 accumulation.  The backward pass
 computes the logits again, a piece of the vocabulary at a time, and keeps the piece's
-gradient in x's dtype (workspace: 1 GiB at most by default, ``vocab_piece`` chooses),
-scaled so that fp16 holds it; a copy of x and, with several pieces, dx in float32 come
-on top.  Tokens without a gradient add nothing, whatever their rows of x hold.
+gradient in x's dtype, scaled so that fp16 holds it (workspace: by default 1 GiB, or
+4096 columns where those are more; ``vocab_piece`` chooses); a copy of x and, with
+several pieces, dx in float32 come on top.  Tokens without a gradient add nothing,
+whatever their rows of x hold.
 
 Waits inside the products are bounded.  One that gives up leaves NaN in the losses it
 had, or parts of the gradients unwritten, and is recorded in the device error word, which
@@ -48,5 +49,5 @@ def linear_cross_entropy_backward(dloss: torch.Tensor, x: torch.Tensor, weight: 
                                   vocab_piece: int = 0) -> tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dweight) in x's dtype from the float32 gradients of loss and lse (one value
     a token); what is not asked for is None.  ``vocab_piece``: columns of the vocabulary
-    at a time, in whole tiles of 256 (0: what fits 1 GiB)."""
+    at a time, in whole tiles of 256 (0: see above)."""
     return _host.xent_backward(dloss, x, weight, target, lse, dlse, ignore_index, x_grad, weight_grad, vocab_piece)

@@ -10,7 +10,7 @@ from typing import Optional
 
 import torch
 
-from . import core, mx4, norm, refcompat
+from . import core, fp8, loss, mx4, norm, refcompat
 
 _U8, _F32, _BF = torch.uint8, torch.float32, torch.bfloat16
 
@@ -204,6 +204,41 @@ def _(dy, h, weight, mean, rstd, p, seed, row_offset, dh, bias_dtype=None):
     return (_empty(h.shape, h.dtype, h), _empty(h.shape, h.dtype, h)) + _weight_grads(h, weight, bias_dtype)
 
 
+@torch.library.custom_op("actcomp::rms_norm", mutates_args=())
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    return norm.rms_norm(x, weight, eps)
+
+
+@rms_norm.register_fake
+def _(x, weight, eps):
+    return _empty(x.shape, x.dtype, x), _empty(x.shape[:-1], _F32, x)
+
+
+@torch.library.custom_op("actcomp::add_rms_norm", mutates_args=())
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor],
+                 eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return norm.add_rms_norm(x, residual, weight, eps)
+
+
+@add_rms_norm.register_fake
+def _(x, residual, weight, eps):
+    return _empty(x.shape, x.dtype, x), _empty(x.shape, x.dtype, x), _empty(x.shape[:-1], _F32, x)
+
+
+@torch.library.custom_op("actcomp::rms_norm_backward", mutates_args=())
+def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], rstd: torch.Tensor,
+                      dh: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    """norm.rms_norm_backward; without a weight its gradient is an empty tensor."""
+    dx, dw = norm.rms_norm_backward(dy, x, weight, rstd, dh)
+    return dx, dx.new_empty(0) if dw is None else dw
+
+
+@rms_norm_backward.register_fake
+def _(dy, x, weight, rstd, dh):
+    dw = x.new_empty(0) if weight is None else _empty(weight.shape, weight.dtype, x)
+    return _empty(x.shape, x.dtype, x), dw
+
+
 # ---------------------------------------------------------------- microscaled 4-bit
 def _mx4_shapes(rows, cols):
     return (rows, (cols + 31) // 32 * 16), ((rows + 127) // 128 * ((cols + 127) // 128) * 512,)
@@ -232,3 +267,60 @@ def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_d
 @mx4_linear.register_fake
 def _(x, codes, scales, out_dtype):
     return _empty(x.shape[:-1] + (codes.shape[0],), out_dtype, x)
+
+
+# ---------------------------------------------------------------- 8-bit floating point
+def _fp8_shapes(rows, cols, tiles):
+    blocks = (rows + 127) // 128 * ((cols + 127) // 128)
+    return (rows, (cols + 15) // 16 * 16), (blocks if tiles else blocks * 128,)
+
+
+@torch.library.custom_op("actcomp::fp8_quantize", mutates_args=())
+def fp8_quantize(x: torch.Tensor, transpose: bool, tiles: bool, format: str) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of fp8.quantize, or with tiles of fp8.quantize_weight."""
+    q = fp8.quantize_weight(x, format) if tiles else fp8.quantize(x, transpose, format)
+    return q.codes, q.scales
+
+
+@fp8_quantize.register_fake
+def _(x, transpose, tiles, format):
+    c, s = _fp8_shapes(x.numel() // x.shape[-1], x.shape[-1], tiles)
+    return _empty(c, _U8, x), _empty(s, _U8, x)
+
+
+@torch.library.custom_op("actcomp::fp8_linear", mutates_args=())
+def fp8_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, format: str,
+               out_dtype: torch.dtype) -> torch.Tensor:
+    """fp8.linear with the buffers of a weight by tiles (codes: (N, K rounded up to 16))."""
+    w = fp8.Fp8(codes.shape[0], x.shape[-1], codes, scales, x.dtype, format, tiles=True)
+    return fp8.linear(x, w, out_dtype)
+
+
+@fp8_linear.register_fake
+def _(x, codes, scales, format, out_dtype):
+    return _empty(x.shape[:-1] + (codes.shape[0],), out_dtype, x)
+
+
+# ---------------------------------------------------------------- cross entropy of a linear layer
+@torch.library.custom_op("actcomp::linear_cross_entropy", mutates_args=())
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
+                         ignore_index: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return loss.linear_cross_entropy(x, weight, target, ignore_index)
+
+
+@linear_cross_entropy.register_fake
+def _(x, weight, target, ignore_index):
+    return _empty(target.shape, _F32, x), _empty(target.shape, _F32, x)
+
+
+@torch.library.custom_op("actcomp::linear_cross_entropy_backward", mutates_args=())
+def linear_cross_entropy_backward(dloss: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
+                                  lse: torch.Tensor, dlse: Optional[torch.Tensor], ignore_index: int,
+                                  vocab_piece: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return loss.linear_cross_entropy_backward(dloss, x, weight, target, lse, dlse, ignore_index,
+                                              vocab_piece=vocab_piece)
+
+
+@linear_cross_entropy_backward.register_fake
+def _(dloss, x, weight, target, lse, dlse, ignore_index, vocab_piece):
+    return _empty(x.shape, x.dtype, x), _empty(weight.shape, weight.dtype, x)

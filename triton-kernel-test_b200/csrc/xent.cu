@@ -394,10 +394,12 @@ static int map_out(CUtensorMap *m, CUtensorMapDataType dt, int es, void *p, int6
 }
 static bool tma_rows(const void *p, int64_t ld, int es) { return aligned(p, 16) && (ld * es) % 16 == 0; }
 
-// Columns of the vocabulary in a piece: what is asked for, or g in at most 1 GiB; pieces
-// of about one size, whole tiles.
+// Columns of the vocabulary in a piece: what is asked for, or g in at most 1 GiB, but 4096
+// at least (every piece reads and writes dx's sums, 8 bytes a value, against 2 operations
+// a value and column); pieces of about one size, whole tiles.
 static int64_t piece_of(int64_t tokens, int64_t vocab, int64_t asked) {
     int64_t most = asked > 0 ? asked : ((int64_t)1 << 29) / (tokens > 0 ? tokens : 1);
+    if (!asked && most < 4096) most = 4096;
     most = most / pair::BN * pair::BN;
     if (most < pair::BN) most = pair::BN;
     const int64_t pieces = (vocab + most - 1) / most;
