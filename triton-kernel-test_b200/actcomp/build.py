@@ -87,7 +87,8 @@ def build_host(force: bool = False) -> str:
     tmp = out + ".tmp"
     subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", src, "-o", tmp,
                     *[f"-I{i}" for i in inc], f"-L{os.path.join(base, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
-                    "-ltorch", "-ltorch_python", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"],
+                    "-ltorch_cuda", "-ltorch", "-ltorch_python",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"],
                    check=True)
     os.replace(tmp, out)
     return out

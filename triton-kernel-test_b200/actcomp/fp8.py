@@ -48,7 +48,7 @@ def _format(name: str) -> int:
     return FORMATS.index(name)
 
 
-@dataclass
+@dataclass(slots=True)
 class Fp8:
     """A rows x cols matrix in 8-bit floating point, a scale per 128 values of a row or
     (``tiles``) per 128 x 128.  ``transposed``: codes hold the transpose, cols x rows,
