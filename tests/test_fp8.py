@@ -296,6 +296,10 @@ def test_linear_layer(dtype, tokens, k, n):
     assert dx.shape == (1, tokens, k)
     product_close(dx[0], g, w.t(), dtype)
     product_close(dw, gt, saved, dtype)
+    g, gt = fp8.quantize_pair(dy, "e5m2")
+    dx, dw = fp8.linear_backward(dy, saved, w, torch.float32, grad_format="e5m2")
+    product_close(dx, g, w.t(), torch.float32)
+    product_close(dw, gt, saved, torch.float32)
 
 
 @pytest.mark.gpu

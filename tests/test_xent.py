@@ -221,6 +221,13 @@ def test_shapes_ignored_and_outside_targets():
     # another ignore_index, inside the vocabulary
     l2, _ = actcomp.linear_cross_entropy(x.cuda(), w.cuda(), t.cuda(), ignore_index=499)
     assert l2[9] == 0 and l2[7].isnan() and torch.equal(l2[10:], loss[10:])
+    # one token without a leading dimension, weight rows and targets at a stride
+    l3, n3 = actcomp.linear_cross_entropy(x[9].cuda(), torch.cat([w, w], 1).cuda()[:, :64], t[9].cuda())
+    assert l3.shape == n3.shape == () and torch.equal(l3, loss[9]) and torch.equal(n3, lse[9])
+    dx, dw = actcomp.linear_cross_entropy_backward(torch.ones((), device="cuda"), x[9].cuda(), w.cuda(), t[9].cuda(), n3)
+    assert dx.shape == (64,) and dw.shape == w.shape
+    wide = torch.stack([t, t + 1], 1).cuda()
+    assert torch.equal(actcomp.linear_cross_entropy(x.cuda(), w.cuda(), wide[:, 0])[0][10:], loss[10:])
     # no token
     e = actcomp.linear_cross_entropy(x[:0].cuda(), w.cuda(), t[:0].cuda())
     assert e[0].shape == (0,)

@@ -143,11 +143,11 @@ def linear_forward(x: torch.Tensor, w: Fp8, out_dtype: Optional[torch.dtype] = N
     return matmul(q, w, out_dtype).view(x.shape[:-1] + (w.rows,)), saved
 
 
-def linear_backward(dy: torch.Tensor, saved: Fp8, w: Fp8,
-                    out_dtype: Optional[torch.dtype] = None) -> tuple[torch.Tensor, torch.Tensor]:
+def linear_backward(dy: torch.Tensor, saved: Fp8, w: Fp8, out_dtype: Optional[torch.dtype] = None,
+                    grad_format: str = "e4m3") -> tuple[torch.Tensor, torch.Tensor]:
     """(dx, dw) of :func:`linear_forward`: dx = dy . W with dy (..., N) by rows and the
     weight's tiles; dw = dy^T . x (N, K), both by columns.  ``out_dtype`` defaults to
-    dy's."""
+    dy's; ``grad_format`` is what dy is held in."""
     if not w.tiles:
         raise ValueError("the input gradient needs the weight by tiles (quantize_weight)")
     if dy.shape[-1] != w.rows or saved.rows != w.cols:
@@ -155,7 +155,7 @@ def linear_backward(dy: torch.Tensor, saved: Fp8, w: Fp8,
                          f"the weight is {w.rows} x {w.cols}")
     if dy.numel() // dy.shape[-1] != saved.cols:
         raise ValueError(f"dy has {dy.numel() // dy.shape[-1]} tokens, the saved input {saved.cols}")
-    q, qt = quantize_pair(dy)
+    q, qt = quantize_pair(dy, grad_format)
     dx = matmul(q, w.t(), out_dtype).view(dy.shape[:-1] + (w.cols,))
     return dx, matmul(qt, saved, out_dtype)
 

@@ -91,6 +91,14 @@ static int rms_types(int dtype, int wide, F f) {
 // 16-byte access to every row: base and row stride
 static bool rows16(const void *p, int64_t ld, int esize) { return !p || (aligned(p, 16) && (ld * esize) % 16 == 0); }
 
+// 1 / sqrt(v): the hardware's approximation and one Newton step whose correction is
+// added in a fused multiply-add, within about half a unit in the last place (an 8-bit
+// output changes its code where the values before it move across a tie).
+__device__ __forceinline__ float rstd_of(float v) {
+    const float r = rsqrtf(v), e = __fmaf_rn(-v * r, r, 1.f), h = __fmaf_rn(0.5f * r, e, r);
+    return v > 0.f && v < INFINITY ? h : r;
+}
+
 // ---------------------------------------------------------------- forward
 template <typename T, typename W>
 struct RmsArgs {
@@ -247,7 +255,7 @@ __global__ void __launch_bounds__(MAXT, rms_ctas(NCH, MAXT))
         for (int k = 0; k < R; ++k) {
             const int64_t rk = r + k * step;
             if (k > 0 && rk >= a.rows) break;
-            const float rstd = inv_sqrt(__fmaf_rn(s[k], inv_n, a.eps));
+            const float rstd = rstd_of(__fmaf_rn(s[k], inv_n, a.eps));
             if (lane == 0 && w0 == 0) a.rstd[rk] = rstd;
             const float2 rstd2 = make_float2(rstd, rstd);
 #pragma unroll
@@ -296,7 +304,7 @@ __global__ void __launch_bounds__(LONG_THREADS) rms_fwd_long_kernel(RmsArgs<T, W
             s += t.x + t.y;
         }
         // two sets of partial sums in turn: one barrier a row
-        const float rstd = inv_sqrt(__fmaf_rn(row_sum<nw>(s, red + turn, warp, lane), inv_n, a.eps));
+        const float rstd = rstd_of(__fmaf_rn(row_sum<nw>(s, red + turn, warp, lane), inv_n, a.eps));
         if (threadIdx.x == 0) a.rstd[r] = rstd;
         const float2 rstd2 = make_float2(rstd, rstd);
         for (int64_t g = warp; g < segs; g += nw) {

@@ -17,7 +17,7 @@
 //             written by the epilogue of its logits, and both gradients' products read
 //             it.  dx is summed over the pieces in float32.
 // Exponentials are base 2 of values scaled by log2 e in one fused multiply-add; sums
-// and maxima are float32, the join is double.
+// and maxima are float32, the last step from them to lse and loss is double.
 //
 // g enters the tensor cores in the activations' type, rounded once.  So that fp16 holds
 // it whatever the size of dloss, each token's g is divided by the power of two s_t
