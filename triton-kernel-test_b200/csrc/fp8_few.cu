@@ -3,17 +3,22 @@
 // the tensor cores' M.
 //
 // It cannot do without the weight's byte a value, read once.  The tiles of 256 x 256
-// (fp8_gemm.cu) would be mostly empty and too few to keep memory busy: 200 x 4096 x
-// 11008 has 43.  Here a CTA takes 128 rows of the weight against all tokens (the MMA's N is
-// their number rounded to 16), and the contraction is cut over a cluster of up
-// to eight CTAs, so that the device has two to four CTAs per SM; their sums meet in
-// shared memory, each CTA adding some of the tokens' columns in the order of the ranks.  Per CTA:
+// (fp8_gemm.cu) would be mostly empty and too few to keep memory busy.  Here a CTA takes
+// 128 rows of the weight against all tokens (the MMA's N is their number rounded to 16),
+// and the contraction is cut over a cluster of up to eight CTAs, so that the device has
+// two to four CTAs per SM; their sums meet in shared memory, each CTA adding some of the
+// tokens' columns in the order of the ranks.  Per CTA:
 //   warp 0      TMA producer: 128 rows x 128 of W, N x 128 of X a stage;
 //   warp 1      TMEM allocation, MMA issue;
 //   warps 2..5  scales from memory to TMEM, every lane quadrant the same (as in
 //               pair_gemm.cuh), then the sums.
-// Tokens on the M side, decoded codes on the warps' own matrix instruction, took 22 us
-// for one token (4096 x 11008): the instruction is made of conversions and 16-bit steps.
+// 4096 x 11008, us with the event's own 2.6: 1 token 17.5, 32 20.5, 128 27 (floor 6.9; the
+// same bytes read and dropped take 14.3); 11008 x 4096 18.5, 20.5, 27.6 (in 256 x 256 tiles
+// 44); 16384 x 16384 50 (41).  What holds it is the start, 4000 to 9000 cycles until the
+// first tile and its scales are there.  Other ways: tokens on the M side with the warps'
+// own 8-bit matrix instruction 20.5 (it is made of conversions and 16-bit steps: 242
+// instructions for 16 x 128 codes); parts of the tokens for more than 128, the weight read
+// again from L2, no better than the tiles.
 #include <algorithm>
 
 #include "pair_gemm.cuh"
@@ -272,16 +277,18 @@ int few_launch(const actcomp_fp8 *a, const actcomp_fp8 *b, const pair::Scales &s
     p.tmem_cols = p.N == 16 ? 128 : 256;  // four or two CTAs per SM
     const int stage = W_BYTES + p.N * 128, smem = few_smem(p.tmem_cols), sms = num_sms(), per_sm = 512 / p.tmem_cols;
     p.stages = (smem - 1024 - 512) / stage;
-    // Ranks by an estimate in blocks of 0.35 us: an SM's share of the CTAs at a CTA's blocks each, and 20 for every
-    // wave's start, first loads and sums.  us (a weight in memory) at 1 | 2 | 4 | 8 ranks: 11008 x 4096, 1 token
-    // 21.3 | 18.5 | 16.4 | 20.5, 64 tokens 22.5 | 24.5 | 30.7 | 36.9; 4096 x 11008, 1 token 38.8 | 26.5 | 20.5 | 18.5.
+    // Ranks by an estimate in blocks of 0.35 us: an SM's share of the CTAs at a CTA's blocks each, 20 for every wave's
+    // start and first loads, and the sums; the most ranks of equal ones (more loads are under way).  us (a weight in
+    // memory) at 1 | 2 | 4 | 8 ranks: 11008 x 4096, 1 token 21.3 | 18.5 | 16.4 | 20.5, 64 tokens 22.5 | 24.5 | 30.7 |
+    // 36.9; 4096 x 11008, 1 token 38.8 | 26.5 | 20.5 | 18.5.
     const int64_t units = (p.n + 127) / 128;
     int ranks = 1;
     int64_t best = INT64_MAX;
     for (int r = 1; r <= 8 && (r == 1 || p.kblocks >= 2 * r); r *= 2) {
         const int64_t ctas = units * r, blocks = (p.kblocks + r - 1) / r;
-        const int64_t cost = (ctas + sms - 1) / sms * blocks + 20 * ((ctas + sms * per_sm - 1) / (sms * per_sm));
-        if (cost < best) best = cost, ranks = r;
+        const int64_t cost = (ctas + sms - 1) / sms * blocks + 20 * ((ctas + sms * per_sm - 1) / (sms * per_sm)) +
+                             (r > 1 ? p.N / 32 : 0);
+        if (cost <= best) best = cost, ranks = r;
     }
     p.k_split = (p.kblocks + ranks - 1) / ranks;
     ACT_CHECK(units * ranks <= INT32_MAX, ACT_E_UNSUPPORTED);

@@ -9,6 +9,14 @@
 // converted from the same registers.  Codes stay in the matrix's own orientation (the
 // tensor cores take either operand with its rows contiguous), so no direction needs a
 // transposition, and the scales of a block row or column are 128 bytes in one piece.
+//
+// 16384 x 11008 on a B200, us and share of the copy rate:
+//             rows        columns     tiles       both        inverse
+//   bf16      99  83 %    86  96 %    84  98 %    152  73 %   90  92 %
+//   float32   150 92 %    138 100 %   134 100 %   192 86 %    180 76 %
+// Rows that are not 16-byte aligned go through shared memory, neighbouring lanes
+// neighbouring values (2050 x 1338 float32: the inverse 22 us value by value, 8.8 so).
+// Three CTAs per SM instead of four: rows 108, columns 95, both 162.
 #include "fp8.cuh"
 #include "mx4.cuh"
 #include "tc_ptx.cuh"
