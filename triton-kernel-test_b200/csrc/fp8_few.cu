@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
         // Columns first .. first + each - 1 are this rank's to add.  The sums go to their ranks' shared memory, over
         // the rings once every rank is done with its own: [rank][column][row].
         const int each = p.N / (int)ranks;
+        tc::drain_after_abort(abort);  // nothing lands in the rings any more
         __syncwarp();
         tc::cluster_sync();
         if (warp >= 2) {
@@ -252,6 +253,8 @@ __global__ void __launch_bounds__(FEW_THREADS)
     }
     tc::tc_fence_before();
     __syncthreads();
+    tc::drain_after_abort(abort);
+    __syncwarp();
     if (warp == 1) {
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem, p.tmem_cols);

@@ -425,6 +425,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     tc::tc_fence_before();
     __syncthreads();
+    tc::drain_after_abort(abort);
+    __syncwarp();
     tc::cluster_sync();  // neither CTA leaves while the other may still read its shared memory or signal it
     if (warp == 1) {
         tc::tc_fence_after();

@@ -217,6 +217,11 @@ __device__ __forceinline__ bool mbar_spin(uint64_t *bar, uint32_t parity, volati
     atomicOr(&g_device_error, DEV_ERR_MBAR_TIMEOUT);
     return false;
 }
+// A CTA that gives up leaves only after its copies and MMAs under way have landed: they
+// take microseconds, this 0.2 ms.  (No barrier tells it: what it waited for did not come.)
+__device__ __forceinline__ void drain_after_abort(volatile int *abort) {
+    for (int i = 0; i < 200 && *abort; ++i) __nanosleep(1000);
+}
 // One lane of the converged warp (the same each time).
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;

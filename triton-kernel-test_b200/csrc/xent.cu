@@ -209,8 +209,16 @@ struct SumEpi {
         float v[32];
         if (add) {
             const int n = p.N - col;
+            if (n >= 32) {  // rows of part are 16-byte aligned
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = i < n ? __ldcg(add + col + i) : 0.f;
+                for (int i = 0; i < 8; ++i) {
+                    const float4 q = __ldcg(reinterpret_cast<const float4 *>(add + col) + i);
+                    v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = i < n ? __ldcg(add + col + i) : 0.f;
+            }
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = (__uint_as_float(r[i]) + v[i]) * f;
         } else {
