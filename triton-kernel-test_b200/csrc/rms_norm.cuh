@@ -21,7 +21,7 @@
 // or ring slots hold are read twice.
 //
 // Measured on a B200, us (floor at the copy rate): 16384 x 4096 bf16
-//   forward 42 (41), with the residual 86 (82), 8-bit 58 (31), 8-bit with the residual
+//   forward 42 (41), with the residual 86 (82), 8-bit 57 (31), 8-bit with the residual
 //   77 (72), backward 67 (61), 84 with dh (82)
 // and float32 94 (82), 188 (164), 66 (51), 142 (133), 128 (123), 140 (164, where dh
 // was in L2).  The 8-bit form without a residual is held by its instructions (issue
@@ -217,13 +217,18 @@ __global__ void __launch_bounds__(MAXT, rms_ctas(NCH, MAXT))
     ring.init(dyn, mine, (int)a.cols, depth, leader);
     if (leader)
         for (int i = 0; i < depth; ++i) fill(i, r0 + i * step);
-    Raw8<W> wv[NCH];
+    // the 8-bit form, which its instructions hold, keeps the weight as float32
+    constexpr bool WIDE = Q && NCH <= 2;
+    Raw8<W> wv[WIDE ? 1 : NCH];
+    F8 wf[WIDE ? NCH : 1];
     int n[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int seg0 = (w0 + i * wpr) * SEG;
         n[i] = count_of<VEC>(seg0, a.cols, lane);
-        wv[i] = load8_or<W, VEC>(a.w, 1.f, seg0, n[i], lane);
+        const Raw8<W> raw = load8_or<W, VEC>(a.w, 1.f, seg0, n[i], lane);
+        if constexpr (WIDE) wf[i] = unpack<W>(raw);
+        else wv[i] = raw;
     }
     int turn = 0;
     for (int64_t r = r0; r < a.rows; r += R * step, ++turn) {
@@ -271,8 +276,13 @@ __global__ void __launch_bounds__(MAXT, rms_ctas(NCH, MAXT))
 #pragma unroll
             for (int i = 0; i < NCH; ++i) {
                 const int seg0 = (w0 + i * wpr) * SEG;
-                stay_packed(wv[i]);
-                const F8 w = unpack<W>(wv[i]);
+                F8 w;
+                if constexpr (WIDE) {
+                    w = wf[i];
+                } else {
+                    stay_packed(wv[i]);
+                    w = unpack<W>(wv[i]);
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[k][i].p[j] = mul2(mul2(v[k][i].p[j], rstd2), w.p[j]);
                 if constexpr (Q)
