@@ -12,6 +12,9 @@ hardware's exponential is within 2^-22, and a sum's terms are added in chains of
   dW    the same over tokens; x's scaled copy is exact in bf16, and in fp16 within 2^-24
         of the largest factor for each token."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -128,6 +131,21 @@ def test_entry_points_validate_without_gpu():
         assert b(**bad) == I, bad
     assert b(dx=P + 1) == A and b(dlse=P + 2) == A and b(n=wsb - 1) == _lib.ACT_E_WORKSPACE
     assert b(ws=P + 128) == _lib.ACT_E_WORKSPACE and b(a=dict(lse=None)) == I
+
+
+def test_pieces_larger_than_the_vocabulary():
+    """Any piece above the vocabulary is the whole of it, up to the largest integer (in
+    its own process: a division by zero ends one)."""
+    code = ("from actcomp import _lib\nf = _lib.load().actcomp_xent_bwd_workspace\n"
+            "for tokens, channels, vocab in ((100, 512, 16000), (1, 8, 1), (8, 64, 256)):\n"
+            "    whole = f(tokens, channels, vocab, (vocab + 255) // 256 * 256)\n"
+            "    for piece in (vocab + 256, 2 ** 31, 2 ** 62, 2 ** 63 - 512, 2 ** 63 - 1):\n"
+            "        assert f(tokens, channels, vocab, piece) == whole > 0, (vocab, piece)\n")
+    import actcomp
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(actcomp.__file__)))
+    env = dict(os.environ, PYTHONPATH=root + os.pathsep + os.environ.get("PYTHONPATH", ""))
+    subprocess.run([sys.executable, "-c", code], check=True, env=env, timeout=300)
 
 
 def test_struct_layouts_match_the_header():

@@ -418,7 +418,8 @@ static bool tma_rows(const void *p, int64_t ld, int es) { return aligned(p, 16) 
 static int64_t piece_of(int64_t tokens, int64_t vocab, int64_t asked) {
     int64_t most = asked > 0 ? asked : ((int64_t)1 << 29) / (tokens > 0 ? tokens : 1);
     if (!asked && most < 4096) most = 4096;
-    most = most / pair::BN * pair::BN;
+    const int64_t whole = (vocab + pair::BN - 1) / pair::BN * pair::BN;
+    most = most < whole ? most / pair::BN * pair::BN : whole;  // any number above the vocabulary is all of it
     if (most < pair::BN) most = pair::BN;
     const int64_t pieces = (vocab + most - 1) / most;
     return ((vocab + pieces - 1) / pieces + pair::BN - 1) / pair::BN * pair::BN;
